@@ -23,6 +23,11 @@ int sm_count();
 int encode_tmap(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,
                 const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swizzle);
 
+// TMA descriptor of one attention operand, [batch][head][row][D] with the given element strides, boxes of
+// 64 channels x box_rows rows (128-byte swizzle; attention.cu).
+int make_attn_map(CUtensorMap* map, const void* base, int dtype, int D, int64_t rows, int heads, int64_t batch,
+                  int64_t row_stride, int64_t head_stride, int64_t batch_stride, int box_rows);
+
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

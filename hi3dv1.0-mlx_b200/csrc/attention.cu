@@ -85,6 +85,12 @@ struct Params {
   // folds the partials of slots [0, slot0) into its own result (merge_kernel's
   // arithmetic, slots in order with this range last) and writes the final rows to `out`.
   int merge_final;
+  // LSE instantiations only (hi3d_flash_attn_fwd_lse): natural log-sum-exp of the scaled
+  // scores at lse[b * lse_batch + h * nq + row] (row = packed row when varlen, b = 0), and
+  // query heads h, h + 1, .. of one group read key head h / kv_group.
+  float* lse;
+  int64_t lse_batch;
+  int kv_group;
 };
 
 // out row (b, qrow, h) of the final result
@@ -98,6 +104,12 @@ __device__ __forceinline__ float slot_lse(const Params& p, int s, int64_t prow, 
   return p.part_lse[((int64_t)s * p.part_rows + prow) * p.heads + h];
 }
 
+constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ int64_t lse_index(const Params& p, int b, int64_t q_start, int64_t qrow, int h) {
+  return (int64_t)(p.cu_q ? 0 : b) * p.lse_batch + (int64_t)h * p.nq + q_start + qrow;
+}
+
 struct Barriers {
   uint64_t q_full;
   uint64_t k_full[4];
@@ -107,6 +119,7 @@ struct Barriers {
   uint64_t s_free[2];  // the tile's softmax has read its scores into registers
   uint64_t p_full[2];
   uint64_t o_done[2];
+  uint64_t v_tail;  // LSE: values of a ragged last block, before its rows past the end are cleared
   uint32_t tmem_base;
   int abort;
 };
@@ -114,7 +127,11 @@ struct Barriers {
 // PARTIAL: key-split launch writing partial O / l and log2-sum-exp (Params::part_o);
 // otherwise one pass over all keys writing `out`.  Two instantiations keep the
 // single-pass kernel free of the split bookkeeping.
-template <typename T, int D, bool PARTIAL>
+// LSE: the form that the backward pass builds on.  It also writes each row's log-sum-exp,
+// gives rows without keys an output of 0 and a log-sum-exp of -inf, takes grouped key heads,
+// and clears the value rows past a ragged sequence's end in shared memory: they belong to the
+// next sequence, and a NaN or infinity there times P = 0 would not be 0.
+template <typename T, int D, bool PARTIAL, bool LSE = false>
 __global__ void __launch_bounds__(kThreads, 1)
     flash_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const Params p) {
@@ -144,6 +161,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     k_start = p.cu_k[b];
     k_len = p.cu_k[b + 1] - k_start;
     bk = 0;
+  }
+  int hk = h;
+  if constexpr (LSE) {
+    hk = h / p.kv_group;
+    clamp_range(q_start, q_len, p.nq);
+    clamp_range(k_start, k_len, p.nk);
   }
   const int64_t q_row0 = (int64_t)t * 2 * kRowsPerTile;
   if (q_row0 >= q_len) return;  // uniform across the CTA
@@ -197,7 +220,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     k_start += (int64_t)kb0 * C::BK;
     k_len -= (int64_t)kb0 * C::BK;
   } else {
-    if (k_len <= 0) return;
+    if (k_len <= 0) {
+      if constexpr (LSE) {
+        for (int e = threadIdx.x; e < 2 * kRowsPerTile * (D / 8); e += blockDim.x) {
+          const int64_t qr = q_row0 + e / (D / 8);
+          if (qr >= q_len) continue;
+          *reinterpret_cast<uint4*>(out_row<T>(p, b, q_start, qr, h) + e % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
+          if (e % (D / 8) == 0) p.lse[lse_index(p, b, q_start, qr, h)] = -INFINITY;
+        }
+      }
+      return;
+    }
     nblk = (int)((k_len + C::BK - 1) / C::BK);
   }
 
@@ -215,6 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bar->p_full[i], kRowsPerTile);
       mbar_init(&bar->o_done[i], 1);
     }
+    if constexpr (LSE) mbar_init(&bar->v_tail, 1);
     bar->abort = 0;
     fence_barrier_init();
   }
@@ -230,6 +264,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
+    int tail_block = -1;  // LSE: the block whose values need clearing past the sequence's end
+    int tail_rows = 0;
+    int tail_issued = 0;
+    if constexpr (LSE) {
+      const int64_t last = k_len - (int64_t)(nblk - 1) * C::BK;
+      if (p.cu_k && last < C::BK) tail_block = nblk - 1, tail_rows = (int)last;
+    }
     if (lane == 0) {
       tma_prefetch_desc(&tmQ);
       tma_prefetch_desc(&tmK);
@@ -246,12 +287,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int krow = (int)(k_start + (int64_t)j * C::BK);
         mbar_arrive_expect_tx(&bar->k_full[s], C::KV_STAGE);
         for (int c = 0; c < C::NCH; ++c)
-          tma_load_4d(sK + s * C::KV_STAGE + c * C::KV_CHUNK, &tmK, &bar->k_full[s], c * 64, krow, h, bk);
-        mbar_arrive_expect_tx(&bar->v_full[s], C::KV_STAGE);
+          tma_load_4d(sK + s * C::KV_STAGE + c * C::KV_CHUNK, &tmK, &bar->k_full[s], c * 64, krow, hk, bk);
+        uint64_t* vbar = LSE && j == tail_block ? &bar->v_tail : &bar->v_full[s];
+        mbar_arrive_expect_tx(vbar, C::KV_STAGE);
         for (int c = 0; c < C::NCH; ++c)
-          tma_load_4d(sV + s * C::KV_STAGE + c * C::KV_CHUNK, &tmV, &bar->v_full[s], c * 64, krow, h, bk);
+          tma_load_4d(sV + s * C::KV_STAGE + c * C::KV_CHUNK, &tmV, vbar, c * 64, krow, hk, bk);
         issued = j + 1;
       }
+      if (LSE && tail_block >= 0) tail_issued = issued == nblk;
       if (*abort) {
         // Drain: let every copy already issued land before the CTA exits.
         mbar_wait(&bar->q_full, 0, abort, 2);
@@ -259,8 +302,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int s = j % C::NST, n = j / C::NST;
           volatile int no_abort = 0;
           mbar_wait(&bar->k_full[s], n & 1, &no_abort, 3);
-          mbar_wait(&bar->v_full[s], n & 1, &no_abort, 3);
+          if (!(LSE && j == tail_block)) mbar_wait(&bar->v_full[s], n & 1, &no_abort, 3);
         }
+      }
+    }
+    if constexpr (LSE) {
+      if (__shfl_sync(0xffffffffu, tail_issued, 0)) {  // the last copy: cleared by the warp, then published
+        uint8_t* v = sV + (tail_block % C::NST) * C::KV_STAGE;
+        volatile int no_abort = 0;
+        mbar_wait(&bar->v_tail, 0, &no_abort, 4);
+        for (int c = 0; c < C::NCH; ++c)
+          for (int e = tail_rows * 8 + lane; e < C::BK * 8; e += 32)
+            *reinterpret_cast<uint4*>(v + c * C::KV_CHUNK + e * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar->v_full[tail_block % C::NST]);
       }
     }
   } else if (warp == 1 || warp == 10) {
@@ -508,6 +564,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         }
       } else {
+        if constexpr (LSE) {
+          if (qrow < q_len) p.lse[lse_index(p, b, q_start, qrow, h)] = (m_run + log2f(l_run)) * kLn2;
+        }
         T* dst = reinterpret_cast<T*>(p.out) + (int64_t)(p.cu_q ? 0 : b) * p.o_batch + (q_start + qrow) * p.o_row +
                  (int64_t)h * p.o_head;
 #pragma unroll
@@ -543,11 +602,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Combines the key-split partials of one (row, head) per warp:
 // out = sum_s 2^(lse_s - max) O_s / sum_s 2^(lse_s - max), rounded once.  Rows
 // whose splits all saw no keys are left untouched, as in the single-pass kernel.
-template <typename T, int D>
+// LSE: those rows get 0 and -inf instead, and every row its natural log-sum-exp, at
+// lse[batch][head][row] with nq rows per head.
+template <typename T, int D, bool LSE = false>
 __global__ void __launch_bounds__(256) merge_kernel(const float* __restrict__ part_o,
                                                     const float* __restrict__ part_lse, T* __restrict__ out,
                                                     int64_t rows, int heads, int splits, int64_t nq, int dense,
-                                                    int64_t o_row, int64_t o_head, int64_t o_batch) {
+                                                    int64_t o_row, int64_t o_head, int64_t o_batch,
+                                                    float* __restrict__ lse = nullptr) {
   constexpr int E = D / 32;  // elements per lane
   const int64_t wid = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
@@ -556,7 +618,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const float* __restrict__ pa
   const int h = (int)(wid - r * heads);
   float mx = -INFINITY;
   for (int s = 0; s < splits; ++s) mx = fmaxf(mx, part_lse[((int64_t)s * rows + r) * heads + h]);
-  if (mx == -INFINITY) return;
+  if (mx == -INFINITY && !LSE) return;
   float acc[E] = {};
   float wsum = 0.f;
   for (int s = 0; s < splits; ++s) {
@@ -568,16 +630,20 @@ __global__ void __launch_bounds__(256) merge_kernel(const float* __restrict__ pa
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] += wgt * po[e];
   }
-  const float inv = 1.0f / wsum;
+  const float inv = LSE && mx == -INFINITY ? 0.0f : 1.0f / wsum;
   const int64_t b = dense ? r / nq : 0, qr = dense ? r - b * nq : r;
   T* dst = out + b * o_batch + qr * o_row + (int64_t)h * o_head + lane * E;
 #pragma unroll
   for (int e = 0; e < E; ++e) dst[e] = Cvt<T>::from_f(acc[e] * inv);
+  if constexpr (LSE) {
+    if (lane == 0)
+      lse[(b * heads + h) * nq + qr] = mx == -INFINITY ? -INFINITY : (mx + log2f(wsum)) * kLn2;
+  }
 }
 
 }  // namespace attn
 
-static int make_attn_map(CUtensorMap* map, const void* base, int dtype, int D, int64_t rows, int heads,
+int make_attn_map(CUtensorMap* map, const void* base, int dtype, int D, int64_t rows, int heads,
                          int64_t batch, int64_t row_stride, int64_t head_stride, int64_t batch_stride, int box_rows) {
   const uint64_t esz = 2;
   uint64_t dims[4] = {(uint64_t)D, (uint64_t)rows, (uint64_t)heads, (uint64_t)batch};
@@ -590,9 +656,10 @@ static int make_attn_map(CUtensorMap* map, const void* base, int dtype, int D, i
 
 // Single pass (part_o == nullptr) or partial results of k_splits key ranges into
 // slots [slot0, slot0 + k_splits) of part_o / part_lse (no merge).
-template <typename T, int D>
+template <typename T, int D, bool LSE = false>
 static int launch_attn(const hi3d_attn_args* a, cudaStream_t st, int k_splits = 1, float* part_o = nullptr,
-                       float* part_lse = nullptr, int slot0 = 0, bool merge_final = false) {
+                       float* part_lse = nullptr, int slot0 = 0, bool merge_final = false, int kv_heads = 0,
+                       float* lse = nullptr) {
   using C = attn::Cfg<D>;
   const bool varlen_q = a->cu_seqlens_q != nullptr, varlen_k = a->cu_seqlens_k != nullptr;
   const int64_t qb = varlen_q ? 1 : a->num_seqs;
@@ -602,9 +669,9 @@ static int launch_attn(const hi3d_attn_args* a, cudaStream_t st, int k_splits = 
   if ((rc = make_attn_map(&mq, a->q, a->dtype, D, a->nq, a->heads, qb, a->q_row, a->q_head, a->q_batch,
                           attn::kRowsPerTile)))
     return rc;
-  if ((rc = make_attn_map(&mk, a->k, a->dtype, D, a->nk, a->heads, kb, a->k_row, a->k_head, a->k_batch, C::BK)))
+  if ((rc = make_attn_map(&mk, a->k, a->dtype, D, a->nk, kv_heads ? kv_heads : a->heads, kb, a->k_row, a->k_head, a->k_batch, C::BK)))
     return rc;
-  if ((rc = make_attn_map(&mv, a->v, a->dtype, D, a->nk, a->heads, kb, a->v_row, a->v_head, a->v_batch, C::BK)))
+  if ((rc = make_attn_map(&mv, a->v, a->dtype, D, a->nk, kv_heads ? kv_heads : a->heads, kb, a->v_row, a->v_head, a->v_batch, C::BK)))
     return rc;
   attn::Params p;
   p.out = a->out;
@@ -627,26 +694,29 @@ static int launch_attn(const hi3d_attn_args* a, cudaStream_t st, int k_splits = 
   p.part_lse = part_lse;
   p.part_rows = varlen_q ? a->nq : (int64_t)a->num_seqs * a->nq;
   p.merge_final = merge_final ? 1 : 0;
+  p.lse = lse;
+  p.lse_batch = (int64_t)a->heads * a->nq;
+  p.kv_group = kv_heads ? a->heads / kv_heads : 1;
   const int64_t grid = (int64_t)p.tiles_per_seq * a->num_seqs * a->heads * k_splits;
   if (grid == 0) return HI3D_OK;
   if (grid > 0x7fffffff) return set_error(HI3D_ERR_INVALID_ARGUMENT, "flash_attn: too many tiles");
-  auto kern = part_o ? attn::flash_fwd_kernel<T, D, true> : attn::flash_fwd_kernel<T, D, false>;
+  auto kern = part_o ? attn::flash_fwd_kernel<T, D, true, LSE> : attn::flash_fwd_kernel<T, D, false, LSE>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return set_error(HI3D_ERR_CUDA, "flash_attn: smem attribute: %s", cudaGetErrorString(e));
   kern<<<(unsigned)grid, attn::kThreads, C::SMEM, st>>>(mq, mk, mv, p);
   return check_launch("flash_attn_fwd");
 }
 
-template <typename T, int D>
+template <typename T, int D, bool LSE = false>
 static int launch_merge(const hi3d_attn_args* a, cudaStream_t st, int num_slots, const float* part_o,
-                        const float* part_lse) {
+                        const float* part_lse, float* lse = nullptr) {
   const bool varlen_q = a->cu_seqlens_q != nullptr;
   const int64_t rows = varlen_q ? a->nq : (int64_t)a->num_seqs * a->nq;
   const int64_t warps = rows * a->heads;
   if (warps == 0) return HI3D_OK;
-  attn::merge_kernel<T, D><<<(unsigned)((warps + 7) / 8), 256, 0, st>>>(
+  attn::merge_kernel<T, D, LSE><<<(unsigned)((warps + 7) / 8), 256, 0, st>>>(
       part_o, part_lse, static_cast<T*>(a->out), rows, a->heads, num_slots, a->nq, varlen_q ? 0 : 1, a->o_row,
-      a->o_head, a->o_batch);
+      a->o_head, a->o_batch, lse);
   return check_launch("flash_attn_merge");
 }
 
@@ -694,6 +764,25 @@ static int dispatch_merge(const hi3d_attn_args* a, cudaStream_t st, int num_slot
     case 64: return launch_merge<T, 64>(a, st, num_slots, part_o, part_lse);
     case 96: return launch_merge<T, 96>(a, st, num_slots, part_o, part_lse);
     default: return launch_merge<T, 128>(a, st, num_slots, part_o, part_lse);
+  }
+}
+
+template <typename T, int D>
+static int run_lse(const hi3d_attn_args* a, int kv_heads, float* lse, int k_splits, float* part_o, float* part_lse,
+                   cudaStream_t st) {
+  if (k_splits == 1)
+    return launch_attn<T, D, true>(a, st, 1, nullptr, nullptr, 0, false, kv_heads, lse);
+  int rc = launch_attn<T, D, true>(a, st, k_splits, part_o, part_lse, 0, false, kv_heads, lse);
+  return rc ? rc : launch_merge<T, D, true>(a, st, k_splits, part_o, part_lse, lse);
+}
+
+template <typename T>
+static int dispatch_lse(const hi3d_attn_args* a, int kv_heads, float* lse, int k_splits, float* part_o,
+                        float* part_lse, cudaStream_t st) {
+  switch (a->head_dim) {
+    case 64: return run_lse<T, 64>(a, kv_heads, lse, k_splits, part_o, part_lse, st);
+    case 96: return run_lse<T, 96>(a, kv_heads, lse, k_splits, part_o, part_lse, st);
+    default: return run_lse<T, 128>(a, kv_heads, lse, k_splits, part_o, part_lse, st);
   }
 }
 
@@ -791,4 +880,27 @@ extern "C" int hi3d_flash_attn_merge(const hi3d_attn_args* a, int num_slots, con
   cudaStream_t st = as_stream(stream);
   return a->dtype == HI3D_BF16 ? dispatch_merge<__nv_bfloat16>(a, st, num_slots, part_o, part_lse)
                                : dispatch_merge<__half>(a, st, num_slots, part_o, part_lse);
+}
+
+extern "C" int hi3d_flash_attn_fwd_lse(const hi3d_attn_args* a, int kv_heads, float* lse, int k_splits,
+                                       void* workspace, int64_t workspace_bytes, void* stream) {
+  int64_t need = 0;
+  int rc = hi3d_flash_attn_split_workspace_size(a, k_splits, &need);
+  if (rc) return rc;
+  if (kv_heads < 1 || a->heads % kv_heads)
+    return set_error(HI3D_ERR_INVALID_ARGUMENT, "flash_attn_fwd_lse: %d key heads do not divide %d query heads",
+                     kv_heads, a->heads);
+  if (!lse) return set_error(HI3D_ERR_INVALID_ARGUMENT, "flash_attn_fwd_lse: null lse");
+  if (a->nk == 0) return set_error(HI3D_ERR_INVALID_ARGUMENT, "flash_attn_fwd_lse: no keys");
+  if (a->nq == 0 || a->num_seqs == 0) return HI3D_OK;
+  if (k_splits > 1 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
+    return set_error(HI3D_ERR_CAPACITY, "flash_attn_fwd_lse: workspace %lld bytes, need %lld (16-byte aligned)",
+                     (long long)workspace_bytes, (long long)need);
+  float* part_o = static_cast<float*>(workspace);
+  float* part_lse = k_splits == 1 ? nullptr
+                                  : reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
+                                                             ((split_part_bytes(a, k_splits) + 255) & ~int64_t(255)));
+  cudaStream_t st = as_stream(stream);
+  return a->dtype == HI3D_BF16 ? dispatch_lse<__nv_bfloat16>(a, kv_heads, lse, k_splits, part_o, part_lse, st)
+                               : dispatch_lse<__half>(a, kv_heads, lse, k_splits, part_o, part_lse, st);
 }

@@ -193,6 +193,26 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
+// Untiled bulk copy of `bytes` (a multiple of 16, both addresses 16-byte aligned).
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// Orders this thread's earlier shared-memory writes before later reads by the tensor core.
+__device__ __forceinline__ void fence_proxy_async() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// [start, start + len) cut to the rows [0, rows) that exist.
+__device__ __forceinline__ void clamp_range(int64_t& start, int64_t& len, int64_t rows) {
+  const int64_t lo = min(max(start, (int64_t)0), rows), hi = min(max(start + len, lo), rows);
+  start = lo;
+  len = hi - lo;
+}
+
 // ---------------------------------------------------------------------------
 // CTA pairs (clusters of two CTAs sharing cta_group::2 MMAs)
 // ---------------------------------------------------------------------------

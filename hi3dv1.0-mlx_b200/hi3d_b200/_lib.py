@@ -50,6 +50,17 @@ class AttnArgs(ctypes.Structure):
     ]
 
 
+class AttnBwdArgs(ctypes.Structure):
+    """Mirror of ``hi3d_attn_bwd_args``."""
+
+    _fields_ = [(n, _c_void_p) for n in ("q", "k", "v", "out", "dout", "lse", "dq", "dk", "dv")]
+    _fields_ += [(f"{t}_{s}", _i64) for t in ("q", "k", "v", "o", "do", "dq", "dk", "dv")
+                 for s in ("row", "head", "batch")]
+    _fields_ += [("cu_seqlens_q", _c_void_p), ("cu_seqlens_k", _c_void_p), ("nq", _i64), ("nk", _i64),
+                 ("num_seqs", _i32), ("heads", _i32), ("kv_heads", _i32), ("head_dim", _i32), ("dtype", _i32),
+                 ("scale", _f32)]
+
+
 # name -> (restype, argtypes); every entry of include/hi3d_b200.h
 SIGNATURES: dict[str, tuple] = {
     "hi3d_version": (_i32, []),
@@ -72,6 +83,9 @@ SIGNATURES: dict[str, tuple] = {
     "hi3d_flash_attn_fwd_partial_merge": (_i32, [ctypes.POINTER(AttnArgs), _i32, _c_void_p, _c_void_p, _i64,
                                                  _c_void_p]),
     "hi3d_flash_attn_merge": (_i32, [ctypes.POINTER(AttnArgs), _i32, _c_void_p, _c_void_p, _c_void_p]),
+    "hi3d_flash_attn_fwd_lse": (_i32, [ctypes.POINTER(AttnArgs), _i32, _c_void_p, _i32, _c_void_p, _i64, _c_void_p]),
+    "hi3d_flash_attn_bwd_workspace_size": (_i32, [ctypes.POINTER(AttnBwdArgs), ctypes.POINTER(_i64)]),
+    "hi3d_flash_attn_bwd": (_i32, [ctypes.POINTER(AttnBwdArgs), _c_void_p, _i64, _c_void_p]),
     "hi3d_nccl_unique_id": (_i32, [_c_void_p]),
     "hi3d_nccl_comm_init": (_i32, [_c_void_p, _i32, _i32, ctypes.POINTER(_c_void_p)]),
     "hi3d_nccl_comm_destroy": (_i32, [_c_void_p]),

@@ -5,6 +5,10 @@
 :func:`flash_attn_varlen` is the packed variable-length form the upstream
 ``flash_attn`` API needs (src/sparc3d/nn/sparse/attention/full_attn.py:56-76).
 
+:func:`flash_attention_lse` / :func:`flash_attention_backward` and their ``flash_attn_varlen_*``
+forms are the training pair (the reference runs forward only); :mod:`hi3d_b200.training` joins
+them for autograd.
+
 Arithmetic (as the reference kernel, attention.py:19-22): ``S = Q K^T`` in fp32,
 online softmax in fp32 in the exp2 domain, ``P`` rounded to the input dtype for
 ``P V`` which accumulates in fp32, output ``O / l`` rounded once.
@@ -308,3 +312,250 @@ def flash_attn_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
         dtype=_lib.dtype_code(q), scale=float(scale))
     _launch(args, q, k_splits)
     return out
+
+
+# ---------------------------------------------------------------------------
+# training: the forward pass with its log-sum-exp, and the gradients
+# ---------------------------------------------------------------------------
+def _aligned(t: torch.Tensor) -> bool:
+    """Whether the kernels' 16-byte loads and TMA boxes can address ``t`` as it lies."""
+    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+            and all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1])))
+
+
+def _fit(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself, or a contiguous copy where its strides or address do not fit the kernels
+    (an expanded gradient, an odd slice)."""
+    if _aligned(t):
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _steps(t: torch.Tensor, order: tuple[int, ...]) -> list[int]:
+    """Element strides of the (row, head[, batch]) axes ``order``.  An axis of one element may have
+    any stride, which the kernels would refuse: a row or head then steps by one head, a batch by 0
+    (one set for every sequence)."""
+    return [t.stride(i) if t.shape[i] != 1 else 0 if n == 2 else t.shape[-1] for n, i in enumerate(order)]
+
+
+def _check_train(q, k, v, heads: int, kv_heads: int, dim: int, same_kv: bool) -> None:
+    if dim not in SUPPORTED_HEAD_DIMS:
+        raise NotImplementedError(f"head_dim {dim} not supported {SUPPORTED_HEAD_DIMS}")
+    if not same_kv or kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError(f"unsupported shapes q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)}")
+    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("flash attention takes float16 or bfloat16 inputs of one dtype")
+    if k.device != q.device or v.device != q.device:
+        raise ValueError("q, k and v must be on one device")
+
+
+def _dense_shape(q, k, v, q_layout: str) -> tuple[int, int, int, int]:
+    if q_layout not in ("bhnd", "bnhd"):
+        raise ValueError(f"unknown q layout {q_layout!r}")
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError(f"unsupported shapes q {tuple(q.shape)} k {tuple(k.shape)}")
+    batch, heads, nq, dim = q.shape if q_layout == "bhnd" else (q.shape[0], q.shape[2], q.shape[1], q.shape[3])
+    _check_train(q, k, v, heads, k.shape[1], dim,
+                 k.shape == v.shape and k.shape[3] == dim and k.shape[0] in (1, batch))
+    return batch, heads, nq, dim
+
+
+def _cu(cu: torch.Tensor | None, like: torch.Tensor, name: str) -> torch.Tensor | None:
+    if cu is None:
+        return None
+    if cu.dim() != 1 or cu.numel() < 1 or cu.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must be a one-dimensional int32 (or int64) tensor of num_seqs + 1 offsets")
+    if cu.device != like.device:
+        raise ValueError(f"{name} must be on the device of q")
+    return cu.to(torch.int32).contiguous()
+
+
+def _forward_lse(args: _lib.AttnArgs, kv_heads: int, lse: torch.Tensor, k_splits) -> None:
+    splits = _resolve_splits(k_splits, args, lse)
+    lib = _lib.load()
+    ws = None
+    if splits > 1:
+        nbytes = ctypes.c_int64()
+        _lib.check(lib.hi3d_flash_attn_split_workspace_size(ctypes.byref(args), splits, ctypes.byref(nbytes)),
+                   "flash_attention split workspace", launched=False)
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=lse.device)
+    rc = lib.hi3d_flash_attn_fwd_lse(ctypes.byref(args), kv_heads, lse.data_ptr(), splits, _lib.ptr(ws),
+                                     0 if ws is None else ws.numel(), _lib.stream(lse))
+    _lib.check(rc, "flash_attention_lse")
+
+
+def flash_attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, q_layout: str = "bhnd",
+                        k_splits: int | str = "auto") -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`flash_attention` for training: ``(out [B, Nq, H * D], lse [B, H, Nq])`` with the fp32
+    log-sum-exp of each row's scaled scores, which :func:`flash_attention_backward` takes.
+
+    ``k, v`` ``[B or 1, Hk, Nk, D]`` with ``Hk`` dividing ``H``: query head ``h`` reads key head
+    ``h // (H // Hk)``.  Without keys (``Nk = 0``) the output is 0 and ``lse`` is ``-inf``.
+    """
+    _lib.require_cuda(q, k, v)
+    batch, heads, nq, dim = _dense_shape(q, k, v, q_layout)
+    with torch.cuda.device(q.device):
+        if k.shape[2] == 0:
+            return (torch.zeros((batch, nq, heads * dim), dtype=q.dtype, device=q.device),
+                    torch.full((batch, heads, nq), -math.inf, device=q.device))
+        out = torch.empty((batch, nq, heads * dim), dtype=q.dtype, device=q.device)
+        lse = torch.empty((batch, heads, nq), dtype=torch.float32, device=q.device)
+        if nq == 0 or batch == 0:
+            return out, lse
+        q, k, v = _fit(q), _fit(k), _fit(v)
+        qr, qh, qb = _steps(q, (2, 1, 0) if q_layout == "bhnd" else (1, 2, 0))
+        kr, kh, kb = _steps(k, (2, 1, 0))
+        vr, vh, vb = _steps(v, (2, 1, 0))
+        args = _lib.AttnArgs(
+            q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(),
+            q_row=qr, q_head=qh, q_batch=qb, k_row=kr, k_head=kh, k_batch=kb, v_row=vr, v_head=vh, v_batch=vb,
+            o_row=heads * dim, o_head=dim, o_batch=nq * heads * dim, nq=nq, nk=k.shape[2], max_seqlen_q=nq,
+            num_seqs=batch, heads=heads, head_dim=dim, dtype=_lib.dtype_code(q), scale=float(scale))
+        _forward_lse(args, k.shape[1], lse, k_splits)
+    return out, lse
+
+
+def flash_attn_varlen_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                          cu_seqlens_k: torch.Tensor | None, max_seqlen_q: int, scale: float,
+                          k_splits: int | str = "auto") -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`flash_attn_varlen` for training: ``(out [Tq, H, D], lse [H, Tq])``.
+
+    ``k, v`` ``[Tk, Hk, D]`` with ``Hk`` dividing ``H``.  A sequence without keys gets an output of 0
+    and ``lse = -inf``.  Sequences never see each other's rows, NaN and infinities included.  The
+    offsets must cover all rows of ``q``.
+    """
+    _lib.require_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k)
+    cu_q, cu_k, heads, dim = _varlen_shape(q, k, v, cu_seqlens_q, cu_seqlens_k)
+    tq, tk = q.shape[0], k.shape[0]
+    with torch.cuda.device(q.device):
+        if tk == 0:
+            return (torch.zeros((tq, heads, dim), dtype=q.dtype, device=q.device),
+                    torch.full((heads, tq), -math.inf, device=q.device))
+        out = torch.empty((tq, heads, dim), dtype=q.dtype, device=q.device)
+        lse = torch.empty((heads, tq), dtype=torch.float32, device=q.device)
+        num_seqs = cu_q.numel() - 1
+        if tq == 0 or num_seqs == 0:
+            return out, lse
+        if int(max_seqlen_q) < 1:
+            raise ValueError("max_seqlen_q must be at least the longest query sequence")
+        q, k, v = _fit(q), _fit(k), _fit(v)
+        (qr, qh), (kr, kh), (vr, vh) = (_steps(t, (0, 1)) for t in (q, k, v))
+        args = _lib.AttnArgs(
+            q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(),
+            q_row=qr, q_head=qh, k_row=kr, k_head=kh, v_row=vr, v_head=vh, o_row=heads * dim, o_head=dim,
+            cu_seqlens_q=cu_q.data_ptr(), cu_seqlens_k=_lib.ptr(cu_k), nq=tq, nk=tk,
+            max_seqlen_q=min(int(max_seqlen_q), tq), num_seqs=num_seqs, heads=heads, head_dim=dim,
+            dtype=_lib.dtype_code(q), scale=float(scale))
+        _forward_lse(args, k.shape[1], lse, k_splits)
+    return out, lse
+
+
+def _varlen_shape(q, k, v, cu_seqlens_q, cu_seqlens_k):
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError(f"unsupported shapes q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)}")
+    _, heads, dim = q.shape
+    _check_train(q, k, v, heads, k.shape[1], dim, k.shape == v.shape and k.shape[2] == dim)
+    cu_q, cu_k = _cu(cu_seqlens_q, q, "cu_seqlens_q"), _cu(cu_seqlens_k, q, "cu_seqlens_k")
+    if cu_k is not None and cu_k.numel() != cu_q.numel():
+        raise ValueError("cu_seqlens_q and cu_seqlens_k must have the same length")
+    return cu_q, cu_k, heads, dim
+
+
+def _grads(out, like) -> list[torch.Tensor]:
+    """The gradients' tensors: the caller's, checked, or new contiguous ones."""
+    got = []
+    for name, given, t in zip(("dq", "dk", "dv"), out or (None, None, None), like):
+        if given is None:
+            given = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        elif given.shape != t.shape or given.dtype != t.dtype or given.device != t.device or not _aligned(given):
+            raise ValueError(f"{name} must have the shape, dtype and device of its input, rows contiguous over the "
+                             "head dimension and 16-byte aligned")
+        got.append(given)
+    return got
+
+
+def _backward(grad_out, q, k, v, out, lse, grads, strides, **sizes) -> None:
+    args = _lib.AttnBwdArgs(dtype=_lib.dtype_code(q), **sizes)
+    for name, t in zip(("q", "k", "v", "out", "dout", "lse", "dq", "dk", "dv"),
+                       (q, k, v, out, grad_out, lse, *grads)):
+        setattr(args, name, t.data_ptr())
+    for name, (row, head, batch) in strides.items():
+        setattr(args, f"{name}_row", row)
+        setattr(args, f"{name}_head", head)
+        setattr(args, f"{name}_batch", batch)
+    lib = _lib.load()
+    nbytes = ctypes.c_int64()
+    _lib.check(lib.hi3d_flash_attn_bwd_workspace_size(ctypes.byref(args), ctypes.byref(nbytes)),
+               "flash_attention_backward workspace", launched=False)
+    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=q.device)
+    rc = lib.hi3d_flash_attn_bwd(ctypes.byref(args), ws.data_ptr(), ws.numel(), _lib.stream(q))
+    _lib.check(rc, "flash_attention_backward")
+
+
+def _check_saved(grad_out, out, lse, q, out_shape, lse_shape) -> None:
+    for name, t in (("grad_out", grad_out), ("out", out)):
+        if tuple(t.shape) != out_shape or t.dtype != q.dtype or t.device != q.device:
+            raise ValueError(f"{name} must be {out_shape} in the dtype and on the device of q, got {tuple(t.shape)}")
+    if tuple(lse.shape) != lse_shape or lse.dtype != torch.float32 or lse.device != q.device:
+        raise ValueError(f"lse must be the float32 {lse_shape} of the forward pass, got {tuple(lse.shape)}")
+
+
+def flash_attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                             out: torch.Tensor, lse: torch.Tensor, scale: float, q_layout: str = "bhnd",
+                             grads: tuple | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(dq, dk, dv)`` of :func:`flash_attention_lse` in the shapes of ``q, k, v``.
+
+    ``dk, dv`` sum over the query heads of a group, and over the batch where the keys are shared.
+    Probabilities are recomputed from ``lse``; P and dS are rounded to the input dtype for the
+    products, sums are fp32 in a fixed order (the same bits on every run), each gradient is rounded
+    once.  ``grads``: optional ``(dq, dk, dv)`` tensors to write, e.g. views of one fused gradient
+    (None entries are allocated).
+    """
+    _lib.require_cuda(grad_out, q, k, v, out, lse)
+    batch, heads, nq, dim = _dense_shape(q, k, v, q_layout)
+    _check_saved(grad_out, out, lse, q, (batch, nq, heads * dim), (batch, heads, nq))
+    with torch.cuda.device(q.device):
+        dq, dk, dv = grads = _grads(grads, (q, k, v))
+        if nq == 0 or batch == 0 or k.shape[2] == 0:
+            for t in grads:
+                t.zero_()
+            return dq, dk, dv
+        q, k, v = _fit(q), _fit(k), _fit(v)
+        rows = lambda t: _fit(t.unflatten(2, (heads, dim)))  # noqa: E731
+        out, grad_out, lse = rows(out), rows(grad_out), lse.contiguous()
+        order = (2, 1, 0) if q_layout == "bhnd" else (1, 2, 0)
+        _backward(grad_out, q, k, v, out, lse, grads,
+                  {"q": _steps(q, order), "dq": _steps(dq, order), "o": _steps(out, (1, 2, 0)),
+                   "do": _steps(grad_out, (1, 2, 0)), "k": _steps(k, (2, 1, 0)), "v": _steps(v, (2, 1, 0)),
+                   "dk": _steps(dk, (2, 1, 0)), "dv": _steps(dv, (2, 1, 0))},
+                  nq=nq, nk=k.shape[2], num_seqs=batch, heads=heads, kv_heads=k.shape[1], head_dim=dim,
+                  scale=float(scale))
+    return dq, dk, dv
+
+
+def flash_attn_varlen_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                               out: torch.Tensor, lse: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                               cu_seqlens_k: torch.Tensor | None, scale: float,
+                               grads: tuple | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(dq, dk, dv)`` of :func:`flash_attn_varlen_lse` in the shapes of ``q, k, v``, as
+    :func:`flash_attention_backward`; with ``cu_seqlens_k=None`` ``dk, dv`` sum over all sequences.
+    No longest length is needed.  The offsets must cover all rows."""
+    _lib.require_cuda(grad_out, q, k, v, out, lse, cu_seqlens_q, cu_seqlens_k)
+    cu_q, cu_k, heads, dim = _varlen_shape(q, k, v, cu_seqlens_q, cu_seqlens_k)
+    tq = q.shape[0]
+    _check_saved(grad_out, out, lse, q, (tq, heads, dim), (heads, tq))
+    with torch.cuda.device(q.device):
+        dq, dk, dv = grads = _grads(grads, (q, k, v))
+        if tq == 0 or k.shape[0] == 0 or cu_q.numel() < 2:
+            for t in grads:
+                t.zero_()
+            return dq, dk, dv
+        q, k, v, out, grad_out, lse = _fit(q), _fit(k), _fit(v), _fit(out), _fit(grad_out), lse.contiguous()
+        step = lambda t: [*_steps(t, (0, 1)), 0]  # noqa: E731
+        _backward(grad_out, q, k, v, out, lse, grads,
+                  {"q": step(q), "k": step(k), "v": step(v), "o": step(out), "do": step(grad_out), "dq": step(dq),
+                   "dk": step(dk), "dv": step(dv)},
+                  cu_seqlens_q=cu_q.data_ptr(), cu_seqlens_k=_lib.ptr(cu_k), nq=tq, nk=k.shape[0],
+                  num_seqs=cu_q.numel() - 1, heads=heads, kv_heads=k.shape[1], head_dim=dim, scale=float(scale))
+    return dq, dk, dv

@@ -155,6 +155,57 @@ HI3D_API int hi3d_flash_attn_split_workspace_size(const hi3d_attn_args* args, in
 HI3D_API int hi3d_flash_attn_fwd_split(const hi3d_attn_args* args, int k_splits, void* workspace,
                                        int64_t workspace_bytes, void* stream);
 
+/* hi3d_flash_attn_fwd_split for training: also writes lse = ln sum_k exp(scale q k^T) (fp32,
+ * [num_seqs][heads][nq], packed: [heads][nq]).  kv_heads divides heads: query head h reads key head
+ * h / (heads / kv_heads).  Rows without keys get out = 0 and lse = -inf.  k_splits == 1 needs no
+ * workspace.  nk >= 1.  The reference has no backward pass; its attention is
+ * src/hi3d_mac/mlx_backend/attention.py:238-277. */
+HI3D_API int hi3d_flash_attn_fwd_lse(const hi3d_attn_args* args, int kv_heads, float* lse, int k_splits,
+                                     void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Gradients of that attention, probabilities recomputed from lse: with P = exp(scale q k^T - lse),
+ * delta = rowsum(dout * out), dS = P * (dout v^T - delta):
+ *   dq = scale dS k,  dk = scale dS^T q,  dv = P^T dout,
+ * dk and dv summed over the query heads of a group and, where keys are shared (k_batch == 0 with
+ * cu_seqlens_k == NULL), over all sequences.  P and dS are rounded to the I/O type for the products,
+ * which accumulate in fp32; each gradient is rounded once.  No atomics on sums: the same bits on
+ * every run.  Layout rules as hi3d_attn_args (strides in elements, multiples of 8; pointers 16-byte
+ * aligned); cu_seqlens are read on the device and cut to the rows that exist, no longest length is
+ * needed.  Rows outside every sequence are not written.  All sizes >= 1. */
+typedef struct hi3d_attn_bwd_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* out;
+  const void* dout;
+  const float* lse;
+  void* dq;
+  void* dk;
+  void* dv;
+  int64_t q_row, q_head, q_batch;
+  int64_t k_row, k_head, k_batch;
+  int64_t v_row, v_head, v_batch;
+  int64_t o_row, o_head, o_batch;
+  int64_t do_row, do_head, do_batch;
+  int64_t dq_row, dq_head, dq_batch;
+  int64_t dk_row, dk_head, dk_batch;
+  int64_t dv_row, dv_head, dv_batch;
+  const int32_t* cu_seqlens_q;
+  const int32_t* cu_seqlens_k;
+  int64_t nq;
+  int64_t nk;
+  int32_t num_seqs;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t dtype;
+  float scale;
+} hi3d_attn_bwd_args;
+
+HI3D_API int hi3d_flash_attn_bwd_workspace_size(const hi3d_attn_bwd_args* args, int64_t* bytes);
+HI3D_API int hi3d_flash_attn_bwd(const hi3d_attn_bwd_args* args, void* workspace, int64_t workspace_bytes,
+                                 void* stream);
+
 /* Partial results for combining attention over disjoint key sets of the same queries (key sets
  * that become available at different times): k_splits key ranges of
  * args' keys, written as O / l (fp32) to part_o[slot0 + s][row][head][head_dim] and the
