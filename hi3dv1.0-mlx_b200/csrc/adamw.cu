@@ -1,0 +1,323 @@
+// AdamW over many tensors at once, states in 32 bits or in 8:
+//
+//   p <- p (1 - lr wd);  m <- b1 m + (1 - b1) g;  v <- b2 v + (1 - b2) g^2
+//   p <- p - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// all in fp32, every operation rounded by itself (no contraction), so the 8-bit codes do not
+// depend on how a compiler fuses.  16-bit weights are the rounded copy of an fp32 master.
+//
+// The states of all tensors lie in flat buffers, each tensor beginning at a multiple of kBlock
+// elements.  8 bits: a block of kBlock values of m, and of u = sqrt(v), is stored as e4m3 codes
+// of value / scale with scale = max|value| / 448 in fp32.  e4m3 keeps 4 bits over 2^-9 .. 448,
+// and the root doubles the range in v to 2^35; a u that is not 0 is never stored as 0, since a
+// step would divide by it.
+//
+// Bound by HBM: 28 bytes an element (32-bit states; fp32 weights, or 16-bit with their master),
+// 16 with 8-bit states.  One warp takes a block at a time, lane l elements 4 l .. 4 l + 3 and
+// 128 + 4 l .. + 3, so every load and store of a warp is one contiguous run, 16 bytes a lane in
+// fp32, and the block's maxima are warp shuffles.  One launch takes up to kMost tensors: their
+// addresses travel in the kernel's parameters, so no table is copied to the device and the
+// launch can be captured.  A CTA finds its tensor by a binary search over the first chunks.
+#include <math.h>
+
+#include "abi.h"
+#include "common.cuh"
+
+namespace hi3d {
+namespace adamw {
+
+constexpr int kBlock = HI3D_ADAMW_BLOCK;
+constexpr int kWarps = 8;
+constexpr int kChunk = 4 * kWarps * kBlock;  // elements of a CTA
+
+struct Entry {
+  void* p;
+  const void* g;
+  int64_t n;
+  uint32_t at;     // offset in the flat states, in blocks
+  uint32_t chunk;  // first CTA
+};
+
+template <int MOST>
+struct Table {
+  Entry e[MOST];
+};
+
+struct Params {
+  int count;
+  float* master;
+  void* m;
+  void* v;
+  float* scale_m;
+  float* scale_u;
+  const float* grad_scale;  // optional
+  float b1, b1c, b2, b2c, decay, step, root, eps;
+};
+
+template <typename T>
+struct Four;  // 4 consecutive values
+template <>
+struct Four<float> {
+  static __device__ __forceinline__ void load(const float* p, float (&v)[4]) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+  }
+  static __device__ __forceinline__ void store(float* p, const float (&v)[4]) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  }
+  static __device__ __forceinline__ float one(float v) { return v; }
+  static __device__ __forceinline__ float back(float v) { return v; }
+};
+template <typename T>
+struct Four16 {
+  static __device__ __forceinline__ void load(const T* p, float (&v)[4]) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    f2_unpack(Cvt<T>::to_f2(u.x), v[0], v[1]);
+    f2_unpack(Cvt<T>::to_f2(u.y), v[2], v[3]);
+  }
+  static __device__ __forceinline__ void store(T* p, const float (&v)[4]) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(Cvt<T>::pack2(v[0], v[1]), Cvt<T>::pack2(v[2], v[3]));
+  }
+  static __device__ __forceinline__ float one(T v) { return Cvt<T>::to_f(v); }
+  static __device__ __forceinline__ T back(float v) { return Cvt<T>::from_f(v); }
+};
+template <>
+struct Four<__half> : Four16<__half> {};
+template <>
+struct Four<__nv_bfloat16> : Four16<__nv_bfloat16> {};
+
+__device__ __forceinline__ void decode4(uint32_t c, float (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t h;
+    const uint16_t two = (uint16_t)(c >> (16 * i));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(two));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ uint32_t encode4(const float (&v)[4]) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(v[1]), "f"(v[0]));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(v[3]), "f"(v[2]));
+  return (uint32_t)lo | ((uint32_t)hi << 16);
+}
+
+__device__ __forceinline__ void update(const Params& a, float gs, float& p, float g, float& m, float& v) {
+  g = __fmul_rn(g, gs);
+  m = __fadd_rn(__fmul_rn(m, a.b1), __fmul_rn(g, a.b1c));
+  v = __fadd_rn(__fmul_rn(v, a.b2), __fmul_rn(__fmul_rn(g, g), a.b2c));
+  const float den = __fadd_rn(__fmul_rn(__fsqrt_rn(v), a.root), a.eps);
+  p = __fsub_rn(__fmul_rn(p, a.decay), __fmul_rn(__fdiv_rn(m, den), a.step));
+}
+
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
+}
+
+// 1 / scale, or 0 where the block holds nothing that it could scale (all zero, or below 2^-111)
+__device__ __forceinline__ float inverse(float scale) { return scale >= 0x1p-120f ? __frcp_rn(scale) : 0.f; }
+
+template <typename P, bool EIGHT, int MOST>
+__global__ void __launch_bounds__(kWarps * 32) adamw_kernel(const __grid_constant__ Table<MOST> table,
+                                                            const __grid_constant__ Params a) {
+  constexpr bool kMaster = sizeof(P) == 2;
+  int lo = 0, hi = a.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (table.e[mid].chunk <= blockIdx.x)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  const Entry& e = table.e[lo];
+  const int64_t n = e.n;
+  P* p = static_cast<P*>(e.p);
+  const P* g = static_cast<const P*>(e.g);
+  const int lane = lane_id();
+  const bool wide = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) & (4 * sizeof(P) - 1)) == 0;
+  const float gs = a.grad_scale ? *a.grad_scale : 1.0f;
+  const int64_t first = (int64_t)(blockIdx.x - e.chunk) * kChunk;
+  for (int64_t at = first + warp_id() * kBlock; at < min(first + kChunk, n); at += kWarps * kBlock) {
+    const int64_t s = (int64_t)e.at * kBlock + at;  // this block in the flat states
+    const bool whole = at + kBlock <= n;
+    float w[2][4], gr[2][4], m[2][4], v[2][4];
+    float sm = 0.f, su = 0.f;
+    if constexpr (EIGHT) sm = a.scale_m[s / kBlock], su = a.scale_u[s / kBlock];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t i = at + h * 128 + lane * 4, f = s + h * 128 + lane * 4;
+      if (whole && wide) {
+        Four<P>::load(g + i, gr[h]);
+        if constexpr (!kMaster) Four<P>::load(p + i, w[h]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          gr[h][k] = i + k < n ? Four<P>::one(g[i + k]) : 0.f;
+          if constexpr (!kMaster) w[h][k] = i + k < n ? Four<P>::one(p[i + k]) : 0.f;
+        }
+      }
+      // the flat buffers are padded to whole blocks
+      if constexpr (kMaster) Four<float>::load(a.master + f, w[h]);
+      if constexpr (EIGHT) {
+        decode4(*reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.m) + f), m[h]);
+        decode4(*reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.v) + f), v[h]);
+      } else {
+        Four<float>::load(static_cast<const float*>(a.m) + f, m[h]);
+        Four<float>::load(static_cast<const float*>(a.v) + f, v[h]);
+      }
+    }
+    float big_m = 0.f, big_u = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (EIGHT) {
+          m[h][k] = __fmul_rn(m[h][k], sm);
+          const float u = __fmul_rn(v[h][k], su);
+          v[h][k] = __fmul_rn(u, u);
+        }
+        update(a, gs, w[h][k], gr[h][k], m[h][k], v[h][k]);
+        if (!whole && at + h * 128 + lane * 4 + k >= n) m[h][k] = v[h][k] = 0.f;  // padding stays 0
+        if constexpr (EIGHT) {
+          v[h][k] = __fsqrt_rn(v[h][k]);
+          big_m = fmaxf(big_m, fabsf(m[h][k]));
+          big_u = fmaxf(big_u, v[h][k]);
+        }
+      }
+    float im = 0.f, iu = 0.f;
+    if constexpr (EIGHT) {
+      sm = __fmul_rn(warp_max(big_m), 1.0f / 448.0f);
+      su = __fmul_rn(warp_max(big_u), 1.0f / 448.0f);
+      im = inverse(sm), iu = inverse(su);
+      if (lane == 0) a.scale_m[s / kBlock] = sm, a.scale_u[s / kBlock] = su;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t i = at + h * 128 + lane * 4, f = s + h * 128 + lane * 4;
+      if (whole && wide) {
+        Four<P>::store(p + i, w[h]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (i + k < n) p[i + k] = Four<P>::back(w[h][k]);
+      }
+      if constexpr (kMaster) {
+        if (whole) {
+          Four<float>::store(a.master + f, w[h]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (i + k < n) a.master[f + k] = w[h][k];
+        }
+      }
+      if constexpr (EIGHT) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          m[h][k] = __fmul_rn(m[h][k], im);
+          const float c = __fmul_rn(v[h][k], iu);
+          v[h][k] = v[h][k] > 0.f && iu > 0.f ? (c < 0x1p-9f ? 0x1p-9f : c) : c;
+        }
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.m) + f) = encode4(m[h]);
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.v) + f) = encode4(v[h]);
+      } else {
+        Four<float>::store(static_cast<float*>(a.m) + f, m[h]);
+        Four<float>::store(static_cast<float*>(a.v) + f, v[h]);
+      }
+    }
+  }
+}
+
+// Tables of two sizes: the parameters of a launch are copied with it, 2 KB for the usual handful
+// of tensors, 24 KB for a model's hundreds.
+constexpr int kFew = 64, kMost = 768;
+
+template <typename P, bool EIGHT, int MOST>
+static int launch(const hi3d_adamw_args* a, const Params& base, int from, int count, cudaStream_t st) {
+  Table<MOST> t;
+  Params p = base;
+  p.count = 0;
+  uint64_t chunks = 0;
+  for (int i = from; i < from + count; ++i) {
+    if (a->numels[i] == 0) continue;
+    Entry& e = t.e[p.count++];
+    e.p = a->params[i], e.g = a->grads[i], e.n = a->numels[i];
+    e.at = (uint32_t)(a->offsets[i] / kBlock);
+    e.chunk = (uint32_t)chunks;
+    chunks += (uint64_t)((a->numels[i] + kChunk - 1) / kChunk);
+    if (chunks > 0x7fffffffu) return set_error(HI3D_ERR_INVALID_ARGUMENT, "adamw_step: too many elements");
+  }
+  if (p.count == 0) return HI3D_OK;
+  adamw_kernel<P, EIGHT, MOST><<<(unsigned)chunks, kWarps * 32, 0, st>>>(t, p);
+  return check_launch("adamw_step");
+}
+
+template <typename P, bool EIGHT>
+static int run(const hi3d_adamw_args* a, const Params& p, cudaStream_t st) {
+  for (int from = 0; from < a->count; from += kMost) {
+    const int count = a->count - from < kMost ? a->count - from : kMost;
+    const int rc = count <= kFew ? launch<P, EIGHT, kFew>(a, p, from, count, st)
+                                 : launch<P, EIGHT, kMost>(a, p, from, count, st);
+    if (rc) return rc;
+  }
+  return HI3D_OK;
+}
+
+}  // namespace adamw
+}  // namespace hi3d
+
+using namespace hi3d;
+
+extern "C" int hi3d_adamw_step(const hi3d_adamw_args* a, void* stream) {
+  using namespace adamw;
+  if (!a || a->count < 0) return set_error(HI3D_ERR_INVALID_ARGUMENT, "adamw_step: null arguments");
+  if (a->count == 0) return HI3D_OK;
+  if (!a->params || !a->grads || !a->numels || !a->offsets || !a->exp_avg || !a->exp_avg_sq)
+    return set_error(HI3D_ERR_INVALID_ARGUMENT, "adamw_step: null pointer");
+  if (a->dtype != HI3D_F16 && a->dtype != HI3D_BF16 && a->dtype != HI3D_F32)
+    return set_error(HI3D_ERR_INVALID_ARGUMENT, "adamw_step: dtype must be f16, bf16 or f32");
+  if (a->state_bits != 8 && a->state_bits != 32)
+    return set_error(HI3D_ERR_INVALID_ARGUMENT, "adamw_step: state_bits must be 8 or 32");
+  if ((a->dtype != HI3D_F32) != (a->master != nullptr))
+    return set_error(HI3D_ERR_INVALID_ARGUMENT, "adamw_step: 16-bit weights need a master, 32-bit ones have none");
+  if ((a->state_bits == 8) != (a->scales != nullptr))
+    return set_error(HI3D_ERR_INVALID_ARGUMENT, "adamw_step: 8-bit states need scales, 32-bit ones have none");
+  if (!aligned16(a->master) || !aligned16(a->exp_avg) || !aligned16(a->exp_avg_sq))
+    return set_error(HI3D_ERR_INVALID_ARGUMENT, "adamw_step: state buffers must be 16-byte aligned");
+  if (a->step < 1 || !(a->beta1 >= 0 && a->beta1 < 1) || !(a->beta2 >= 0 && a->beta2 < 1) || !(a->eps >= 0) ||
+      !(a->lr >= 0) || !(a->weight_decay >= 0))
+    return set_error(HI3D_ERR_INVALID_ARGUMENT,
+                     "adamw_step: step >= 1, betas in [0, 1), lr, eps and weight_decay not negative");
+  if (a->total < 0 || a->total % kBlock || a->total / kBlock > 0xffffffffll)
+    return set_error(HI3D_ERR_INVALID_ARGUMENT, "adamw_step: %lld state elements, not a multiple of %d",
+                     (long long)a->total, kBlock);
+  const int size = a->dtype == HI3D_F32 ? 4 : 2;
+  for (int i = 0; i < a->count; ++i) {
+    const int64_t n = a->numels[i], at = a->offsets[i];
+    if (n < 0 || at < 0 || at % kBlock || at > a->total || n > a->total - at)
+      return set_error(HI3D_ERR_INVALID_ARGUMENT, "adamw_step: tensor %d (%lld elements at %lld) outside the states",
+                       i, (long long)n, (long long)at);
+    const uintptr_t p = reinterpret_cast<uintptr_t>(a->params[i]), g = reinterpret_cast<uintptr_t>(a->grads[i]);
+    if (n > 0 && (!p || !g || (p | g) % size))
+      return set_error(HI3D_ERR_INVALID_ARGUMENT, "adamw_step: tensor %d: null or misaligned pointer", i);
+  }
+  Params p;
+  p.count = 0;
+  p.master = a->master, p.m = a->exp_avg, p.v = a->exp_avg_sq;
+  p.scale_m = a->scales, p.scale_u = a->scales ? a->scales + a->total / kBlock : nullptr;
+  p.grad_scale = a->grad_scale;
+  p.b1 = (float)a->beta1, p.b1c = (float)(1 - a->beta1), p.b2 = (float)a->beta2, p.b2c = (float)(1 - a->beta2);
+  p.decay = (float)(1 - a->lr * a->weight_decay);
+  p.step = (float)(a->lr / (1 - pow(a->beta1, (double)a->step)));
+  p.root = (float)pow(1 - pow(a->beta2, (double)a->step), -0.5);
+  p.eps = (float)a->eps;
+  cudaStream_t st = as_stream(stream);
+  const bool eight = a->state_bits == 8;
+  switch (a->dtype) {
+    case HI3D_F32: return eight ? run<float, true>(a, p, st) : run<float, false>(a, p, st);
+    case HI3D_F16: return eight ? run<__half, true>(a, p, st) : run<__half, false>(a, p, st);
+    default: return eight ? run<__nv_bfloat16, true>(a, p, st) : run<__nv_bfloat16, false>(a, p, st);
+  }
+}

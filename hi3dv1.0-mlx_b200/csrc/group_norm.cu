@@ -1,0 +1,610 @@
+// Group norm with an activation over channels-last rows, and its gradient, for ragged samples.
+//
+//   mu, r over the rows of a sample and the channels of a group;  xh = (x - mu) r
+//   u = xh w + b;  y = act(u)
+//   du = dy act'(u);  dw = sum du xh;  db = sum du        (over all rows)
+//   dx = r (du w - mean(du w) - xh mean(du w xh))          (means over the sample and group)
+//
+// Each direction is three launches:
+//   1. chunks of rows, one CTA each: per-channel sums of the chunk (forward: mean and squared
+//      deviations about it, from sums shifted by the first value, so a large mean costs no bits;
+//      backward: sum du and sum du xh);
+//   2. per sample and channel, the chunks in order (forward: pooled deviations; backward: sums,
+//      and dw, db over all samples), 32 channels a CTA;
+//   3. the chunks again, last first: a CTA folds the channels of each group (shared memory) and
+//      writes y or dx.  The last chunks of pass 1 are the ones still in L2.
+// Fixed orders everywhere: no atomics.  A chunk belongs to one sample; sample s begins at chunk
+// offsets[s] / R + s, which covers every sample's rows without a host copy of the offsets.
+//
+// Bound by HBM: x is read twice forward, x and dy twice backward (once each where they stay in
+// L2), y and dx written once with a streaming hint.  Four rows' loads are in flight per thread.
+#include <type_traits>
+
+#include "abi.h"
+#include "common.cuh"
+
+namespace hi3d {
+namespace gn {
+
+constexpr int kThreads = 256;
+
+struct Shape {
+  int64_t rows;            // all samples' rows
+  const int32_t* offsets;  // [samples + 1], or null: samples of rows / samples rows each
+  int samples, channels, groups;
+  int64_t chunk;           // rows of a chunk (R)
+  int chunks;              // over all samples
+  int cols;                // threads across the channels of one CTA
+  int fold;                // lanes that fold one group's channels (a power of two, at most 32)
+};
+
+__device__ __forceinline__ int64_t offset(const Shape& s, int i) {
+  if (!s.offsets) return s.rows / s.samples * i;
+  return min(max((int64_t)s.offsets[i], (int64_t)0), s.rows);
+}
+__device__ __forceinline__ int64_t first_chunk(const Shape& s, int i) { return offset(s, i) / s.chunk + i; }
+
+// The sample of chunk c and the chunk's rows [r0, r1) (empty for a sample's unused last chunk).
+__device__ __forceinline__ int find_chunk(const Shape& s, int c, int64_t& r0, int64_t& r1) {
+  int lo = 0, hi = s.samples - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first_chunk(s, mid) <= c)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  const int64_t end = max(offset(s, lo + 1), offset(s, lo)), k = c - first_chunk(s, lo);
+  r0 = k < 0 ? end : min(end, offset(s, lo) + k * s.chunk);
+  r1 = min(end, r0 + s.chunk);
+  return lo;
+}
+
+// body(group, lane, lanes) for each group with s.fold lanes side by side; lanes past the last
+// group take part (group >= groups) so that the warp's shuffles are whole.
+template <typename F>
+__device__ __forceinline__ void each_group(const Shape& s, F body) {
+  const int lane = threadIdx.x & (s.fold - 1), at = threadIdx.x / s.fold, step = kThreads / s.fold;
+  for (int g = 0; g < s.groups; g += step) body(g + at, lane);
+}
+__device__ __forceinline__ float fold_sum(const Shape& s, float v) {
+  for (int m = s.fold >> 1; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+  return v;
+}
+
+// V consecutive channels as fp32: 16 bytes of any type, or one value.
+template <typename T, int V>
+__device__ __forceinline__ void load(const T* p, float (&v)[V]) {
+  if constexpr (V == 1) {
+    if constexpr (sizeof(T) == 4)
+      v[0] = *p;
+    else
+      v[0] = Cvt<T>::to_f(*p);
+  } else if constexpr (sizeof(T) == 4) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+  } else {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    f2_unpack(Cvt<T>::to_f2(u.x), v[0], v[1]);
+    f2_unpack(Cvt<T>::to_f2(u.y), v[2], v[3]);
+    f2_unpack(Cvt<T>::to_f2(u.z), v[4], v[5]);
+    f2_unpack(Cvt<T>::to_f2(u.w), v[6], v[7]);
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store(T* p, const float (&v)[V]) {
+  if constexpr (V == 1) {
+    if constexpr (sizeof(T) == 4)
+      *p = v[0];
+    else
+      *p = Cvt<T>::from_f(v[0]);
+  } else if constexpr (sizeof(T) == 4) {
+    __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
+  } else {
+    __stcs(reinterpret_cast<uint4*>(p), make_uint4(Cvt<T>::pack2(v[0], v[1]), Cvt<T>::pack2(v[2], v[3]),
+                                                   Cvt<T>::pack2(v[4], v[5]), Cvt<T>::pack2(v[6], v[7])));
+  }
+}
+
+// sigmoid with exp and the reciprocal on the MUFU unit (relative error about 2^-21); below -80,
+// where it is under 2^-115, it is held there: the reciprocal's range ends soon after.
+__device__ __forceinline__ float sigmoid(float u) { return __fdividef(1.0f, 1.0f + __expf(-fmaxf(u, -80.0f))); }
+
+template <bool ACT>
+__device__ __forceinline__ float act(float u) {
+  return ACT ? u * sigmoid(u) : u;
+}
+template <bool ACT>
+__device__ __forceinline__ float act_grad(float u) {
+  if (!ACT) return 1.0f;
+  const float s = sigmoid(u);
+  return s * (1.0f + u * (1.0f - s));
+}
+
+// ---------------------------------------------------------------- pass 1
+// Threads: column x (V channels from x V), row lane y; lanes' results join in lane order.
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) stats_kernel(const T* __restrict__ x, const Shape s,
+                                                         float2* __restrict__ part) {
+  extern __shared__ float2 sh[];  // [lanes][cols V]
+  __shared__ int count[kThreads];
+  int64_t r0, r1;
+  find_chunk(s, blockIdx.x, r0, r1);
+  const int lanes = kThreads / s.cols, cx = threadIdx.x % s.cols, y = threadIdx.x / s.cols;
+  const int ch = (blockIdx.y * s.cols + cx) * V;
+  const bool on = y < lanes && ch < s.channels;
+  float k[V], a[V] = {}, b[V] = {};
+  int n = 0;
+  if (on) {
+    const T* p = x + ch;
+    int64_t r = r0 + y;
+    if (r < r1) load<T, V>(p + r * s.channels, k);
+    n = r < r1 ? (int)((r1 - r + lanes - 1) / lanes) : 0;
+    for (; r + 3 * lanes < r1; r += 4 * lanes) {
+      float v[4][V];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) load<T, V>(p + (r + u * lanes) * s.channels, v[u]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float d = v[u][i] - k[i];
+          a[i] += d;
+          b[i] = fmaf(d, d, b[i]);
+        }
+    }
+    for (; r < r1; r += lanes) {
+      float v[V];
+      load<T, V>(p + r * s.channels, v);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float d = v[i] - k[i];
+        a[i] += d;
+        b[i] = fmaf(d, d, b[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float m = n ? a[i] / n : 0.f;  // mean - k
+      sh[(y * s.cols + cx) * V + i] = n ? make_float2(k[i] + m, fmaxf(0.f, fmaf(-a[i], m, b[i]))) : make_float2(0.f, 0.f);
+    }
+  }
+  if (cx == 0 && y < lanes) count[y] = n;
+  __syncthreads();
+  for (int e = threadIdx.x; e < s.cols * V; e += kThreads) {
+    const int c = blockIdx.y * s.cols * V + e;
+    if (c >= s.channels) break;
+    float mean = 0.f, dev = 0.f, have = 0.f;
+    for (int l = 0; l < lanes; ++l) {
+      const float m = (float)count[l];
+      if (m == 0.f) break;
+      const float2 o = sh[l * s.cols * V + e];
+      const float d = o.x - mean, f = m / (have + m);
+      mean = fmaf(d, f, mean);
+      dev += o.y + d * d * have * f;
+      have += m;
+    }
+    part[(int64_t)blockIdx.x * s.channels + c] = make_float2(mean, dev);
+  }
+}
+
+template <typename T, int V, bool ACT>
+__global__ void __launch_bounds__(kThreads) sums_kernel(const T* __restrict__ x, const T* __restrict__ dy,
+                                                        const Shape s, const float* __restrict__ mean,
+                                                        const float* __restrict__ rstd, const float* __restrict__ w,
+                                                        const float* __restrict__ b, float2* __restrict__ part) {
+  extern __shared__ float2 sh[];  // [lanes][cols V]
+  int64_t r0, r1;
+  const int smp = find_chunk(s, blockIdx.x, r0, r1);
+  const int lanes = kThreads / s.cols, cx = threadIdx.x % s.cols, y = threadIdx.x / s.cols;
+  const int ch = (blockIdx.y * s.cols + cx) * V;
+  if (y < lanes && ch < s.channels) {
+    const int width = s.channels / s.groups;
+    float mu[V], rs[V], ww[V], bb[V], a[V] = {}, c[V] = {};
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int64_t g = (int64_t)smp * s.groups + (ch + i) / width;
+      mu[i] = mean[g], rs[i] = rstd[g], ww[i] = w[ch + i], bb[i] = b[ch + i];
+    }
+    auto add = [&](const float (&v)[V], const float (&d)[V]) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float xh = (v[i] - mu[i]) * rs[i];
+        const float du = d[i] * act_grad<ACT>(fmaf(xh, ww[i], bb[i]));
+        a[i] += du;
+        c[i] = fmaf(du, xh, c[i]);
+      }
+    };
+    int64_t r = r0 + y;
+    for (; r + 1 * lanes < r1; r += 2 * lanes) {
+      float v[2][V], d[2][V];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        load<T, V>(x + (r + u * lanes) * s.channels + ch, v[u]);
+        load<T, V>(dy + (r + u * lanes) * s.channels + ch, d[u]);
+      }
+      add(v[0], d[0]);
+      add(v[1], d[1]);
+    }
+    for (; r < r1; r += lanes) {
+      float v[V], d[V];
+      load<T, V>(x + r * s.channels + ch, v);
+      load<T, V>(dy + r * s.channels + ch, d);
+      add(v, d);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) sh[(y * s.cols + cx) * V + i] = make_float2(a[i], c[i]);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < s.cols * V; e += kThreads) {
+    const int c = blockIdx.y * s.cols * V + e;
+    if (c >= s.channels) break;
+    float2 t = make_float2(0.f, 0.f);
+    for (int l = 0; l < lanes; ++l) {
+      const float2 o = sh[l * s.cols * V + e];
+      t.x += o.x, t.y += o.y;
+    }
+    part[(int64_t)blockIdx.x * s.channels + c] = t;
+  }
+}
+
+// ---------------------------------------------------------------- pass 2
+// 32 channels x 32 chunk lanes a CTA, one sample (forward): {mean, squared deviations} of each
+// channel over the sample's rows.
+__global__ void __launch_bounds__(1024) pool_kernel(const float2* __restrict__ part, const Shape s,
+                                                    float2* __restrict__ chan) {
+  __shared__ float red[32][33];
+  const int c = blockIdx.x * 32 + threadIdx.x, smp = blockIdx.y;
+  const int64_t lo = offset(s, smp), len = max(offset(s, smp + 1) - lo, (int64_t)0);
+  const int64_t base = first_chunk(s, smp);
+  const int chunks = (int)((len + s.chunk - 1) / s.chunk);
+  auto rows = [&](int k) { return (float)min(s.chunk, len - k * s.chunk); };
+  auto fold = [&](float v) {  // over the 32 lanes, in order; every thread gets its channel's
+    red[threadIdx.y][threadIdx.x] = v;
+    __syncthreads();
+    float t = 0.f;
+#pragma unroll
+    for (int y = 0; y < 32; ++y) t += red[y][threadIdx.x];
+    __syncthreads();
+    return t;
+  };
+  // means relative to the first chunk's, so that their sum keeps its bits
+  const bool on = c < s.channels && chunks > 0;
+  const float first = on ? part[base * s.channels + c].x : 0.f;
+  float a = 0.f;
+  if (on)
+    for (int k = threadIdx.y; k < chunks; k += 32)
+      a = fmaf(part[(base + k) * s.channels + c].x - first, rows(k), a);
+  const float m = chunks > 0 ? fold(a) / (float)len : 0.f;
+  float d = 0.f;
+  if (on)
+    for (int k = threadIdx.y; k < chunks; k += 32) {
+      const float2 p = part[(base + k) * s.channels + c];
+      const float e = (p.x - first) - m;
+      d += fmaf(e * e, rows(k), p.y);
+    }
+  const float dev = chunks > 0 ? fold(d) : 0.f;
+  if (threadIdx.y == 0 && c < s.channels) chan[(int64_t)smp * s.channels + c] = make_float2(first + m, dev);
+}
+
+// Backward: sums of each sample and channel, dw and db over the samples in order.
+__global__ void __launch_bounds__(1024) total_kernel(const float2* __restrict__ part, const Shape s,
+                                                     float2* __restrict__ chan, float* __restrict__ dw,
+                                                     float* __restrict__ db) {
+  __shared__ float2 red[32][33];
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  float2 all = make_float2(0.f, 0.f);
+  for (int smp = 0; smp < s.samples; ++smp) {
+    const int64_t lo = offset(s, smp), len = max(offset(s, smp + 1) - lo, (int64_t)0);
+    const int64_t base = first_chunk(s, smp);
+    const int chunks = (int)((len + s.chunk - 1) / s.chunk);
+    float2 a = make_float2(0.f, 0.f);
+    if (c < s.channels)
+      for (int k = threadIdx.y; k < chunks; k += 32) {
+        const float2 p = part[(base + k) * s.channels + c];
+        a.x += p.x, a.y += p.y;
+      }
+    red[threadIdx.y][threadIdx.x] = a;
+    __syncthreads();
+    if (threadIdx.y == 0 && c < s.channels) {
+      float2 t = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int y = 0; y < 32; ++y) t.x += red[y][threadIdx.x].x, t.y += red[y][threadIdx.x].y;
+      chan[(int64_t)smp * s.channels + c] = t;
+      all.x += t.x, all.y += t.y;
+    }
+    __syncthreads();
+  }
+  if (threadIdx.y == 0 && c < s.channels) db[c] = all.x, dw[c] = all.y;
+}
+
+// ---------------------------------------------------------------- pass 3
+// sh[g]: {mean, rstd} of the sample's group g, from its channels' means and deviations
+template <typename T, int V, bool ACT>
+__global__ void __launch_bounds__(kThreads) apply_kernel(const T* __restrict__ x, const Shape s,
+                                                         const float2* __restrict__ chan, float eps,
+                                                         const float* __restrict__ w, const float* __restrict__ b,
+                                                         T* __restrict__ out, float* __restrict__ mean,
+                                                         float* __restrict__ rstd) {
+  extern __shared__ float2 sh[];
+  const int c0 = (int)gridDim.x - 1 - (int)blockIdx.x;
+  int64_t r0, r1;
+  const int smp = find_chunk(s, c0, r0, r1);
+  const bool first = c0 == first_chunk(s, smp);
+  if (r0 >= r1 && !first) return;
+  const int width = s.channels / s.groups;
+  const float len = (float)max(offset(s, smp + 1) - offset(s, smp), (int64_t)0);
+  each_group(s, [&](int g, int lane) {
+    const bool on = g < s.groups;
+    const float2* p = chan + (int64_t)smp * s.channels + (on ? g : 0) * width;
+    const float k = p[0].x;
+    float m = 0.f, d = 0.f;
+#pragma unroll 4
+    for (int i = lane; i < width; i += s.fold) m += p[i].x - k;
+    m = fold_sum(s, m) / width;
+#pragma unroll 4
+    for (int i = lane; i < width; i += s.fold) {
+      const float e = (p[i].x - k) - m;
+      d += fmaf(e * e, len, p[i].y);
+    }
+    d = fold_sum(s, d);
+    if (!on || lane != 0) return;
+    const float r = 1.0f / sqrtf((len > 0.f ? d / (len * width) : 0.f) + eps);
+    sh[g] = make_float2(k + m, r);
+    if (first && blockIdx.y == 0) {
+      mean[(int64_t)smp * s.groups + g] = k + m;
+      rstd[(int64_t)smp * s.groups + g] = r;
+    }
+  });
+  __syncthreads();
+  const int lanes = kThreads / s.cols, cx = threadIdx.x % s.cols, y = threadIdx.x / s.cols;
+  const int ch = (blockIdx.y * s.cols + cx) * V;
+  if (y >= lanes || ch >= s.channels) return;
+  float mu[V], ww[V], bb[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float2 st = sh[(ch + i) / width];
+    mu[i] = st.x, ww[i] = st.y * w[ch + i], bb[i] = b[ch + i];
+  }
+  auto put = [&](int64_t r, const float (&v)[V]) {
+    float o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = act<ACT>(fmaf(v[i] - mu[i], ww[i], bb[i]));
+    store<T, V>(out + r * s.channels + ch, o);
+  };
+  int64_t r = r0 + y;
+  for (; r + 3 * lanes < r1; r += 4 * lanes) {
+    float v[4][V];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) load<T, V>(x + (r + u * lanes) * s.channels + ch, v[u]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) put(r + u * lanes, v[u]);
+  }
+  for (; r < r1; r += lanes) {
+    float v[V];
+    load<T, V>(x + r * s.channels + ch, v);
+    put(r, v);
+  }
+}
+
+// sh[g]: {mean(du w), mean(du w xh)} over the sample and group
+template <typename T, int V, bool ACT>
+__global__ void __launch_bounds__(kThreads) grad_kernel(const T* __restrict__ x, const T* __restrict__ dy,
+                                                        const Shape s, const float2* __restrict__ chan,
+                                                        const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                        const float* __restrict__ w, const float* __restrict__ b,
+                                                        T* __restrict__ dx) {
+  extern __shared__ float2 sh[];
+  int64_t r0, r1;
+  const int smp = find_chunk(s, (int)gridDim.x - 1 - (int)blockIdx.x, r0, r1);
+  if (r0 >= r1) return;
+  const int width = s.channels / s.groups;
+  const float count = (float)(offset(s, smp + 1) - offset(s, smp)) * width;
+  each_group(s, [&](int g, int lane) {
+    const bool on = g < s.groups;
+    const float2* p = chan + (int64_t)smp * s.channels + (on ? g : 0) * width;
+    const float* wg = w + (on ? g : 0) * width;
+    float a = 0.f, c = 0.f;
+#pragma unroll 4
+    for (int i = lane; i < width; i += s.fold) {
+      a = fmaf(p[i].x, wg[i], a);
+      c = fmaf(p[i].y, wg[i], c);
+    }
+    a = fold_sum(s, a), c = fold_sum(s, c);
+    if (on && lane == 0) sh[g] = make_float2(a / count, c / count);
+  });
+  __syncthreads();
+  const int lanes = kThreads / s.cols, cx = threadIdx.x % s.cols, y = threadIdx.x / s.cols;
+  const int ch = (blockIdx.y * s.cols + cx) * V;
+  if (y >= lanes || ch >= s.channels) return;
+  float mu[V], rs[V], ww[V], bb[V], c1[V], c2[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int g = (ch + i) / width;
+    mu[i] = mean[(int64_t)smp * s.groups + g], rs[i] = rstd[(int64_t)smp * s.groups + g];
+    ww[i] = w[ch + i], bb[i] = b[ch + i], c1[i] = sh[g].x, c2[i] = sh[g].y;
+  }
+  auto put = [&](int64_t r, const float (&v)[V], const float (&d)[V]) {
+    float o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float xh = (v[i] - mu[i]) * rs[i];
+      const float du = d[i] * act_grad<ACT>(fmaf(xh, ww[i], bb[i]));
+      o[i] = rs[i] * (fmaf(du, ww[i], -c1[i]) - xh * c2[i]);
+    }
+    store<T, V>(dx + r * s.channels + ch, o);
+  };
+  int64_t r = r0 + y;
+  for (; r + lanes < r1; r += 2 * lanes) {
+    float v[2][V], d[2][V];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      load<T, V>(x + (r + u * lanes) * s.channels + ch, v[u]);
+      load<T, V>(dy + (r + u * lanes) * s.channels + ch, d[u]);
+    }
+    put(r, v[0], d[0]);
+    put(r + lanes, v[1], d[1]);
+  }
+  for (; r < r1; r += lanes) {
+    float v[V], d[V];
+    load<T, V>(x + r * s.channels + ch, v);
+    load<T, V>(dy + r * s.channels + ch, d);
+    put(r, v, d);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+constexpr int kMaxGroups = 4096;  // a CTA holds a pair per group in shared memory
+
+// Chunks per SM: enough CTAs to fill the machine several times over (the last wave is short),
+// few enough that the partial sums stay small beside x.
+constexpr int kChunksPerSm = 8;
+
+static Shape make_shape(const hi3d_group_norm_args* a, bool wide) {
+  Shape s;
+  s.rows = a->rows, s.offsets = a->offsets;
+  s.samples = a->samples, s.channels = (int)a->channels, s.groups = a->groups;
+  const int vec = wide ? (a->dtype == HI3D_F32 ? 4 : 8) : 1;
+  const int across = (s.channels + vec - 1) / vec;
+  s.cols = across < kThreads ? across : kThreads;
+  const int lanes = kThreads / s.cols;
+  const int64_t want = (a->rows + (int64_t)kChunksPerSm * sm_count() - 1) / ((int64_t)kChunksPerSm * sm_count());
+  const int64_t least = 4 * lanes;
+  s.chunk = want < least ? least : want;
+  s.chunks = (int)(a->rows / s.chunk + a->samples);
+  s.fold = 1;
+  while (s.fold < 32 && s.fold * 2 <= s.channels / s.groups) s.fold *= 2;
+  return s;
+}
+
+static int64_t round256(int64_t b) { return (b + 255) & ~int64_t(255); }
+
+static int64_t workspace(const Shape& s) {
+  return round256((int64_t)s.chunks * s.channels * 8) + round256((int64_t)s.samples * s.channels * 8);
+}
+
+static int check_args(const hi3d_group_norm_args* a) {
+  if (!a) return set_error(HI3D_ERR_INVALID_ARGUMENT, "group_norm: null arguments");
+  if (a->rows < 0 || a->samples < 1 || a->channels < 1 || a->groups < 1 || a->channels % a->groups)
+    return set_error(HI3D_ERR_INVALID_ARGUMENT, "group_norm: %lld channels in %d groups, %d samples of %lld rows",
+                     (long long)a->channels, a->groups, a->samples, (long long)a->rows);
+  if (!a->offsets && a->rows % a->samples)
+    return set_error(HI3D_ERR_INVALID_ARGUMENT, "group_norm: %lld rows in %d equal samples", (long long)a->rows,
+                     a->samples);
+  if (a->groups > kMaxGroups || a->channels > (1 << 20) || a->samples > 65535)
+    return set_error(HI3D_ERR_UNSUPPORTED, "group_norm: at most %d groups, 2^20 channels, 65535 samples", kMaxGroups);
+  if (a->dtype != HI3D_F16 && a->dtype != HI3D_BF16 && a->dtype != HI3D_F32)
+    return set_error(HI3D_ERR_INVALID_ARGUMENT, "group_norm: dtype must be f16, bf16 or f32");
+  if (a->act != 0 && a->act != 1) return set_error(HI3D_ERR_INVALID_ARGUMENT, "group_norm: act must be 0 or 1 (swish)");
+  if (!(a->eps > 0.f)) return set_error(HI3D_ERR_INVALID_ARGUMENT, "group_norm: eps must be positive");
+  if (a->rows / 64 > 0x3fffffff) return set_error(HI3D_ERR_INVALID_ARGUMENT, "group_norm: too many rows");
+  return HI3D_OK;
+}
+
+// 16-byte accesses: whole vectors in a row, and aligned addresses
+static bool is_wide(const hi3d_group_norm_args* a, const void* p, const void* q, const void* r) {
+  const int vec = a->dtype == HI3D_F32 ? 4 : 8;
+  return a->channels % vec == 0 && aligned16(p) && aligned16(q) && aligned16(r);
+}
+
+static int check_workspace(const Shape& s, void* ws, int64_t bytes) {
+  if (ws && (reinterpret_cast<uintptr_t>(ws) & 15u) == 0 && bytes >= workspace(s)) return HI3D_OK;
+  return set_error(HI3D_ERR_CAPACITY, "group_norm: workspace %lld bytes, need %lld (16-byte aligned)", (long long)bytes,
+                   (long long)workspace(s));
+}
+
+template <typename T, int V, bool ACT>
+static int forward(const hi3d_group_norm_args* a, const Shape& s, float2* part, float2* chan, cudaStream_t st) {
+  const T* x = static_cast<const T*>(a->x);
+  const unsigned tiles = (unsigned)((s.channels + s.cols * V - 1) / (s.cols * V));
+  const dim3 grid((unsigned)s.chunks, tiles);
+  int rc;
+  stats_kernel<T, V><<<grid, kThreads, (size_t)(kThreads / s.cols) * s.cols * V * 8, st>>>(x, s, part);
+  if ((rc = check_launch("group_norm statistics"))) return rc;
+  pool_kernel<<<dim3((unsigned)((s.channels + 31) / 32), (unsigned)s.samples), dim3(32, 32), 0, st>>>(part, s, chan);
+  if ((rc = check_launch("group_norm pooling"))) return rc;
+  apply_kernel<T, V, ACT><<<grid, kThreads, (size_t)s.groups * 8, st>>>(
+      x, s, chan, a->eps, a->weight, a->bias, static_cast<T*>(a->y), a->mean, a->rstd);
+  return check_launch("group_norm");
+}
+
+template <typename T, int V, bool ACT>
+static int backward(const hi3d_group_norm_args* a, const Shape& s, float2* part, float2* chan, cudaStream_t st) {
+  const T *x = static_cast<const T*>(a->x), *dy = static_cast<const T*>(a->dy);
+  const unsigned tiles = (unsigned)((s.channels + s.cols * V - 1) / (s.cols * V));
+  const dim3 grid((unsigned)s.chunks, tiles);
+  int rc;
+  sums_kernel<T, V, ACT><<<grid, kThreads, (size_t)(kThreads / s.cols) * s.cols * V * 8, st>>>(
+      x, dy, s, a->mean, a->rstd, a->weight, a->bias, part);
+  if ((rc = check_launch("group_norm gradient sums"))) return rc;
+  total_kernel<<<(unsigned)((s.channels + 31) / 32), dim3(32, 32), 0, st>>>(part, s, chan, a->dweight, a->dbias);
+  if ((rc = check_launch("group_norm gradient totals"))) return rc;
+  grad_kernel<T, V, ACT><<<grid, kThreads, (size_t)s.groups * 8, st>>>(x, dy, s, chan, a->mean, a->rstd, a->weight,
+                                                                      a->bias, static_cast<T*>(a->dx));
+  return check_launch("group_norm gradient");
+}
+
+template <typename T, bool FWD>
+static int run(const hi3d_group_norm_args* a, const Shape& s, bool wide, uint8_t* ws, cudaStream_t st) {
+  constexpr int V = sizeof(T) == 4 ? 4 : 8;
+  float2* part = reinterpret_cast<float2*>(ws);
+  float2* chan = reinterpret_cast<float2*>(ws + round256((int64_t)s.chunks * s.channels * 8));
+  if constexpr (FWD) {
+    if (wide) return a->act ? forward<T, V, true>(a, s, part, chan, st) : forward<T, V, false>(a, s, part, chan, st);
+    return a->act ? forward<T, 1, true>(a, s, part, chan, st) : forward<T, 1, false>(a, s, part, chan, st);
+  } else {
+    if (wide) return a->act ? backward<T, V, true>(a, s, part, chan, st) : backward<T, V, false>(a, s, part, chan, st);
+    return a->act ? backward<T, 1, true>(a, s, part, chan, st) : backward<T, 1, false>(a, s, part, chan, st);
+  }
+}
+
+template <bool FWD>
+static int dispatch(const hi3d_group_norm_args* a, const Shape& s, bool wide, uint8_t* ws, cudaStream_t st) {
+  switch (a->dtype) {
+    case HI3D_F32: return run<float, FWD>(a, s, wide, ws, st);
+    case HI3D_F16: return run<__half, FWD>(a, s, wide, ws, st);
+    default: return run<__nv_bfloat16, FWD>(a, s, wide, ws, st);
+  }
+}
+
+}  // namespace gn
+}  // namespace hi3d
+
+using namespace hi3d;
+
+extern "C" int hi3d_group_norm_act_workspace_size(const hi3d_group_norm_args* a, int64_t* bytes) {
+  int rc = gn::check_args(a);
+  if (rc) return rc;
+  if (!bytes) return set_error(HI3D_ERR_INVALID_ARGUMENT, "group_norm: null bytes");
+  // whichever form the addresses allow
+  const int64_t w = gn::workspace(gn::make_shape(a, true)), n = gn::workspace(gn::make_shape(a, false));
+  *bytes = w > n ? w : n;
+  return HI3D_OK;
+}
+
+extern "C" int hi3d_group_norm_act_fwd(const hi3d_group_norm_args* a, void* workspace, int64_t workspace_bytes,
+                                       void* stream) {
+  int rc = gn::check_args(a);
+  if (rc) return rc;
+  if (!a->weight || !a->bias || !a->mean || !a->rstd || (a->rows > 0 && (!a->x || !a->y)))
+    return set_error(HI3D_ERR_INVALID_ARGUMENT, "group_norm_act_fwd: null pointer");
+  const bool wide = gn::is_wide(a, a->x, a->y, nullptr);
+  const gn::Shape s = gn::make_shape(a, wide);
+  if ((rc = gn::check_workspace(s, workspace, workspace_bytes))) return rc;
+  return gn::dispatch<true>(a, s, wide, static_cast<uint8_t*>(workspace), as_stream(stream));
+}
+
+extern "C" int hi3d_group_norm_act_bwd(const hi3d_group_norm_args* a, void* workspace, int64_t workspace_bytes,
+                                       void* stream) {
+  int rc = gn::check_args(a);
+  if (rc) return rc;
+  if (!a->weight || !a->bias || !a->mean || !a->rstd || !a->dweight || !a->dbias ||
+      (a->rows > 0 && (!a->x || !a->dy || !a->dx)))
+    return set_error(HI3D_ERR_INVALID_ARGUMENT, "group_norm_act_bwd: null pointer");
+  const bool wide = gn::is_wide(a, a->x, a->dy, a->dx);
+  const gn::Shape s = gn::make_shape(a, wide);
+  if ((rc = gn::check_workspace(s, workspace, workspace_bytes))) return rc;
+  return gn::dispatch<false>(a, s, wide, static_cast<uint8_t*>(workspace), as_stream(stream));
+}

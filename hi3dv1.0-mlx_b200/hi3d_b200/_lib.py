@@ -61,6 +61,26 @@ class AttnBwdArgs(ctypes.Structure):
                  ("scale", _f32)]
 
 
+class GroupNormArgs(ctypes.Structure):
+    """Mirror of ``hi3d_group_norm_args``."""
+
+    _fields_ = [(n, _c_void_p) for n in ("x", "weight", "bias", "offsets", "mean", "rstd", "y", "dy", "dx", "dweight",
+                                         "dbias")]
+    _fields_ += [("rows", _i64), ("channels", _i64), ("samples", _i32), ("groups", _i32), ("act", _i32),
+                 ("dtype", _i32), ("eps", _f32)]
+
+
+class AdamWArgs(ctypes.Structure):
+    """Mirror of ``hi3d_adamw_args``."""
+
+    _fields_ = [("params", ctypes.POINTER(_c_void_p)), ("grads", ctypes.POINTER(_c_void_p)),
+                ("numels", ctypes.POINTER(_i64)), ("offsets", ctypes.POINTER(_i64))]
+    _fields_ += [(n, _c_void_p) for n in ("master", "exp_avg", "exp_avg_sq", "scales", "grad_scale")]
+    _fields_ += [("total", _i64), ("step", _i64)]
+    _fields_ += [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")]
+    _fields_ += [("count", _i32), ("dtype", _i32), ("state_bits", _i32)]
+
+
 # name -> (restype, argtypes); every entry of include/hi3d_b200.h
 SIGNATURES: dict[str, tuple] = {
     "hi3d_version": (_i32, []),
@@ -121,6 +141,10 @@ SIGNATURES: dict[str, tuple] = {
     "hi3d_group_norm_stats": (_i32, [_c_void_p, _i64, _i64, _i32, _f32, _c_void_p, _c_void_p, _c_void_p, _i64, _i32,
                                      _c_void_p]),
     "hi3d_group_norm_swish": (_i32, [_c_void_p, _i64, _i64] + [_c_void_p] * 5 + [_i32, _i32, _c_void_p]),
+    "hi3d_group_norm_act_workspace_size": (_i32, [ctypes.POINTER(GroupNormArgs), ctypes.POINTER(_i64)]),
+    "hi3d_group_norm_act_fwd": (_i32, [ctypes.POINTER(GroupNormArgs), _c_void_p, _i64, _c_void_p]),
+    "hi3d_group_norm_act_bwd": (_i32, [ctypes.POINTER(GroupNormArgs), _c_void_p, _i64, _c_void_p]),
+    "hi3d_adamw_step": (_i32, [ctypes.POINTER(AdamWArgs), _c_void_p]),
     "hi3d_child_table_workspace_size": (_i32, [_i64, ctypes.POINTER(_i64)]),
     "hi3d_child_structure": (_i32, [_c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
     "hi3d_child_table": (_i32, [_c_void_p, _i64, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p]),

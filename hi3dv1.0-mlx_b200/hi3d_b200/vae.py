@@ -6,6 +6,8 @@ its helpers:
 * :func:`group_stats`, :func:`group_norm_swish`, :func:`conv_gn_swish` -- ``conv(swish(GN(x)))``
   (vae.py:142-192, kernels.py:242-296): statistics by a deterministic two-stage reduction, the
   activated features written once, then the gathered tcgen05 convolution;
+* :func:`group_norm_act`, :func:`group_norm_act_backward` -- the norm for training: ragged samples,
+  every float type, with its gradient (:mod:`hi3d_b200.training` joins them for autograd);
 * :func:`child_neighbour_table` -- the octree child table from the parent table and the
   occupancy masks (sparse.py:46-95), on the GPU;
 * :func:`serialization`, :func:`window_index`, :func:`window_attention` -- the serialized
@@ -72,6 +74,91 @@ def conv_gn_swish(x: torch.Tensor, level: sparse.Level, norm_weight: torch.Tenso
     act = group_norm_swish(x, mean, inv, norm_weight, norm_bias, out_dtype=torch.float16)
     return sparse.conv(act.to(dtype), level.table, conv_weight.to(dtype), conv_bias, n_in=level.n,
                        tap_mask=level.tap_mask)
+
+
+def _norm_args(x, weight, bias, groups: int, act, eps: float, offsets, mean, rstd):
+    if x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise ValueError("group_norm_act takes float16, bfloat16 or float32 features")
+    if x.dim() < 2:
+        raise ValueError(f"x must be [rows, C] or [samples, ..., C], got {tuple(x.shape)}")
+    c = x.shape[-1]
+    if act not in (None, "swish"):
+        raise ValueError(f"unknown activation {act!r}")
+    if groups < 1 or c < 1 or c % groups:
+        raise ValueError(f"{c} channels do not divide into {groups} groups")
+    if weight.shape != (c,) or bias.shape != (c,):
+        raise ValueError(f"weight and bias must be [{c}]")
+    rows = x.numel() // c
+    samples = 1 if x.dim() == 2 else x.shape[0]
+    if offsets is not None:
+        if x.dim() != 2:
+            raise ValueError("offsets are for packed rows [rows, C]")
+        if offsets.dim() != 1 or offsets.numel() < 2 or offsets.dtype not in (torch.int32, torch.int64):
+            raise ValueError("offsets must be a one-dimensional int32 (or int64) tensor of samples + 1 row offsets")
+        offsets = offsets.to(torch.int32).contiguous()
+        samples = offsets.numel() - 1
+    if any(t.device != x.device for t in (weight, bias, offsets, mean, rstd) if t is not None):
+        raise ValueError("all tensors must be on the device of x")
+    return samples, offsets, _lib.GroupNormArgs(
+        x=x.data_ptr(), weight=weight.data_ptr(), bias=bias.data_ptr(), offsets=_lib.ptr(offsets), rows=rows,
+        channels=c, samples=samples, groups=groups, act=int(act is not None), dtype=_lib.dtype_code(x), eps=float(eps))
+
+
+def _norm_call(name: str, args, x) -> None:
+    lib = _lib.load()
+    nb = ctypes.c_int64()
+    _lib.check(lib.hi3d_group_norm_act_workspace_size(ctypes.byref(args), ctypes.byref(nb)), name, launched=False)
+    ws = torch.empty(nb.value, dtype=torch.uint8, device=x.device)
+    rc = getattr(lib, name)(ctypes.byref(args), ws.data_ptr(), ws.numel(), _lib.stream(x))
+    _lib.check(rc, name)
+
+
+def group_norm_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, groups: int, eps: float = 1e-6,
+                   act: str | None = "swish", offsets: torch.Tensor | None = None,
+                   ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(y, mean, rstd)``: ``act(GroupNorm(x))`` over channels-last rows, in fp32, ``y`` rounded once to
+    the type of ``x``; ``mean, rstd`` fp32 ``[samples, groups]`` for :func:`group_norm_act_backward`.
+
+    ``x`` is one sample ``[rows, C]``, packed samples ``[rows, C]`` with row ``offsets [samples + 1]``
+    (some may be empty; they must cover all rows), or ``[samples, ..., C]``.  ``weight, bias`` ``[C]``.
+    """
+    _lib.require_cuda(x, weight, bias, offsets)
+    x, weight, bias = x.contiguous(), weight.detach().float().contiguous(), bias.detach().float().contiguous()
+    with torch.cuda.device(x.device):
+        samples, offsets, args = _norm_args(x, weight, bias, groups, act, eps, offsets, None, None)
+        y = torch.empty_like(x)
+        mean = torch.empty((samples, groups), dtype=torch.float32, device=x.device)
+        rstd = torch.empty_like(mean)
+        if samples:
+            args.y, args.mean, args.rstd = y.data_ptr(), mean.data_ptr(), rstd.data_ptr()
+            _norm_call("hi3d_group_norm_act_fwd", args, x)
+    return y, mean, rstd
+
+
+def group_norm_act_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                            weight: torch.Tensor, bias: torch.Tensor, act: str | None = "swish",
+                            offsets: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(dx, dweight, dbias)`` of :func:`group_norm_act`: ``dx`` in the type of ``x``, the others fp32
+    ``[C]``, summed over all samples in a fixed order."""
+    _lib.require_cuda(dy, x, mean, rstd, weight, bias, offsets)
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+        raise ValueError(f"dy must be like x {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
+    if mean.dim() != 2 or mean.shape != rstd.shape or mean.dtype != torch.float32 or rstd.dtype != torch.float32:
+        raise ValueError("mean and rstd must be the float32 [samples, groups] of the forward pass")
+    x, dy, mean, rstd = x.contiguous(), dy.contiguous(), mean.contiguous(), rstd.contiguous()
+    weight, bias = weight.detach().float().contiguous(), bias.detach().float().contiguous()
+    with torch.cuda.device(x.device):
+        samples, offsets, args = _norm_args(x, weight, bias, mean.shape[1], act, 1.0, offsets, mean, rstd)
+        if mean.shape[0] != samples:
+            raise ValueError(f"mean and rstd are of {mean.shape[0]} samples, x and offsets of {samples}")
+        dx = torch.empty_like(x)
+        dweight = torch.zeros(x.shape[-1], dtype=torch.float32, device=x.device)
+        dbias = torch.zeros_like(dweight)
+        if samples:
+            args.mean, args.rstd, args.dy, args.dx = mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), dx.data_ptr()
+            args.dweight, args.dbias = dweight.data_ptr(), dbias.data_ptr()
+            _norm_call("hi3d_group_norm_act_bwd", args, x)
+    return dx, dweight, dbias
 
 
 def child_neighbour_table(parent_table: torch.Tensor, child_mask: torch.Tensor):

@@ -485,6 +485,81 @@ HI3D_API int hi3d_group_norm_swish(const void* x, int64_t n, int64_t channels, c
                                    const float* weight, const float* bias, void* out, int in_dtype, int out_dtype,
                                    void* stream);
 
+/* Group norm with an activation over channels-last rows, for training, and its gradient (the
+ * reference's decoder runs forward only: src/hi3d_mac/mlx_backend/vae.py:142-192).  x [rows,
+ * channels] in the given type; sample s holds rows [offsets[s], offsets[s + 1]) (device int32,
+ * ascending, cut to the rows that exist), or without offsets rows / samples each.  Per sample and
+ * group of channels / groups channels, mean and variance over its rows and channels:
+ *   u = (x - mean) / sqrt(var + eps) * weight + bias,  y = u (act 0) or u sigmoid(u) (act 1),
+ * in fp32, y rounded once.  forward writes y and mean, rstd [samples][groups] (an empty sample: 0 and
+ * 1 / sqrt(eps)); backward reads x, dy, mean, rstd and writes dx and, over all samples, dweight and
+ * dbias (fp32 [channels]).  Deterministic (fixed summation order).  Rows outside every sample are
+ * not written. */
+typedef struct hi3d_group_norm_args {
+  const void* x;
+  const float* weight;
+  const float* bias;
+  const int32_t* offsets;
+  float* mean;
+  float* rstd;
+  void* y;        /* forward */
+  const void* dy; /* backward, with the three below */
+  void* dx;
+  float* dweight;
+  float* dbias;
+  int64_t rows;
+  int64_t channels;
+  int32_t samples;
+  int32_t groups;
+  int32_t act;
+  int32_t dtype;
+  float eps;
+} hi3d_group_norm_args;
+
+HI3D_API int hi3d_group_norm_act_workspace_size(const hi3d_group_norm_args* args, int64_t* bytes);
+HI3D_API int hi3d_group_norm_act_fwd(const hi3d_group_norm_args* args, void* workspace, int64_t workspace_bytes,
+                                     void* stream);
+HI3D_API int hi3d_group_norm_act_bwd(const hi3d_group_norm_args* args, void* workspace, int64_t workspace_bytes,
+                                     void* stream);
+
+/* ---- optimiser ------------------------------------------------------------- */
+/* One AdamW step of `count` tensors of one type, in place (the reference has no optimiser):
+ *   g = grad * grad_scale;  p = p (1 - lr weight_decay);  m = beta1 m + (1 - beta1) g;
+ *   v = beta2 v + (1 - beta2) g^2;
+ *   p -= lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * in fp32, each operation rounded.  params, grads, numels and offsets are host arrays of `count`;
+ * params and grads are device pointers of the given type.  16-bit weights are the rounded copy of
+ * `master` (fp32, flat), 32-bit ones have none.  Tensor i's state lies at element offsets[i] (a
+ * multiple of HI3D_ADAMW_BLOCK) of the flat buffers of `total` elements, padded with zeros:
+ *   state_bits 32: exp_avg = m, exp_avg_sq = v, fp32;
+ *   state_bits  8: e4m3 codes of m / s and sqrt(v) / s, s = max|.| / 448 of each block of
+ *     HI3D_ADAMW_BLOCK values; scales [2][total / HI3D_ADAMW_BLOCK] = s of m, s of sqrt(v).
+ * grad_scale: optional device scalar.  The host arrays may be reused once the call returns. */
+#define HI3D_ADAMW_BLOCK 256
+typedef struct hi3d_adamw_args {
+  void* const* params;
+  const void* const* grads;
+  const int64_t* numels;
+  const int64_t* offsets;
+  float* master;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* scales;
+  const float* grad_scale;
+  int64_t total;
+  int64_t step; /* counts from 1 */
+  double lr;
+  double beta1;
+  double beta2;
+  double eps;
+  double weight_decay;
+  int32_t count;
+  int32_t dtype;
+  int32_t state_bits;
+} hi3d_adamw_args;
+
+HI3D_API int hi3d_adamw_step(const hi3d_adamw_args* args, void* stream);
+
 /* Bytes of workspace hi3d_child_structure / hi3d_child_table need for num_parents parents. */
 HI3D_API int hi3d_child_table_workspace_size(int64_t num_parents, int64_t* bytes);
 
