@@ -16,8 +16,8 @@
 // only lengthen the key CTAs' stream: the sum over the heads of a group and over the batch is
 // the same accumulation.
 //
-// CTA (320 threads): warp 0 loads (TMA ring of NST stages), warp 1 issues the MMAs and owns the
-// TMEM, warps 2-9 compute; warps 2-5 take the first half of a block's columns, 6-9 the second.
+// CTA (576 threads): warp 0 loads (TMA ring of NST stages), warp 1 issues the MMAs and owns the
+// TMEM, warps 2-17 compute; each four of them take a quarter of a block's columns.
 // TMEM: S is double-buffered, T single, then the accumulators.  P and dS (16-bit) are written
 // over the S columns that the same warp has read, and are the A operands of the last products.
 // Per block j the issuer runs T(j+1) as soon as T(j) has been read, the accumulator products
@@ -30,7 +30,8 @@
 namespace hi3d {
 namespace attn_bwd {
 
-constexpr int kThreads = 320;
+constexpr int kGroups = 4;           // column groups of a block: 4 compute warps each
+constexpr int kThreads = 64 + kGroups * 128;
 constexpr int kRows = 128;           // stationary rows of a CTA
 constexpr float kLog2e = 1.4426950408889634f;
 // Exponentials of each 16 pairs evaluated on the FMA pipe instead of the MUFU unit.
@@ -66,7 +67,7 @@ template <int D, bool KV>
 struct Cfg {
   static constexpr int NCH = (D + 63) / 64;
   static constexpr int BN = D <= 64 ? 128 : 64;  // streamed rows of a block
-  static constexpr int HC = BN / 2;              // columns of one compute warp
+  static constexpr int HC = BN / kGroups;        // columns of one compute warp
   static constexpr int NST = 4;
   static constexpr int X_CHUNK = kRows * 128;
   static constexpr int X_BYTES = NCH * X_CHUNK;  // one stationary operand
@@ -204,6 +205,26 @@ __device__ __forceinline__ int ds_exponent(const unsigned* amax, int D) {
   return min(max(k, -40), 40);
 }
 
+template <int N>
+__device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&r)[N]) {
+  if constexpr (N == 8) {
+    tmem_ld8(taddr, r);
+  } else if constexpr (N == 16) {
+    tmem_ld16(taddr, r);
+  } else {
+#pragma unroll
+    for (int c = 0; c < N / 32; ++c) tmem_ld32(taddr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
+  }
+}
+template <int N>
+__device__ __forceinline__ void store_columns(uint32_t taddr, const uint32_t (&r)[N]) {
+  static_assert(N == 8 || N == 16, "columns of one chunk");
+  if constexpr (N == 8)
+    tmem_st8(taddr, r);
+  else
+    tmem_st16(taddr, r);
+}
+
 template <typename T, int D, bool KV>
 __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap* tmX2, const CUtensorMap* tmY1,
                                      const CUtensorMap* tmY2, const Params& p, int cta, uint8_t* smem) {
@@ -284,10 +305,10 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
     }
     mbar_init(&bar->tail, 1);
     mbar_init(&bar->t_full, 1);
-    mbar_init(&bar->t_free, 8);  // one arrival per compute warp
+    mbar_init(&bar->t_free, 4 * kGroups);  // one arrival per compute warp
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar->s_full[i], 1);
-      mbar_init(&bar->pd_full[i], 8);
+      mbar_init(&bar->pd_full[i], 4 * kGroups);
       mbar_init(&bar->acc_done[i], 1);
     }
     bar->abort = 0;
@@ -353,7 +374,10 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
+    // The whole warp runs the loop and one elected lane issues: under `if (lane == 0)` the compiler
+    // does not know that descriptors and addresses are the same in all active lanes, and an MMA
+    // costs 50 cycles and more to issue (measured alone, 64 columns: 53 cycles against 33).
+    {
       constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
       constexpr uint32_t idesc_s = make_idesc(1, fmt, 0, 0, kRows, BN);
       constexpr uint32_t idesc_acc = make_idesc(1, fmt, 0, 1, kRows, D);
@@ -361,27 +385,28 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
       const uint64_t dX2 = smem_desc(smem_u32(sX2), 16, 1024, kLayoutSW128);
       const uint64_t dY = smem_desc(smem_u32(sY), 16, 1024, kLayoutSW128);
       const uint64_t dYt = smem_desc(smem_u32(sY), C::Y_CHUNK, 1024, kLayoutSW128);  // rows as the K dimension
-      auto product = [&](uint32_t d, uint64_t x, uint32_t y_off) {  // d = x y^T over the channels
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      auto product = [&](uint32_t d, uint64_t x, uint32_t y_off, uint64_t* done) {  // d = x y^T over the channels
+        if (!elect_one()) return;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks)
           mma_f16_ss(d, x + (((ks >> 2) * C::X_CHUNK + (ks & 3) * 32) >> 4),
                      dY + ((y_off + (ks >> 2) * C::Y_CHUNK + (ks & 3) * 32) >> 4), idesc_s, ks > 0 ? 1u : 0u);
+        tc_commit(done);
       };
-      // acc += a y over the block's rows; a: HC / 2 TMEM columns in each half of the S buffer
+      // acc += a y over the block's rows; a: HC / 2 TMEM columns in each group of the S buffer
       auto accumulate = [&](uint32_t d, uint32_t a, uint32_t y_off, bool more) {
 #pragma unroll
         for (int ks = 0; ks < BN / 16; ++ks) {
-          const int half = ks / (HC / 16), k = ks % (HC / 16);
-          mma_f16_ts(d, a + half * HC + k * 8, dYt + ((y_off + ks * 2048) >> 4), idesc_acc, more || ks > 0 ? 1u : 0u);
+          const int group = ks / (HC / 16), k = ks % (HC / 16);
+          mma_f16_ts(d, a + group * HC + k * 8, dYt + ((y_off + ks * 2048) >> 4), idesc_acc, more || ks > 0 ? 1u : 0u);
         }
       };
       auto scores = [&](int j) {
-        product(tmem + (j & 1) * BN, dX1, (j % NST) * C::STAGE);
-        tc_commit(&bar->s_full[j & 1]);
+        product(tm + (j & 1) * BN, dX1, (j % NST) * C::STAGE, &bar->s_full[j & 1]);
       };
       auto gradient = [&](int j) {
-        product(tmem + C::T_COL, dX2, (j % NST) * C::STAGE + C::Y_BYTES);
-        tc_commit(&bar->t_full);
+        product(tm + C::T_COL, dX2, (j % NST) * C::STAGE + C::Y_BYTES, &bar->t_full);
       };
       bool ok = mbar_wait(&bar->x_full, 0, abort, 310) && mbar_wait(&bar->full[0], 0, abort, 311);
       if (ok) {
@@ -401,12 +426,15 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
         }
         if (!(ok = mbar_wait(&bar->pd_full[j & 1], (j >> 1) & 1, abort, 313))) break;
         tc_fence_after();
-        const uint32_t a = tmem + (j & 1) * BN;
+        const uint32_t a = tm + (j & 1) * BN;
         const uint32_t y = (j % NST) * C::STAGE;
-        accumulate(tmem + C::ACC_COL, a + HC / 2, y, j > 0);
-        if constexpr (KV) accumulate(tmem + C::ACC_COL + D, a, y + C::Y_BYTES, j > 0);
-        tc_commit(&bar->acc_done[j & 1]);
-        if (j + NST < n) tc_commit(&bar->empty[j % NST]);
+        if (elect_one()) {
+          accumulate(tm + C::ACC_COL, a + HC / 2, y, j > 0);
+          if constexpr (KV) accumulate(tm + C::ACC_COL + D, a, y + C::Y_BYTES, j > 0);
+          tc_commit(&bar->acc_done[j & 1]);
+          if (j + NST < n) tc_commit(&bar->empty[j % NST]);
+        }
+        __syncwarp();
         if (j + 2 < n) {
           const int j2 = j + 2;
           if (!(ok = mbar_wait(&bar->full[j2 % NST], (j2 / NST) & 1, abort, 311))) break;
@@ -419,11 +447,12 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
     }
   } else {
     // ------------------------------------------------------------ compute
-    const int half = (warp - 2) >> 2;
+    const int group = (warp - 2) >> 2;
+    constexpr int CH = HC < 32 ? HC : 32;  // columns handled at a time
     const int sub = warp & 3;
     const int row = sub * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(sub * 32) << 16;
-    const uint32_t tT = tmem + lane_addr + C::T_COL + half * HC;
+    const uint32_t tT = tmem + lane_addr + C::T_COL + group * HC;
     const uint64_t scale2x2 = f2_splat(p.scale2);
     const int kexp = kHalf ? ds_exponent(p.amax, D) : 0;
     // key CTAs keep P 2^kPShift in 16 bits: dS takes the rest of its exponent here
@@ -438,29 +467,28 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
     const uint64_t nl2 = f2_splat(nl), nd2 = f2_splat(nd);
     bool ok = true;
     for (int j = 0; j < n; ++j, it.next()) {
-      const uint32_t tS = tmem + lane_addr + (j & 1) * BN + half * HC;
-      const int valid = it.valid() - half * HC;  // valid columns of this warp's half
-      const float4* st = reinterpret_cast<const float4*>(sStat + (j % NST) * BN * 8) + half * (HC / 2);
+      const uint32_t tS = tmem + lane_addr + (j & 1) * BN + group * HC;
+      const int valid = it.valid() - group * HC;  // valid columns of this warp's group
+      const float4* st = reinterpret_cast<const float4*>(sStat + (j % NST) * BN * 8) + group * (HC / 2);
       if (KV && !(ok = mbar_wait(&bar->full[j % NST], (j / NST) & 1, abort, 320))) break;
       if (!(ok = mbar_wait(&bar->s_full[j & 1], (j >> 1) & 1, abort, 321))) break;
       tc_fence_after();
       uint32_t sv[HC];
-#pragma unroll
-      for (int c = 0; c < HC / 32; ++c) tmem_ld32(tS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&sv[c * 32]));
+      load_columns<HC>(tS, sv);
       tmem_wait_ld();
 #pragma unroll
-      for (int c = 0; c < HC / 32; ++c) {
+      for (int c = 0; c < HC / CH; ++c) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int i = c * 32 + 2 * e;
+        for (int e = 0; e < CH / 2; ++e) {
+          const int i = c * CH + 2 * e;
           uint64_t bias = nl2;
           if constexpr (KV) {
-            const float2 l = *reinterpret_cast<const float2*>(st + c * 16 + e);
+            const float2 l = *reinterpret_cast<const float2*>(st + c * (CH / 2) + e);
             bias = f2_pack(l.x, l.y);
           }
           const uint64_t x = f2_fma(f2_pack(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), scale2x2, bias);
           uint64_t pp;
-          if (e < kEmuPairs) {
+          if (e % 16 < kEmuPairs * CH / 32) {
             pp = f2_exp2_poly(x);
           } else {
             float x0, x1;
@@ -474,35 +502,34 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
         }
         if (valid < HC) {  // past the end: not a probability, whatever the scores were
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (c * 32 + e >= valid) sv[c * 32 + e] = 0u;
+          for (int e = 0; e < CH; ++e)
+            if (c * CH + e >= valid) sv[c * CH + e] = 0u;
         }
         if constexpr (KV) {
-          uint32_t pk[16];
+          uint32_t pk[CH / 2];
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            pk[e] = Cvt<T>::pack2(__uint_as_float(sv[c * 32 + 2 * e]), __uint_as_float(sv[c * 32 + 2 * e + 1]));
-          tmem_st16(tS + c * 16, pk);
+          for (int e = 0; e < CH / 2; ++e)
+            pk[e] = Cvt<T>::pack2(__uint_as_float(sv[c * CH + 2 * e]), __uint_as_float(sv[c * CH + 2 * e + 1]));
+          store_columns<CH / 2>(tS + c * (CH / 2), pk);
         }
       }
       if (!(ok = mbar_wait(&bar->t_full, j & 1, abort, 322))) break;
       tc_fence_after();
       uint32_t tv[HC];
-#pragma unroll
-      for (int c = 0; c < HC / 32; ++c) tmem_ld32(tT + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&tv[c * 32]));
+      load_columns<HC>(tT, tv);
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar->t_free);
 #pragma unroll
-      for (int c = 0; c < HC / 32; ++c) {
-        uint32_t pk[16];
+      for (int c = 0; c < HC / CH; ++c) {
+        uint32_t pk[CH / 2];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int i = c * 32 + 2 * e;
+        for (int e = 0; e < CH / 2; ++e) {
+          const int i = c * CH + 2 * e;
           uint64_t d = nd2;
           if constexpr (KV) {
-            const float4 q = st[c * 16 + e];
+            const float4 q = st[c * (CH / 2) + e];
             d = f2_pack(q.z, q.w);
           }
           uint64_t pr = f2_pack(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
@@ -513,19 +540,19 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
         }
         if (valid < HC) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            if (c * 32 + 2 * e >= valid) pk[e] &= 0xffff0000u;
-            if (c * 32 + 2 * e + 1 >= valid) pk[e] &= 0x0000ffffu;
+          for (int e = 0; e < CH / 2; ++e) {
+            if (c * CH + 2 * e >= valid) pk[e] &= 0xffff0000u;
+            if (c * CH + 2 * e + 1 >= valid) pk[e] &= 0x0000ffffu;
           }
         }
-        tmem_st16(tS + HC / 2 + c * 16, pk);
+        store_columns<CH / 2>(tS + HC / 2 + c * (CH / 2), pk);
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar->pd_full[j & 1]);
     }
-    // ---- epilogue: half of the channels each
+    // ---- epilogue: the groups alternate, W channels at a time
     if (ok && mbar_wait(&bar->acc_done[(n - 1) & 1], ((n - 1) >> 1) & 1, abort, 323)) {
       tc_fence_after();
       const int64_t r = row0 + row;
@@ -541,21 +568,22 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
         part += (((set * (cu ? 1 : sets) + x_batch) * xheads + h) * rows + x_start + r) * D;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
-          const int d0 = c * 32 + half * 16;  // the halves alternate, 16 channels at a time
-          uint32_t v[16];
+          constexpr int W = 32 / kGroups;
+          const int d0 = c * 32 + group * W;
+          uint32_t v[W];
           __syncwarp();
-          tmem_ld16(tmem + lane_addr + C::ACC_COL + w * D + d0, v);
+          load_columns<W>(tmem + lane_addr + C::ACC_COL + w * D + d0, v);
           tmem_wait_ld();
           if (r < x_len) {
             if (partial) {
 #pragma unroll
-              for (int e = 0; e < 16; e += 4)
+              for (int e = 0; e < W; e += 4)
                 *reinterpret_cast<float4*>(part + d0 + e) =
                     make_float4(__uint_as_float(v[e]) * f, __uint_as_float(v[e + 1]) * f,
                                 __uint_as_float(v[e + 2]) * f, __uint_as_float(v[e + 3]) * f);
             } else {
 #pragma unroll
-              for (int e = 0; e < 16; e += 8) {
+              for (int e = 0; e < W; e += 8) {
                 uint4 o;
                 o.x = Cvt<T>::pack2(__uint_as_float(v[e]) * f, __uint_as_float(v[e + 1]) * f);
                 o.y = Cvt<T>::pack2(__uint_as_float(v[e + 2]) * f, __uint_as_float(v[e + 3]) * f);
