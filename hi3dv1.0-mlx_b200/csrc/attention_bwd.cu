@@ -16,12 +16,14 @@
 // only lengthen the key CTAs' stream: the sum over the heads of a group and over the batch is
 // the same accumulation.
 //
-// CTA (576 threads): warp 0 loads (TMA ring of NST stages), warp 1 issues the MMAs and owns the
-// TMEM, warps 2-17 compute; each four of them take a quarter of a block's columns.
+// CTA (640 threads; head dims over 64: 384): warp 0 loads (TMA ring of NST stages) and owns the TMEM; warps 1-3 issue the
+// MMAs, one each for S, T and the accumulators, so that none queues behind another's waits (a
+// wait costs 80-100 cycles even when it is over); the others compute, each four of them 32 of a
+// block's columns.
 // TMEM: S is double-buffered, T single, then the accumulators.  P and dS (16-bit) are written
 // over the S columns that the same warp has read, and are the A operands of the last products.
-// Per block j the issuer runs T(j+1) as soon as T(j) has been read, the accumulator products
-// of j when P(j), dS(j) are published, then S(j+2), so a warp finds the next scores ready.
+// S(j+2) runs when the accumulator products of j are done with its buffer, T(j+1) as soon as T(j)
+// has been read, so a compute warp finds the next block ready.
 #include <type_traits>
 
 #include "abi.h"
@@ -30,11 +32,10 @@
 namespace hi3d {
 namespace attn_bwd {
 
-constexpr int kGroups = 4;           // column groups of a block: 4 compute warps each
-constexpr int kThreads = 64 + kGroups * 128;
 constexpr int kRows = 128;           // stationary rows of a CTA
 constexpr float kLog2e = 1.4426950408889634f;
-// Exponentials of each 16 pairs evaluated on the FMA pipe instead of the MUFU unit.
+// Of the 16 pairs of exponentials that a thread takes, those evaluated on the FMA pipe instead of
+// the MUFU unit.
 constexpr int kEmuPairs = 4;
 // fp16 only: P is stored times 2^kPShift (P <= 1, so at most 256), which keeps probabilities
 // down to 2^-22 normal numbers; dV is divided by it at the end.
@@ -67,7 +68,10 @@ template <int D, bool KV>
 struct Cfg {
   static constexpr int NCH = (D + 63) / 64;
   static constexpr int BN = D <= 64 ? 128 : 64;  // streamed rows of a block
-  static constexpr int HC = BN / kGroups;        // columns of one compute warp
+  static constexpr int SUB = D <= 64 ? 2 : 1;
+  static constexpr int HC = 32 * SUB;            // columns of a block that one compute warp takes
+  static constexpr int GROUPS = BN / HC;         // column groups of a block: 4 compute warps each
+  static constexpr int THREADS = 128 + GROUPS * 128;
   static constexpr int NST = 4;
   static constexpr int X_CHUNK = kRows * 128;
   static constexpr int X_BYTES = NCH * X_CHUNK;  // one stationary operand
@@ -173,22 +177,24 @@ struct Stream {
     return n;
   }
   __device__ __forceinline__ void skip(int64_t n) {
-    while (n > 0 && b < b_end) {
+    n += (int64_t)g * nblk + blk;
+    while (b < b_end) {
       const int64_t here = (int64_t)groups() * nblk;
-      if (n >= here) {
-        n -= here;
-        ++b;
-        load();
-        continue;
+      if (n < here) {
+        g = (int)(n / nblk);
+        blk = (int)(n - (int64_t)g * nblk);
+        return;
       }
-      g = (int)(n / nblk);
-      blk = (int)(n - (int64_t)g * nblk);
-      return;
+      n -= here;
+      g = blk = 0;
+      ++b;
+      load();
     }
   }
   __device__ __forceinline__ int head() const { return head0 + g; }
   __device__ __forceinline__ int batch() const { return (KV ? p.cu_q : p.cu_k) ? 0 : b; }
   __device__ __forceinline__ int row() const { return (int)(start + (int64_t)blk * BN); }
+  __device__ __forceinline__ int tail() const { return (int)(len % BN); }  // rows of a ragged last block
   __device__ __forceinline__ int valid() const { return (int)min((int64_t)BN, len - (int64_t)blk * BN); }
   // this block's statistics (KV)
   __device__ __forceinline__ const float4* stat() const {
@@ -207,29 +213,38 @@ __device__ __forceinline__ int ds_exponent(const unsigned* amax, int D) {
 
 template <int N>
 __device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&r)[N]) {
-  if constexpr (N == 8) {
+  if constexpr (N == 8)
     tmem_ld8(taddr, r);
-  } else if constexpr (N == 16) {
+  else
     tmem_ld16(taddr, r);
+}
+
+// 32 lanes x 32 fp32 columns, and 32 lanes x 16 columns of packed 16-bit pairs.  BY_COLUMN: a
+// thread holds four rows of eight columns (two halves of 16 lanes), else one row.
+template <bool BY_COLUMN>
+__device__ __forceinline__ void load_block(uint32_t taddr, uint32_t (&r)[32]) {
+  if constexpr (BY_COLUMN) {
+    tmem_ld_16x256b_x4(taddr, *reinterpret_cast<uint32_t(*)[16]>(&r[0]));
+    tmem_ld_16x256b_x4(taddr + (16u << 16), *reinterpret_cast<uint32_t(*)[16]>(&r[16]));
   } else {
-#pragma unroll
-    for (int c = 0; c < N / 32; ++c) tmem_ld32(taddr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
+    tmem_ld32(taddr, r);
   }
 }
-template <int N>
-__device__ __forceinline__ void store_columns(uint32_t taddr, const uint32_t (&r)[N]) {
-  static_assert(N == 8 || N == 16, "columns of one chunk");
-  if constexpr (N == 8)
-    tmem_st8(taddr, r);
-  else
+template <bool BY_COLUMN>
+__device__ __forceinline__ void store_block(uint32_t taddr, const uint32_t (&r)[16]) {
+  if constexpr (BY_COLUMN) {
+    tmem_st_16x128b_x4(taddr, *reinterpret_cast<const uint32_t(*)[8]>(&r[0]));
+    tmem_st_16x128b_x4(taddr + (16u << 16), *reinterpret_cast<const uint32_t(*)[8]>(&r[8]));
+  } else {
     tmem_st16(taddr, r);
+  }
 }
 
 template <typename T, int D, bool KV>
 __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap* tmX2, const CUtensorMap* tmY1,
                                      const CUtensorMap* tmY2, const Params& p, int cta, uint8_t* smem) {
   using C = Cfg<D, KV>;
-  constexpr int BN = C::BN, HC = C::HC, NST = C::NST;
+  constexpr int BN = C::BN, HC = C::HC, SUB = C::SUB, NST = C::NST, kGroups = C::GROUPS, kThreads = C::THREADS;
   constexpr bool kHalf = std::is_same<T, __half>::value;
   uint8_t* sX1 = smem;              // K or Q
   uint8_t* sX2 = sX1 + C::X_BYTES;  // V or dO
@@ -314,7 +329,7 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
     bar->abort = 0;
     fence_barrier_init();
   }
-  if (warp == 1) {
+  if (warp == 0) {
     tmem_alloc(&bar->tmem_base, 512);
     tmem_relinquish();
   }
@@ -372,8 +387,9 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
       for (int j = issued > NST ? issued - NST : 0; j < issued; ++j)
         mbar_wait(&bar->full[j % NST], (j / NST) & 1, &no_abort, 304);
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
+  } else if (warp < 4) {
+    // ------------------------------------------------------------ MMA issuers
+    const int role_id = warp - 1;
     // The whole warp runs the loop and one elected lane issues: under `if (lane == 0)` the compiler
     // does not know that descriptors and addresses are the same in all active lanes, and an MMA
     // costs 50 cycles and more to issue (measured alone, 64 columns: 53 cycles against 33).
@@ -402,53 +418,35 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
           mma_f16_ts(d, a + group * HC + k * 8, dYt + ((y_off + ks * 2048) >> 4), idesc_acc, more || ks > 0 ? 1u : 0u);
         }
       };
-      auto scores = [&](int j) {
-        product(tm + (j & 1) * BN, dX1, (j % NST) * C::STAGE, &bar->s_full[j & 1]);
-      };
-      auto gradient = [&](int j) {
-        product(tm + C::T_COL, dX2, (j % NST) * C::STAGE + C::Y_BYTES, &bar->t_full);
-      };
-      bool ok = mbar_wait(&bar->x_full, 0, abort, 310) && mbar_wait(&bar->full[0], 0, abort, 311);
-      if (ok) {
-        tc_fence_after();
-        scores(0);
-        gradient(0);
-        if (n > 1 && (ok = mbar_wait(&bar->full[1], 0, abort, 311))) {
-          tc_fence_after();
-          scores(1);
-        }
-      }
+      bool ok = role_id == 2 || mbar_wait(&bar->x_full, 0, abort, 310);
       for (int j = 0; ok && j < n; ++j) {
-        if (j + 1 < n) {
-          if (!(ok = mbar_wait(&bar->t_free, j & 1, abort, 312))) break;
-          tc_fence_after();
-          gradient(j + 1);
-        }
-        if (!(ok = mbar_wait(&bar->pd_full[j & 1], (j >> 1) & 1, abort, 313))) break;
-        tc_fence_after();
-        const uint32_t a = tm + (j & 1) * BN;
         const uint32_t y = (j % NST) * C::STAGE;
-        if (elect_one()) {
-          accumulate(tm + C::ACC_COL, a + HC / 2, y, j > 0);
-          if constexpr (KV) accumulate(tm + C::ACC_COL + D, a, y + C::Y_BYTES, j > 0);
-          tc_commit(&bar->acc_done[j & 1]);
-          if (j + NST < n) tc_commit(&bar->empty[j % NST]);
+        if (!(ok = mbar_wait(&bar->full[j % NST], (j / NST) & 1, abort, 311))) break;
+        if (role_id == 0) {  // S(j), once the products that read P(j - 2), dS(j - 2) from this buffer are done
+          if (j > 1 && !(ok = mbar_wait(&bar->acc_done[j & 1], ((j - 2) >> 1) & 1, abort, 314))) break;
+          tc_fence_after();
+          product(tm + (j & 1) * BN, dX1, y, &bar->s_full[j & 1]);
+        } else if (role_id == 1) {  // T(j), once T(j - 1) has been read
+          if (j > 0 && !(ok = mbar_wait(&bar->t_free, (j - 1) & 1, abort, 312))) break;
+          tc_fence_after();
+          product(tm + C::T_COL, dX2, y + C::Y_BYTES, &bar->t_full);
+        } else {  // the accumulators, once P(j), dS(j) are written
+          if (!(ok = mbar_wait(&bar->pd_full[j & 1], (j >> 1) & 1, abort, 313))) break;
+          tc_fence_after();
+          const uint32_t a = tm + (j & 1) * BN;
+          if (elect_one()) {
+            accumulate(tm + C::ACC_COL, a + HC / 2, y, j > 0);
+            if constexpr (KV) accumulate(tm + C::ACC_COL + D, a, y + C::Y_BYTES, j > 0);
+            tc_commit(&bar->acc_done[j & 1]);
+            if (j + NST < n) tc_commit(&bar->empty[j % NST]);
+          }
         }
         __syncwarp();
-        if (j + 2 < n) {
-          const int j2 = j + 2;
-          if (!(ok = mbar_wait(&bar->full[j2 % NST], (j2 / NST) & 1, abort, 311))) break;
-          // the products that read P, dS from this S buffer have to be done before it is overwritten
-          if (!(ok = mbar_wait(&bar->acc_done[j & 1], (j >> 1) & 1, abort, 314))) break;
-          tc_fence_after();
-          scores(j2);
-        }
       }
     }
   } else {
     // ------------------------------------------------------------ compute
-    const int group = (warp - 2) >> 2;
-    constexpr int CH = HC < 32 ? HC : 32;  // columns handled at a time
+    const int group = (warp - 4) >> 2;
     const int sub = warp & 3;
     const int row = sub * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(sub * 32) << 16;
@@ -465,92 +463,101 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
       nd = (row & 1) ? st.w : st.z;
     }
     const uint64_t nl2 = f2_splat(nl), nd2 = f2_splat(nd);
-    bool ok = true;
-    for (int j = 0; j < n; ++j, it.next()) {
+    // A thread holds 16 pairs of neighbouring columns, pair e in registers 2 e, 2 e + 1.  Query CTAs
+    // (statistics by row): one row, columns 2 e, 2 e + 1.  Key CTAs (statistics by column): four
+    // rows of eight columns, column 8 k + 2 (lane % 4) with k = (e / 2) % 4, so that four 16-byte
+    // shared loads serve a block where one row a thread needs 32 (which bound the kernel: a
+    // broadcast still moves 16 bytes to each lane).
+    const int col0 = KV ? 2 * (lane & 3) : 0;
+    auto column = [&](int e) { return col0 + (KV ? 8 * ((e >> 1) & 3) : 2 * e); };
+    // One block; MASK: only its first `valid` rows are the sequence's.
+    auto block = [&](int j, int valid, auto mask) -> bool {
+      constexpr bool MASK = decltype(mask)::value;
       const uint32_t tS = tmem + lane_addr + (j & 1) * BN + group * HC;
-      const int valid = it.valid() - group * HC;  // valid columns of this warp's group
-      const float4* st = reinterpret_cast<const float4*>(sStat + (j % NST) * BN * 8) + group * (HC / 2);
-      if (KV && !(ok = mbar_wait(&bar->full[j % NST], (j / NST) & 1, abort, 320))) break;
-      if (!(ok = mbar_wait(&bar->s_full[j & 1], (j >> 1) & 1, abort, 321))) break;
+      const float4* st = reinterpret_cast<const float4*>(sStat + (j % NST) * BN * 8) + group * (HC / 2) + (lane & 3);
+      float4 q[4];
+      uint32_t sv[SUB][32], pk[16];
+      if (KV && !mbar_wait(&bar->full[j % NST], (j / NST) & 1, abort, 320)) return false;
+      if (!mbar_wait(&bar->s_full[j & 1], (j >> 1) & 1, abort, 321)) return false;
       tc_fence_after();
-      uint32_t sv[HC];
-      load_columns<HC>(tS, sv);
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) load_block<KV>(tS + u * 32, sv[u]);
       tmem_wait_ld();
 #pragma unroll
-      for (int c = 0; c < HC / CH; ++c) {
-#pragma unroll
-        for (int e = 0; e < CH / 2; ++e) {
-          const int i = c * CH + 2 * e;
-          uint64_t bias = nl2;
-          if constexpr (KV) {
-            const float2 l = *reinterpret_cast<const float2*>(st + c * (CH / 2) + e);
-            bias = f2_pack(l.x, l.y);
-          }
-          const uint64_t x = f2_fma(f2_pack(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), scale2x2, bias);
-          uint64_t pp;
-          if (e % 16 < kEmuPairs * CH / 32) {
-            pp = f2_exp2_poly(x);
-          } else {
-            float x0, x1;
-            f2_unpack(x, x0, x1);
-            pp = f2_pack(ex2_approx(x0), ex2_approx(x1));
-          }
-          float p0, p1;
-          f2_unpack(pp, p0, p1);
-          sv[i] = __float_as_uint(p0);
-          sv[i + 1] = __float_as_uint(p1);
-        }
-        if (valid < HC) {  // past the end: not a probability, whatever the scores were
-#pragma unroll
-          for (int e = 0; e < CH; ++e)
-            if (c * CH + e >= valid) sv[c * CH + e] = 0u;
-        }
+      for (int u = 0; u < SUB; ++u) {
         if constexpr (KV) {
-          uint32_t pk[CH / 2];
 #pragma unroll
-          for (int e = 0; e < CH / 2; ++e)
-            pk[e] = Cvt<T>::pack2(__uint_as_float(sv[c * CH + 2 * e]), __uint_as_float(sv[c * CH + 2 * e + 1]));
-          store_columns<CH / 2>(tS + c * (CH / 2), pk);
+          for (int k = 0; k < 4; ++k) q[k] = st[u * 16 + 4 * k];
         }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          uint64_t bias = nl2;
+          if constexpr (KV) bias = f2_pack(q[(e >> 1) & 3].x, q[(e >> 1) & 3].y);
+          const uint64_t x =
+              f2_fma(f2_pack(__uint_as_float(sv[u][2 * e]), __uint_as_float(sv[u][2 * e + 1])), scale2x2, bias);
+          float p0, p1;
+          if (e % 4 == 0 && e < 4 * kEmuPairs) {
+            f2_unpack(f2_exp2_poly(x), p0, p1);
+          } else {
+            f2_unpack(x, p0, p1);
+            p0 = ex2_approx(p0), p1 = ex2_approx(p1);
+          }
+          if constexpr (MASK) {  // past the end: not a probability, whatever the scores were
+            const int c = u * 32 + column(e) + group * HC;
+            p0 = c < valid ? p0 : 0.f;
+            p1 = c + 1 < valid ? p1 : 0.f;
+          }
+          sv[u][2 * e] = __float_as_uint(p0);
+          sv[u][2 * e + 1] = __float_as_uint(p1);
+          if constexpr (KV) pk[e] = Cvt<T>::pack2(p0, p1);
+        }
+        if constexpr (KV) store_block<KV>(tS + u * 16, pk);
       }
-      if (!(ok = mbar_wait(&bar->t_full, j & 1, abort, 322))) break;
+      if (!mbar_wait(&bar->t_full, j & 1, abort, 322)) return false;
       tc_fence_after();
-      uint32_t tv[HC];
-      load_columns<HC>(tT, tv);
-      tmem_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar->t_free);
 #pragma unroll
-      for (int c = 0; c < HC / CH; ++c) {
-        uint32_t pk[CH / 2];
+      for (int u = 0; u < SUB; ++u) {
+        uint32_t tv[32];
+        load_block<KV>(tT + u * 32, tv);
+        if constexpr (KV && SUB > 1) {
 #pragma unroll
-        for (int e = 0; e < CH / 2; ++e) {
-          const int i = c * CH + 2 * e;
+          for (int k = 0; k < 4; ++k) q[k] = st[u * 16 + 4 * k];
+        }
+        tmem_wait_ld();
+        if (u == SUB - 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar->t_free);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
           uint64_t d = nd2;
-          if constexpr (KV) {
-            const float4 q = st[c * (CH / 2) + e];
-            d = f2_pack(q.z, q.w);
-          }
-          uint64_t pr = f2_pack(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
+          if constexpr (KV) d = f2_pack(q[(e >> 1) & 3].z, q[(e >> 1) & 3].w);
+          uint64_t pr = f2_pack(__uint_as_float(sv[u][2 * e]), __uint_as_float(sv[u][2 * e + 1]));
           if constexpr (KV && kHalf) pr = f2_mul(pr, gain);
-          const uint64_t ds =
-              f2_mul(pr, f2_add(f2_pack(__uint_as_float(tv[i]), __uint_as_float(tv[i + 1])), d));
-          pk[e] = Cvt<T>::from_f2(ds);
-        }
-        if (valid < HC) {
-#pragma unroll
-          for (int e = 0; e < CH / 2; ++e) {
-            if (c * CH + 2 * e >= valid) pk[e] &= 0xffff0000u;
-            if (c * CH + 2 * e + 1 >= valid) pk[e] &= 0x0000ffffu;
+          pk[e] = Cvt<T>::from_f2(
+              f2_mul(pr, f2_add(f2_pack(__uint_as_float(tv[2 * e]), __uint_as_float(tv[2 * e + 1])), d)));
+          if constexpr (MASK) {
+            const int c = u * 32 + column(e) + group * HC;
+            if (c >= valid) pk[e] &= 0xffff0000u;
+            if (c + 1 >= valid) pk[e] &= 0x0000ffffu;
           }
         }
-        store_columns<CH / 2>(tS + HC / 2 + c * (CH / 2), pk);
+        store_block<KV>(tS + HC / 2 + u * 16, pk);
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar->pd_full[j & 1]);
+      return true;
+    };
+    bool ok = true;
+    for (int j = 0; ok && j < n;) {
+      // the blocks of one sequence and head; its last may be ragged
+      const int m = min(n - j, it.nblk - it.blk), whole = (int)(it.len / BN) - it.blk;
+      for (int i = 0; ok && i < m; ++i, ++j)
+        ok = i < whole ? block(j, BN, std::false_type()) : block(j, it.tail(), std::true_type());
+      it.skip(m);
     }
     // ---- epilogue: the groups alternate, W channels at a time
     if (ok && mbar_wait(&bar->acc_done[(n - 1) & 1], ((n - 1) >> 1) & 1, abort, 323)) {
@@ -568,7 +575,7 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
         part += (((set * (cu ? 1 : sets) + x_batch) * xheads + h) * rows + x_start + r) * D;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
-          constexpr int W = 32 / kGroups;
+          constexpr int W = 32 / kGroups;  // 8 or 16
           const int d0 = c * 32 + group * W;
           uint32_t v[W];
           __syncwarp();
@@ -600,14 +607,14 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
+  if (warp == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Cfg<D, true>::THREADS, 1)
     bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
                const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                const __grid_constant__ CUtensorMap tmQs, const __grid_constant__ CUtensorMap tmDOs,
@@ -903,7 +910,7 @@ static int launch(const hi3d_attn_bwd_args* a, const Plan& n, uint8_t* ws, cudaS
   auto kern = bwd_kernel<T, D>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, CK::SMEM);
   if (e != cudaSuccess) return set_error(HI3D_ERR_CUDA, "flash_attn_bwd: smem attribute: %s", cudaGetErrorString(e));
-  kern<<<(unsigned)(n.kv_ctas + n.q_ctas), kThreads, CK::SMEM, st>>>(mq, md, mk, mv, mqs, mds, mks, mvs, p);
+  kern<<<(unsigned)(n.kv_ctas + n.q_ctas), CK::THREADS, CK::SMEM, st>>>(mq, md, mk, mv, mqs, mds, mks, mvs, p);
   if ((rc = check_launch("flash_attn_bwd"))) return rc;
 
   ReduceJob jobs[3] = {};
