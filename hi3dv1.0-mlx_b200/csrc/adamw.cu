@@ -3,8 +3,11 @@
 //   p <- p (1 - lr wd);  m <- b1 m + (1 - b1) g;  v <- b2 v + (1 - b2) g^2
 //   p <- p - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
-// all in fp32, every operation rounded by itself (no contraction), so the 8-bit codes do not
-// depend on how a compiler fuses.  16-bit weights are the rounded copy of an fp32 master.
+// all in fp32.  The moments' products and sums are rounded one by one (no contraction), so the
+// 8-bit codes do not depend on how a compiler fuses; the root and the quotient are the MUFU
+// unit's (2 units in the last place each, on an update that is itself a small part of p): with
+// correctly rounded ones the 8-bit step was bound by issue, not by HBM.  16-bit weights are the
+// rounded copy of an fp32 master.
 //
 // The states of all tensors lie in flat buffers, each tensor beginning at a multiple of kBlock
 // elements.  8 bits: a block of kBlock values of m, and of u = sqrt(v), is stored as e4m3 codes
@@ -103,12 +106,21 @@ __device__ __forceinline__ uint32_t encode4(const float (&v)[4]) {
   return (uint32_t)lo | ((uint32_t)hi << 16);
 }
 
-__device__ __forceinline__ void update(const Params& a, float gs, float& p, float g, float& m, float& v) {
+// sqrt(x) to 2 units in the last place; below 2^-126 0, which adds nothing to eps
+__device__ __forceinline__ float root_approx(float x) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// u: the root of the new v
+__device__ __forceinline__ void update(const Params& a, float gs, float& p, float g, float& m, float& v, float& u) {
   g = __fmul_rn(g, gs);
   m = __fadd_rn(__fmul_rn(m, a.b1), __fmul_rn(g, a.b1c));
   v = __fadd_rn(__fmul_rn(v, a.b2), __fmul_rn(__fmul_rn(g, g), a.b2c));
-  const float den = __fadd_rn(__fmul_rn(__fsqrt_rn(v), a.root), a.eps);
-  p = __fsub_rn(__fmul_rn(p, a.decay), __fmul_rn(__fdiv_rn(m, den), a.step));
+  u = root_approx(v);
+  const float den = __fadd_rn(__fmul_rn(u, a.root), a.eps);
+  p = __fsub_rn(__fmul_rn(p, a.decay), __fmul_rn(__fdividef(m, den), a.step));
 }
 
 __device__ __forceinline__ float warp_max(float x) {
@@ -179,10 +191,11 @@ __global__ void __launch_bounds__(kWarps * 32) adamw_kernel(const __grid_constan
           const float u = __fmul_rn(v[h][k], su);
           v[h][k] = __fmul_rn(u, u);
         }
-        update(a, gs, w[h][k], gr[h][k], m[h][k], v[h][k]);
+        float u;
+        update(a, gs, w[h][k], gr[h][k], m[h][k], v[h][k], u);
+        if constexpr (EIGHT) v[h][k] = u;
         if (!whole && at + h * 128 + lane * 4 + k >= n) m[h][k] = v[h][k] = 0.f;  // padding stays 0
         if constexpr (EIGHT) {
-          v[h][k] = __fsqrt_rn(v[h][k]);
           big_m = fmaxf(big_m, fabsf(m[h][k]));
           big_u = fmaxf(big_u, v[h][k]);
         }

@@ -27,25 +27,31 @@ namespace hi3d {
 namespace gn {
 
 constexpr int kThreads = 256;
+constexpr int kInFlight = 4;  // rows whose loads a thread has in flight (two tensors: half)
 
 struct Shape {
-  int64_t rows;            // all samples' rows
+  int rows;                // all samples' rows
   const int32_t* offsets;  // [samples + 1], or null: samples of rows / samples rows each
   int samples, channels, groups;
-  int64_t chunk;           // rows of a chunk (R)
+  int chunk;               // rows of a chunk (R)
   int chunks;              // over all samples
   int cols;                // threads across the channels of one CTA
   int fold;                // lanes that fold one group's channels (a power of two, at most 32)
 };
 
-__device__ __forceinline__ int64_t offset(const Shape& s, int i) {
-  if (!s.offsets) return s.rows / s.samples * i;
-  return min(max((int64_t)s.offsets[i], (int64_t)0), s.rows);
+__device__ __forceinline__ int offset(const Shape& s, int i) {
+  if (!s.offsets) return s.samples == 1 ? (i ? s.rows : 0) : s.rows / s.samples * i;
+  return min(max(s.offsets[i], 0), s.rows);
 }
-__device__ __forceinline__ int64_t first_chunk(const Shape& s, int i) { return offset(s, i) / s.chunk + i; }
+__device__ __forceinline__ int first_chunk(const Shape& s, int i) { return offset(s, i) / s.chunk + i; }
 
-// The sample of chunk c and the chunk's rows [r0, r1) (empty for a sample's unused last chunk).
-__device__ __forceinline__ int find_chunk(const Shape& s, int c, int64_t& r0, int64_t& r1) {
+// A chunk's sample, the sample's rows, and the chunk's rows [r0, r1) (empty for a sample's unused
+// last chunk).
+struct Chunk {
+  int sample, len, r0, r1;
+  bool first;
+};
+__device__ __forceinline__ Chunk find_chunk(const Shape& s, int c) {
   int lo = 0, hi = s.samples - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -54,10 +60,14 @@ __device__ __forceinline__ int find_chunk(const Shape& s, int c, int64_t& r0, in
     else
       hi = mid - 1;
   }
-  const int64_t end = max(offset(s, lo + 1), offset(s, lo)), k = c - first_chunk(s, lo);
-  r0 = k < 0 ? end : min(end, offset(s, lo) + k * s.chunk);
-  r1 = min(end, r0 + s.chunk);
-  return lo;
+  const int begin = offset(s, lo), end = max(offset(s, lo + 1), begin), k = c - (begin / s.chunk + lo);
+  Chunk r;
+  r.sample = lo;
+  r.len = end - begin;
+  r.first = k == 0;
+  r.r0 = k < 0 ? end : (int)min((int64_t)end, begin + (int64_t)k * s.chunk);
+  r.r1 = (int)min((int64_t)end, (int64_t)r.r0 + s.chunk);
+  return r;
 }
 
 // body(group, lane, lanes) for each group with s.fold lanes side by side; lanes past the last
@@ -72,25 +82,77 @@ __device__ __forceinline__ float fold_sum(const Shape& s, float v) {
   return v;
 }
 
-// V consecutive channels as fp32: 16 bytes of any type, or one value.
+// V consecutive channels: 16 bytes of any type, or one value; unpacked to fp32 when used, so that
+// rows in flight hold 4 registers each.
 template <typename T, int V>
-__device__ __forceinline__ void load(const T* p, float (&v)[V]) {
-  if constexpr (V == 1) {
+struct Raw {
+  uint4 u;
+  __device__ __forceinline__ void load(const T* p) { u = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void get(float (&v)[V]) const {
+    if constexpr (sizeof(T) == 4) {
+      v[0] = __uint_as_float(u.x), v[1] = __uint_as_float(u.y), v[2] = __uint_as_float(u.z), v[3] = __uint_as_float(u.w);
+    } else {
+      f2_unpack(Cvt<T>::to_f2(u.x), v[0], v[1]);
+      f2_unpack(Cvt<T>::to_f2(u.y), v[2], v[3]);
+      f2_unpack(Cvt<T>::to_f2(u.z), v[4], v[5]);
+      f2_unpack(Cvt<T>::to_f2(u.w), v[6], v[7]);
+    }
+  }
+};
+template <typename T>
+struct Raw<T, 1> {
+  T u;
+  __device__ __forceinline__ void load(const T* p) { u = *p; }
+  __device__ __forceinline__ void get(float (&v)[1]) const {
     if constexpr (sizeof(T) == 4)
-      v[0] = *p;
+      v[0] = u;
     else
-      v[0] = Cvt<T>::to_f(*p);
-  } else if constexpr (sizeof(T) == 4) {
-    const float4 f = *reinterpret_cast<const float4*>(p);
-    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-  } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    f2_unpack(Cvt<T>::to_f2(u.x), v[0], v[1]);
-    f2_unpack(Cvt<T>::to_f2(u.y), v[2], v[3]);
-    f2_unpack(Cvt<T>::to_f2(u.z), v[4], v[5]);
-    f2_unpack(Cvt<T>::to_f2(u.w), v[6], v[7]);
+      v[0] = Cvt<T>::to_f(u);
+  }
+};
+
+// body(row, values of x[, values of dy]) for rows r, r + step, .. below end, U rows' loads in flight
+template <typename T, int V, int U, typename F>
+__device__ __forceinline__ void each_row(const T* x, int64_t stride, int r, int end, int step, F body) {
+  Raw<T, V> a[U];
+  float v[V];
+  for (; r + (U - 1) * step < end; r += U * step) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) a[u].load(x + (r + u * step) * stride);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      a[u].get(v);
+      body(r + u * step, v);
+    }
+  }
+  for (; r < end; r += step) {
+    a[0].load(x + r * stride);
+    a[0].get(v);
+    body(r, v);
   }
 }
+template <typename T, int V, int U, typename F>
+__device__ __forceinline__ void each_row(const T* x, const T* y, int64_t stride, int r, int end, int step, F body) {
+  Raw<T, V> a[U], b[U];
+  float v[V], w[V];
+  for (; r + (U - 1) * step < end; r += U * step) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) a[u].load(x + (r + u * step) * stride), b[u].load(y + (r + u * step) * stride);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      a[u].get(v);
+      b[u].get(w);
+      body(r + u * step, v, w);
+    }
+  }
+  for (; r < end; r += step) {
+    a[0].load(x + r * stride), b[0].load(y + r * stride);
+    a[0].get(v);
+    b[0].get(w);
+    body(r, v, w);
+  }
+}
+
 template <typename T, int V>
 __device__ __forceinline__ void store(T* p, const float (&v)[V]) {
   if constexpr (V == 1) {
@@ -128,41 +190,26 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const T* __restrict__ x
                                                          float2* __restrict__ part) {
   extern __shared__ float2 sh[];  // [lanes][cols V]
   __shared__ int count[kThreads];
-  int64_t r0, r1;
-  find_chunk(s, blockIdx.x, r0, r1);
+  const Chunk t = find_chunk(s, blockIdx.x);
   const int lanes = kThreads / s.cols, cx = threadIdx.x % s.cols, y = threadIdx.x / s.cols;
   const int ch = (blockIdx.y * s.cols + cx) * V;
   const bool on = y < lanes && ch < s.channels;
   float k[V], a[V] = {}, b[V] = {};
-  int n = 0;
+  const int r = t.r0 + y, n = y < lanes && r < t.r1 ? (t.r1 - r + lanes - 1) / lanes : 0;
   if (on) {
-    const T* p = x + ch;
-    int64_t r = r0 + y;
-    if (r < r1) load<T, V>(p + r * s.channels, k);
-    n = r < r1 ? (int)((r1 - r + lanes - 1) / lanes) : 0;
-    for (; r + 3 * lanes < r1; r += 4 * lanes) {
-      float v[4][V];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) load<T, V>(p + (r + u * lanes) * s.channels, v[u]);
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float d = v[u][i] - k[i];
-          a[i] += d;
-          b[i] = fmaf(d, d, b[i]);
-        }
+    if (n) {
+      Raw<T, V> first;
+      first.load(x + ch + (int64_t)r * s.channels);
+      first.get(k);
     }
-    for (; r < r1; r += lanes) {
-      float v[V];
-      load<T, V>(p + r * s.channels, v);
+    each_row<T, V, kInFlight>(x + ch, s.channels, r, t.r1, lanes, [&](int, const float (&v)[V]) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float d = v[i] - k[i];
         a[i] += d;
         b[i] = fmaf(d, d, b[i]);
       }
-    }
+    });
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const float m = n ? a[i] / n : 0.f;  // mean - k
@@ -188,50 +235,38 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const T* __restrict__ x
   }
 }
 
-template <typename T, int V, bool ACT>
+// UNI: a vector's channels lie in one group, whose statistics are then one value each.
+template <typename T, int V, bool ACT, bool UNI>
 __global__ void __launch_bounds__(kThreads) sums_kernel(const T* __restrict__ x, const T* __restrict__ dy,
                                                         const Shape s, const float* __restrict__ mean,
                                                         const float* __restrict__ rstd, const float* __restrict__ w,
                                                         const float* __restrict__ b, float2* __restrict__ part) {
   extern __shared__ float2 sh[];  // [lanes][cols V]
-  int64_t r0, r1;
-  const int smp = find_chunk(s, blockIdx.x, r0, r1);
+  const Chunk t = find_chunk(s, blockIdx.x);
   const int lanes = kThreads / s.cols, cx = threadIdx.x % s.cols, y = threadIdx.x / s.cols;
   const int ch = (blockIdx.y * s.cols + cx) * V;
   if (y < lanes && ch < s.channels) {
+    constexpr int G = UNI ? 1 : V;
     const int width = s.channels / s.groups;
-    float mu[V], rs[V], ww[V], bb[V], a[V] = {}, c[V] = {};
+    float mu[G], rs[G], ww[V], bb[V], a[V] = {}, c[V] = {};
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int64_t g = (int64_t)smp * s.groups + (ch + i) / width;
-      mu[i] = mean[g], rs[i] = rstd[g], ww[i] = w[ch + i], bb[i] = b[ch + i];
+      if (i < G) {
+        const int64_t g = (int64_t)t.sample * s.groups + (ch + i) / width;
+        mu[i] = mean[g], rs[i] = rstd[g];
+      }
+      ww[i] = w[ch + i], bb[i] = b[ch + i];
     }
-    auto add = [&](const float (&v)[V], const float (&d)[V]) {
+    each_row<T, V, kInFlight / 2>(x + ch, dy + ch, s.channels, t.r0 + y, t.r1, lanes,
+                                  [&](int, const float (&v)[V], const float (&d)[V]) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float xh = (v[i] - mu[i]) * rs[i];
+        const float xh = (v[i] - mu[i % G]) * rs[i % G];
         const float du = d[i] * act_grad<ACT>(fmaf(xh, ww[i], bb[i]));
         a[i] += du;
         c[i] = fmaf(du, xh, c[i]);
       }
-    };
-    int64_t r = r0 + y;
-    for (; r + 1 * lanes < r1; r += 2 * lanes) {
-      float v[2][V], d[2][V];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        load<T, V>(x + (r + u * lanes) * s.channels + ch, v[u]);
-        load<T, V>(dy + (r + u * lanes) * s.channels + ch, d[u]);
-      }
-      add(v[0], d[0]);
-      add(v[1], d[1]);
-    }
-    for (; r < r1; r += lanes) {
-      float v[V], d[V];
-      load<T, V>(x + r * s.channels + ch, v);
-      load<T, V>(dy + r * s.channels + ch, d);
-      add(v, d);
-    }
+    });
 #pragma unroll
     for (int i = 0; i < V; ++i) sh[(y * s.cols + cx) * V + i] = make_float2(a[i], c[i]);
   }
@@ -250,41 +285,41 @@ __global__ void __launch_bounds__(kThreads) sums_kernel(const T* __restrict__ x,
 
 // ---------------------------------------------------------------- pass 2
 // 32 channels x 32 chunk lanes a CTA, one sample (forward): {mean, squared deviations} of each
-// channel over the sample's rows.
+// channel over the sample's rows, from the chunks' means about the first chunk's (so their
+// squares keep their bits) and deviations.
 __global__ void __launch_bounds__(1024) pool_kernel(const float2* __restrict__ part, const Shape s,
                                                     float2* __restrict__ chan) {
-  __shared__ float red[32][33];
+  __shared__ float red[3][32][33];
   const int c = blockIdx.x * 32 + threadIdx.x, smp = blockIdx.y;
-  const int64_t lo = offset(s, smp), len = max(offset(s, smp + 1) - lo, (int64_t)0);
-  const int64_t base = first_chunk(s, smp);
-  const int chunks = (int)((len + s.chunk - 1) / s.chunk);
-  auto rows = [&](int k) { return (float)min(s.chunk, len - k * s.chunk); };
-  auto fold = [&](float v) {  // over the 32 lanes, in order; every thread gets its channel's
-    red[threadIdx.y][threadIdx.x] = v;
-    __syncthreads();
-    float t = 0.f;
-#pragma unroll
-    for (int y = 0; y < 32; ++y) t += red[y][threadIdx.x];
-    __syncthreads();
-    return t;
-  };
-  // means relative to the first chunk's, so that their sum keeps its bits
+  const int lo = offset(s, smp), len = max(offset(s, smp + 1) - lo, 0);
+  const int64_t base = lo / s.chunk + smp;
+  const int chunks = (len + s.chunk - 1) / s.chunk;
   const bool on = c < s.channels && chunks > 0;
-  const float first = on ? part[base * s.channels + c].x : 0.f;
-  float a = 0.f;
-  if (on)
-    for (int k = threadIdx.y; k < chunks; k += 32)
-      a = fmaf(part[(base + k) * s.channels + c].x - first, rows(k), a);
-  const float m = chunks > 0 ? fold(a) / (float)len : 0.f;
-  float d = 0.f;
-  if (on)
+  const float2* p = part + base * s.channels + c;
+  const float first = on ? p->x : 0.f;
+  float a = 0.f, b = 0.f, d = 0.f;
+  if (on) {
+#pragma unroll 8
     for (int k = threadIdx.y; k < chunks; k += 32) {
-      const float2 p = part[(base + k) * s.channels + c];
-      const float e = (p.x - first) - m;
-      d += fmaf(e * e, rows(k), p.y);
+      const float2 q = p[(int64_t)k * s.channels];
+      const float e = q.x - first, n = (float)min(s.chunk, len - k * s.chunk);
+      a = fmaf(e, n, a);
+      b = fmaf(e * e, n, b);
+      d += q.y;
     }
-  const float dev = chunks > 0 ? fold(d) : 0.f;
-  if (threadIdx.y == 0 && c < s.channels) chan[(int64_t)smp * s.channels + c] = make_float2(first + m, dev);
+  }
+  red[0][threadIdx.y][threadIdx.x] = a;
+  red[1][threadIdx.y][threadIdx.x] = b;
+  red[2][threadIdx.y][threadIdx.x] = d;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < s.channels) {
+    a = b = d = 0.f;
+#pragma unroll
+    for (int y = 0; y < 32; ++y)
+      a += red[0][y][threadIdx.x], b += red[1][y][threadIdx.x], d += red[2][y][threadIdx.x];
+    const float m = chunks > 0 ? a / (float)len : 0.f;
+    chan[(int64_t)smp * s.channels + c] = make_float2(first + m, d + fmaxf(0.f, fmaf(-a, m, b)));
+  }
 }
 
 // Backward: sums of each sample and channel, dw and db over the samples in order.
@@ -295,15 +330,17 @@ __global__ void __launch_bounds__(1024) total_kernel(const float2* __restrict__ 
   const int c = blockIdx.x * 32 + threadIdx.x;
   float2 all = make_float2(0.f, 0.f);
   for (int smp = 0; smp < s.samples; ++smp) {
-    const int64_t lo = offset(s, smp), len = max(offset(s, smp + 1) - lo, (int64_t)0);
-    const int64_t base = first_chunk(s, smp);
-    const int chunks = (int)((len + s.chunk - 1) / s.chunk);
+    const int lo = offset(s, smp), len = max(offset(s, smp + 1) - lo, 0);
+    const int64_t base = lo / s.chunk + smp;
+    const int chunks = (len + s.chunk - 1) / s.chunk;
     float2 a = make_float2(0.f, 0.f);
-    if (c < s.channels)
+    if (c < s.channels) {
+#pragma unroll 8
       for (int k = threadIdx.y; k < chunks; k += 32) {
         const float2 p = part[(base + k) * s.channels + c];
         a.x += p.x, a.y += p.y;
       }
+    }
     red[threadIdx.y][threadIdx.x] = a;
     __syncthreads();
     if (threadIdx.y == 0 && c < s.channels) {
@@ -320,20 +357,18 @@ __global__ void __launch_bounds__(1024) total_kernel(const float2* __restrict__ 
 
 // ---------------------------------------------------------------- pass 3
 // sh[g]: {mean, rstd} of the sample's group g, from its channels' means and deviations
-template <typename T, int V, bool ACT>
+template <typename T, int V, bool ACT, bool UNI>
 __global__ void __launch_bounds__(kThreads) apply_kernel(const T* __restrict__ x, const Shape s,
                                                          const float2* __restrict__ chan, float eps,
                                                          const float* __restrict__ w, const float* __restrict__ b,
                                                          T* __restrict__ out, float* __restrict__ mean,
                                                          float* __restrict__ rstd) {
   extern __shared__ float2 sh[];
-  const int c0 = (int)gridDim.x - 1 - (int)blockIdx.x;
-  int64_t r0, r1;
-  const int smp = find_chunk(s, c0, r0, r1);
-  const bool first = c0 == first_chunk(s, smp);
-  if (r0 >= r1 && !first) return;
+  const Chunk t = find_chunk(s, (int)gridDim.x - 1 - (int)blockIdx.x);
+  const int smp = t.sample;
+  if (t.r0 >= t.r1 && !t.first) return;
   const int width = s.channels / s.groups;
-  const float len = (float)max(offset(s, smp + 1) - offset(s, smp), (int64_t)0);
+  const float len = (float)t.len;
   each_group(s, [&](int g, int lane) {
     const bool on = g < s.groups;
     const float2* p = chan + (int64_t)smp * s.channels + (on ? g : 0) * width;
@@ -351,7 +386,7 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(const T* __restrict__ x
     if (!on || lane != 0) return;
     const float r = 1.0f / sqrtf((len > 0.f ? d / (len * width) : 0.f) + eps);
     sh[g] = make_float2(k + m, r);
-    if (first && blockIdx.y == 0) {
+    if (t.first && blockIdx.y == 0) {
       mean[(int64_t)smp * s.groups + g] = k + m;
       rstd[(int64_t)smp * s.groups + g] = r;
     }
@@ -360,46 +395,34 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(const T* __restrict__ x
   const int lanes = kThreads / s.cols, cx = threadIdx.x % s.cols, y = threadIdx.x / s.cols;
   const int ch = (blockIdx.y * s.cols + cx) * V;
   if (y >= lanes || ch >= s.channels) return;
-  float mu[V], ww[V], bb[V];
+  constexpr int G = UNI ? 1 : V;
+  float mu[G], ww[V], bb[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const float2 st = sh[(ch + i) / width];
-    mu[i] = st.x, ww[i] = st.y * w[ch + i], bb[i] = b[ch + i];
+    mu[i % G] = st.x, ww[i] = st.y * w[ch + i], bb[i] = b[ch + i];
   }
-  auto put = [&](int64_t r, const float (&v)[V]) {
+  each_row<T, V, kInFlight>(x + ch, s.channels, t.r0 + y, t.r1, lanes, [&](int r, const float (&v)[V]) {
     float o[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = act<ACT>(fmaf(v[i] - mu[i], ww[i], bb[i]));
-    store<T, V>(out + r * s.channels + ch, o);
-  };
-  int64_t r = r0 + y;
-  for (; r + 3 * lanes < r1; r += 4 * lanes) {
-    float v[4][V];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) load<T, V>(x + (r + u * lanes) * s.channels + ch, v[u]);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) put(r + u * lanes, v[u]);
-  }
-  for (; r < r1; r += lanes) {
-    float v[V];
-    load<T, V>(x + r * s.channels + ch, v);
-    put(r, v);
-  }
+    for (int i = 0; i < V; ++i) o[i] = act<ACT>(fmaf(v[i] - mu[i % G], ww[i], bb[i]));
+    store<T, V>(out + (int64_t)r * s.channels + ch, o);
+  });
 }
 
 // sh[g]: {mean(du w), mean(du w xh)} over the sample and group
-template <typename T, int V, bool ACT>
+template <typename T, int V, bool ACT, bool UNI>
 __global__ void __launch_bounds__(kThreads) grad_kernel(const T* __restrict__ x, const T* __restrict__ dy,
                                                         const Shape s, const float2* __restrict__ chan,
                                                         const float* __restrict__ mean, const float* __restrict__ rstd,
                                                         const float* __restrict__ w, const float* __restrict__ b,
                                                         T* __restrict__ dx) {
   extern __shared__ float2 sh[];
-  int64_t r0, r1;
-  const int smp = find_chunk(s, (int)gridDim.x - 1 - (int)blockIdx.x, r0, r1);
-  if (r0 >= r1) return;
+  const Chunk t = find_chunk(s, (int)gridDim.x - 1 - (int)blockIdx.x);
+  const int smp = t.sample;
+  if (t.r0 >= t.r1) return;
   const int width = s.channels / s.groups;
-  const float count = (float)(offset(s, smp + 1) - offset(s, smp)) * width;
+  const float count = (float)t.len * width;
   each_group(s, [&](int g, int lane) {
     const bool on = g < s.groups;
     const float2* p = chan + (int64_t)smp * s.channels + (on ? g : 0) * width;
@@ -417,40 +440,28 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const T* __restrict__ x,
   const int lanes = kThreads / s.cols, cx = threadIdx.x % s.cols, y = threadIdx.x / s.cols;
   const int ch = (blockIdx.y * s.cols + cx) * V;
   if (y >= lanes || ch >= s.channels) return;
-  float mu[V], rs[V], ww[V], bb[V], c1[V], c2[V];
+  constexpr int G = UNI ? 1 : V;
+  float mu[G], rs[G], c1[G], c2[G], ww[V], bb[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int g = (ch + i) / width;
-    mu[i] = mean[(int64_t)smp * s.groups + g], rs[i] = rstd[(int64_t)smp * s.groups + g];
-    ww[i] = w[ch + i], bb[i] = b[ch + i], c1[i] = sh[g].x, c2[i] = sh[g].y;
+    if (i < G) {
+      const int g = (ch + i) / width;
+      mu[i] = mean[(int64_t)smp * s.groups + g], rs[i] = rstd[(int64_t)smp * s.groups + g];
+      c1[i] = sh[g].x, c2[i] = sh[g].y;
+    }
+    ww[i] = w[ch + i], bb[i] = b[ch + i];
   }
-  auto put = [&](int64_t r, const float (&v)[V], const float (&d)[V]) {
+  each_row<T, V, kInFlight / 2>(x + ch, dy + ch, s.channels, t.r0 + y, t.r1, lanes,
+                                [&](int r, const float (&v)[V], const float (&d)[V]) {
     float o[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float xh = (v[i] - mu[i]) * rs[i];
+      const float xh = (v[i] - mu[i % G]) * rs[i % G];
       const float du = d[i] * act_grad<ACT>(fmaf(xh, ww[i], bb[i]));
-      o[i] = rs[i] * (fmaf(du, ww[i], -c1[i]) - xh * c2[i]);
+      o[i] = rs[i % G] * (fmaf(du, ww[i], -c1[i % G]) - xh * c2[i % G]);
     }
-    store<T, V>(dx + r * s.channels + ch, o);
-  };
-  int64_t r = r0 + y;
-  for (; r + lanes < r1; r += 2 * lanes) {
-    float v[2][V], d[2][V];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      load<T, V>(x + (r + u * lanes) * s.channels + ch, v[u]);
-      load<T, V>(dy + (r + u * lanes) * s.channels + ch, d[u]);
-    }
-    put(r, v[0], d[0]);
-    put(r + lanes, v[1], d[1]);
-  }
-  for (; r < r1; r += lanes) {
-    float v[V], d[V];
-    load<T, V>(x + r * s.channels + ch, v);
-    load<T, V>(dy + r * s.channels + ch, d);
-    put(r, v, d);
-  }
+    store<T, V>(dx + (int64_t)r * s.channels + ch, o);
+  });
 }
 
 // ---------------------------------------------------------------------------
@@ -464,16 +475,15 @@ constexpr int kChunksPerSm = 8;
 
 static Shape make_shape(const hi3d_group_norm_args* a, bool wide) {
   Shape s;
-  s.rows = a->rows, s.offsets = a->offsets;
+  s.rows = (int)a->rows, s.offsets = a->offsets;
   s.samples = a->samples, s.channels = (int)a->channels, s.groups = a->groups;
   const int vec = wide ? (a->dtype == HI3D_F32 ? 4 : 8) : 1;
   const int across = (s.channels + vec - 1) / vec;
   s.cols = across < kThreads ? across : kThreads;
-  const int lanes = kThreads / s.cols;
-  const int64_t want = (a->rows + (int64_t)kChunksPerSm * sm_count() - 1) / ((int64_t)kChunksPerSm * sm_count());
-  const int64_t least = 4 * lanes;
+  const int lanes = kThreads / s.cols, ctas = kChunksPerSm * sm_count();
+  const int want = (int)((a->rows + ctas - 1) / ctas), least = kInFlight * lanes;
   s.chunk = want < least ? least : want;
-  s.chunks = (int)(a->rows / s.chunk + a->samples);
+  s.chunks = (int)(a->rows / s.chunk) + a->samples;
   s.fold = 1;
   while (s.fold < 32 && s.fold * 2 <= s.channels / s.groups) s.fold *= 2;
   return s;
@@ -499,7 +509,7 @@ static int check_args(const hi3d_group_norm_args* a) {
     return set_error(HI3D_ERR_INVALID_ARGUMENT, "group_norm: dtype must be f16, bf16 or f32");
   if (a->act != 0 && a->act != 1) return set_error(HI3D_ERR_INVALID_ARGUMENT, "group_norm: act must be 0 or 1 (swish)");
   if (!(a->eps > 0.f)) return set_error(HI3D_ERR_INVALID_ARGUMENT, "group_norm: eps must be positive");
-  if (a->rows / 64 > 0x3fffffff) return set_error(HI3D_ERR_INVALID_ARGUMENT, "group_norm: too many rows");
+  if (a->rows > 0x7ff00000) return set_error(HI3D_ERR_INVALID_ARGUMENT, "group_norm: too many rows");
   return HI3D_OK;
 }
 
@@ -515,7 +525,7 @@ static int check_workspace(const Shape& s, void* ws, int64_t bytes) {
                    (long long)workspace(s));
 }
 
-template <typename T, int V, bool ACT>
+template <typename T, int V, bool ACT, bool UNI>
 static int forward(const hi3d_group_norm_args* a, const Shape& s, float2* part, float2* chan, cudaStream_t st) {
   const T* x = static_cast<const T*>(a->x);
   const unsigned tiles = (unsigned)((s.channels + s.cols * V - 1) / (s.cols * V));
@@ -525,25 +535,33 @@ static int forward(const hi3d_group_norm_args* a, const Shape& s, float2* part, 
   if ((rc = check_launch("group_norm statistics"))) return rc;
   pool_kernel<<<dim3((unsigned)((s.channels + 31) / 32), (unsigned)s.samples), dim3(32, 32), 0, st>>>(part, s, chan);
   if ((rc = check_launch("group_norm pooling"))) return rc;
-  apply_kernel<T, V, ACT><<<grid, kThreads, (size_t)s.groups * 8, st>>>(
+  apply_kernel<T, V, ACT, UNI><<<grid, kThreads, (size_t)s.groups * 8, st>>>(
       x, s, chan, a->eps, a->weight, a->bias, static_cast<T*>(a->y), a->mean, a->rstd);
   return check_launch("group_norm");
 }
 
-template <typename T, int V, bool ACT>
+template <typename T, int V, bool ACT, bool UNI>
 static int backward(const hi3d_group_norm_args* a, const Shape& s, float2* part, float2* chan, cudaStream_t st) {
   const T *x = static_cast<const T*>(a->x), *dy = static_cast<const T*>(a->dy);
   const unsigned tiles = (unsigned)((s.channels + s.cols * V - 1) / (s.cols * V));
   const dim3 grid((unsigned)s.chunks, tiles);
   int rc;
-  sums_kernel<T, V, ACT><<<grid, kThreads, (size_t)(kThreads / s.cols) * s.cols * V * 8, st>>>(
+  sums_kernel<T, V, ACT, UNI><<<grid, kThreads, (size_t)(kThreads / s.cols) * s.cols * V * 8, st>>>(
       x, dy, s, a->mean, a->rstd, a->weight, a->bias, part);
   if ((rc = check_launch("group_norm gradient sums"))) return rc;
   total_kernel<<<(unsigned)((s.channels + 31) / 32), dim3(32, 32), 0, st>>>(part, s, chan, a->dweight, a->dbias);
   if ((rc = check_launch("group_norm gradient totals"))) return rc;
-  grad_kernel<T, V, ACT><<<grid, kThreads, (size_t)s.groups * 8, st>>>(x, dy, s, chan, a->mean, a->rstd, a->weight,
-                                                                      a->bias, static_cast<T*>(a->dx));
+  grad_kernel<T, V, ACT, UNI><<<grid, kThreads, (size_t)s.groups * 8, st>>>(
+      x, dy, s, chan, a->mean, a->rstd, a->weight, a->bias, static_cast<T*>(a->dx));
   return check_launch("group_norm gradient");
+}
+
+template <typename T, bool FWD, int V, bool UNI>
+static int pick_act(const hi3d_group_norm_args* a, const Shape& s, float2* part, float2* chan, cudaStream_t st) {
+  if constexpr (FWD)
+    return a->act ? forward<T, V, true, UNI>(a, s, part, chan, st) : forward<T, V, false, UNI>(a, s, part, chan, st);
+  else
+    return a->act ? backward<T, V, true, UNI>(a, s, part, chan, st) : backward<T, V, false, UNI>(a, s, part, chan, st);
 }
 
 template <typename T, bool FWD>
@@ -551,13 +569,9 @@ static int run(const hi3d_group_norm_args* a, const Shape& s, bool wide, uint8_t
   constexpr int V = sizeof(T) == 4 ? 4 : 8;
   float2* part = reinterpret_cast<float2*>(ws);
   float2* chan = reinterpret_cast<float2*>(ws + round256((int64_t)s.chunks * s.channels * 8));
-  if constexpr (FWD) {
-    if (wide) return a->act ? forward<T, V, true>(a, s, part, chan, st) : forward<T, V, false>(a, s, part, chan, st);
-    return a->act ? forward<T, 1, true>(a, s, part, chan, st) : forward<T, 1, false>(a, s, part, chan, st);
-  } else {
-    if (wide) return a->act ? backward<T, V, true>(a, s, part, chan, st) : backward<T, V, false>(a, s, part, chan, st);
-    return a->act ? backward<T, 1, true>(a, s, part, chan, st) : backward<T, 1, false>(a, s, part, chan, st);
-  }
+  if (!wide) return pick_act<T, FWD, 1, true>(a, s, part, chan, st);
+  return s.channels / s.groups % V == 0 ? pick_act<T, FWD, V, true>(a, s, part, chan, st)
+                                        : pick_act<T, FWD, V, false>(a, s, part, chan, st);
 }
 
 template <bool FWD>

@@ -7,6 +7,7 @@ GPU run can never silently take another code path.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -221,6 +222,14 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(t: torch.Tensor):
+    """Context in which the device of ``t`` is current: the library launches on the current device."""
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def require_cuda(*ts: torch.Tensor | None) -> None:

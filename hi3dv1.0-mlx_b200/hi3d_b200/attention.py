@@ -395,7 +395,7 @@ def flash_attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale
     """
     _lib.require_cuda(q, k, v)
     batch, heads, nq, dim = _dense_shape(q, k, v, q_layout)
-    with torch.cuda.device(q.device):
+    with _lib.on_device(q):
         if k.shape[2] == 0:
             return (torch.zeros((batch, nq, heads * dim), dtype=q.dtype, device=q.device),
                     torch.full((batch, heads, nq), -math.inf, device=q.device))
@@ -428,7 +428,7 @@ def flash_attn_varlen_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_
     _lib.require_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k)
     cu_q, cu_k, heads, dim = _varlen_shape(q, k, v, cu_seqlens_q, cu_seqlens_k)
     tq, tk = q.shape[0], k.shape[0]
-    with torch.cuda.device(q.device):
+    with _lib.on_device(q):
         if tk == 0:
             return (torch.zeros((tq, heads, dim), dtype=q.dtype, device=q.device),
                     torch.full((heads, tq), -math.inf, device=q.device))
@@ -515,7 +515,7 @@ def flash_attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.T
     _lib.require_cuda(grad_out, q, k, v, out, lse)
     batch, heads, nq, dim = _dense_shape(q, k, v, q_layout)
     _check_saved(grad_out, out, lse, q, (batch, nq, heads * dim), (batch, heads, nq))
-    with torch.cuda.device(q.device):
+    with _lib.on_device(q):
         dq, dk, dv = grads = _grads(grads, (q, k, v))
         if nq == 0 or batch == 0 or k.shape[2] == 0:
             for t in grads:
@@ -545,7 +545,7 @@ def flash_attn_varlen_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch
     cu_q, cu_k, heads, dim = _varlen_shape(q, k, v, cu_seqlens_q, cu_seqlens_k)
     tq = q.shape[0]
     _check_saved(grad_out, out, lse, q, (tq, heads, dim), (heads, tq))
-    with torch.cuda.device(q.device):
+    with _lib.on_device(q):
         dq, dk, dv = grads = _grads(grads, (q, k, v))
         if tq == 0 or k.shape[0] == 0 or cu_q.numel() < 2:
             for t in grads:

@@ -98,7 +98,7 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor], exp_avg: t
         grad_scale=_lib.ptr(grad_scale), total=total, step=int(step), lr=float(lr), beta1=float(betas[0]),
         beta2=float(betas[1]), eps=float(eps), weight_decay=float(weight_decay), count=n,
         dtype=_lib.dtype_code(first), state_bits=8 if eight else 32)
-    with torch.cuda.device(device):
+    with _lib.on_device(first):
         _lib.check(_lib.load().hi3d_adamw_step(ctypes.byref(args), _lib.stream(first)), "adamw_step")
 
 

@@ -124,11 +124,10 @@ def group_norm_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, gr
     """
     _lib.require_cuda(x, weight, bias, offsets)
     x, weight, bias = x.contiguous(), weight.detach().float().contiguous(), bias.detach().float().contiguous()
-    with torch.cuda.device(x.device):
+    with _lib.on_device(x):
         samples, offsets, args = _norm_args(x, weight, bias, groups, act, eps, offsets, None, None)
         y = torch.empty_like(x)
-        mean = torch.empty((samples, groups), dtype=torch.float32, device=x.device)
-        rstd = torch.empty_like(mean)
+        mean, rstd = torch.empty((2, samples, groups), dtype=torch.float32, device=x.device)
         if samples:
             args.y, args.mean, args.rstd = y.data_ptr(), mean.data_ptr(), rstd.data_ptr()
             _norm_call("hi3d_group_norm_act_fwd", args, x)
@@ -147,17 +146,19 @@ def group_norm_act_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tenso
         raise ValueError("mean and rstd must be the float32 [samples, groups] of the forward pass")
     x, dy, mean, rstd = x.contiguous(), dy.contiguous(), mean.contiguous(), rstd.contiguous()
     weight, bias = weight.detach().float().contiguous(), bias.detach().float().contiguous()
-    with torch.cuda.device(x.device):
+    with _lib.on_device(x):
         samples, offsets, args = _norm_args(x, weight, bias, mean.shape[1], act, 1.0, offsets, mean, rstd)
         if mean.shape[0] != samples:
             raise ValueError(f"mean and rstd are of {mean.shape[0]} samples, x and offsets of {samples}")
         dx = torch.empty_like(x)
-        dweight = torch.zeros(x.shape[-1], dtype=torch.float32, device=x.device)
-        dbias = torch.zeros_like(dweight)
+        dweight, dbias = torch.empty((2, x.shape[-1]), dtype=torch.float32, device=x.device)
         if samples:
             args.mean, args.rstd, args.dy, args.dx = mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), dx.data_ptr()
             args.dweight, args.dbias = dweight.data_ptr(), dbias.data_ptr()
             _norm_call("hi3d_group_norm_act_bwd", args, x)
+        else:
+            dweight.zero_()
+            dbias.zero_()
     return dx, dweight, dbias
 
 
