@@ -23,6 +23,8 @@
 // launch can be captured.  A CTA finds its tensor by a binary search over the first chunks.
 #include <math.h>
 
+#include <type_traits>
+
 #include "abi.h"
 #include "common.cuh"
 
@@ -32,6 +34,7 @@ namespace adamw {
 constexpr int kBlock = HI3D_ADAMW_BLOCK;
 constexpr int kWarps = 8;
 constexpr int kChunk = 4 * kWarps * kBlock;  // elements of a CTA
+constexpr int kCtas8 = 4;                    // CTAs an SM holds with 8-bit states (at most 64 registers)
 
 struct Entry {
   void* p;
@@ -57,37 +60,50 @@ struct Params {
   float b1, b1c, b2, b2c, decay, step, root, eps;
 };
 
+// 4 consecutive values as they lie in memory
 template <typename T>
-struct Four;  // 4 consecutive values
-template <>
-struct Four<float> {
-  static __device__ __forceinline__ void load(const float* p, float (&v)[4]) {
-    const float4 f = *reinterpret_cast<const float4*>(p);
-    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-  }
-  static __device__ __forceinline__ void store(float* p, const float (&v)[4]) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  }
-  static __device__ __forceinline__ float one(float v) { return v; }
-  static __device__ __forceinline__ float back(float v) { return v; }
-};
-template <typename T>
-struct Four16 {
-  static __device__ __forceinline__ void load(const T* p, float (&v)[4]) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
+struct Four {  // 16-bit types
+  uint2 u;
+  __device__ __forceinline__ void load(const T* p) { u = *reinterpret_cast<const uint2*>(p); }
+  __device__ __forceinline__ void get(float (&v)[4]) const {
     f2_unpack(Cvt<T>::to_f2(u.x), v[0], v[1]);
     f2_unpack(Cvt<T>::to_f2(u.y), v[2], v[3]);
   }
   static __device__ __forceinline__ void store(T* p, const float (&v)[4]) {
     *reinterpret_cast<uint2*>(p) = make_uint2(Cvt<T>::pack2(v[0], v[1]), Cvt<T>::pack2(v[2], v[3]));
   }
-  static __device__ __forceinline__ float one(T v) { return Cvt<T>::to_f(v); }
-  static __device__ __forceinline__ T back(float v) { return Cvt<T>::from_f(v); }
 };
 template <>
-struct Four<__half> : Four16<__half> {};
+struct Four<float> {
+  float4 u;
+  __device__ __forceinline__ void load(const float* p) { u = *reinterpret_cast<const float4*>(p); }
+  __device__ __forceinline__ void get(float (&v)[4]) const { v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w; }
+  static __device__ __forceinline__ void store(float* p, const float (&v)[4]) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  }
+};
+struct Codes {
+  uint32_t u;
+  __device__ __forceinline__ void load(const uint8_t* p) { u = *reinterpret_cast<const uint32_t*>(p); }
+  __device__ __forceinline__ void get(float (&v)[4]) const;
+};
+
+template <typename T>
+__device__ __forceinline__ float one(T v) {
+  return Cvt<T>::to_f(v);
+}
 template <>
-struct Four<__nv_bfloat16> : Four16<__nv_bfloat16> {};
+__device__ __forceinline__ float one<float>(float v) {
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ T back(float v) {
+  return Cvt<T>::from_f(v);
+}
+template <>
+__device__ __forceinline__ float back<float>(float v) {
+  return v;
+}
 
 __device__ __forceinline__ void decode4(uint32_t c, float (&v)[4]) {
 #pragma unroll
@@ -99,6 +115,7 @@ __device__ __forceinline__ void decode4(uint32_t c, float (&v)[4]) {
     v[2 * i] = f.x, v[2 * i + 1] = f.y;
   }
 }
+__device__ __forceinline__ void Codes::get(float (&v)[4]) const { decode4(u, v); }
 __device__ __forceinline__ uint32_t encode4(const float (&v)[4]) {
   uint16_t lo, hi;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(v[1]), "f"(v[0]));
@@ -132,10 +149,143 @@ __device__ __forceinline__ float warp_max(float x) {
 // 1 / scale, or 0 where the block holds nothing that it could scale (all zero, or below 2^-111)
 __device__ __forceinline__ float inverse(float scale) { return scale >= 0x1p-120f ? __frcp_rn(scale) : 0.f; }
 
+// One block of a tensor's values as a lane holds them.
+template <typename P, bool EIGHT>
+struct Block {
+  using State = typename std::conditional<EIGHT, uint8_t, float>::type;
+  Four<P> g[2];
+  Four<float> w[2];  // the fp32 weights: the tensor's own or the master's
+  typename std::conditional<EIGHT, Codes, Four<float>>::type m[2], v[2];
+  float sm, su;
+
+  // i: the lane's first element in the tensor, f: in the flat states
+  __device__ __forceinline__ void load(const Params& a, const P* p, const P* gr, int64_t i, int64_t f) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      g[h].load(gr + i + h * 128);
+      if constexpr (sizeof(P) == 4)
+        w[h].load(p + i + h * 128);
+      else
+        w[h].load(a.master + f + h * 128);
+    }
+    load_state(a, f);
+  }
+  __device__ __forceinline__ void load_state(const Params& a, int64_t f) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      m[h].load(static_cast<const State*>(a.m) + f + h * 128);
+      v[h].load(static_cast<const State*>(a.v) + f + h * 128);
+    }
+    if constexpr (EIGHT) sm = a.scale_m[f / kBlock], su = a.scale_u[f / kBlock];
+  }
+};
+
+// New moments of four values in m and v (8 bits: v holds its root) and weights in w.
+template <bool EIGHT>
+__device__ __forceinline__ void update4(const Params& a, float gs, float sm, float su, const float (&g)[4],
+                                        float (&w)[4], float (&m)[4], float (&v)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (EIGHT) {
+      m[k] = __fmul_rn(m[k], sm);
+      const float u = __fmul_rn(v[k], su);
+      v[k] = __fmul_rn(u, u);
+    }
+    float u;
+    update(a, gs, w[k], g[k], m[k], v[k], u);
+    if constexpr (EIGHT) v[k] = u;
+  }
+}
+
+// The states of a block whose lane holds m and v (its root), written with their scales.
+__device__ __forceinline__ void store_codes(const Params& a, int64_t f, float (&m)[2][4], float (&v)[2][4]) {
+  float big_m = 0.f, big_u = 0.f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) big_m = fmaxf(big_m, fabsf(m[h][k])), big_u = fmaxf(big_u, v[h][k]);
+  const float sm = __fmul_rn(warp_max(big_m), 1.0f / 448.0f), su = __fmul_rn(warp_max(big_u), 1.0f / 448.0f);
+  const float im = inverse(sm), iu = inverse(su);
+  if (lane_id() == 0) a.scale_m[f / kBlock] = sm, a.scale_u[f / kBlock] = su;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      m[h][k] = __fmul_rn(m[h][k], im);
+      const float c = __fmul_rn(v[h][k], iu);
+      v[h][k] = v[h][k] > 0.f && iu > 0.f ? (c < 0x1p-9f ? 0x1p-9f : c) : c;
+    }
+    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.m) + f + h * 128) = encode4(m[h]);
+    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.v) + f + h * 128) = encode4(v[h]);
+  }
+}
+
+// A whole block of an aligned tensor.
+template <typename P, bool EIGHT>
+__device__ __forceinline__ void whole_block(const Params& a, float gs, P* p, int64_t i, int64_t f,
+                                            const Block<P, EIGHT>& b) {
+  float m[2][4], v[2][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float w[4], g[4];
+    b.g[h].get(g);
+    b.w[h].get(w);
+    b.m[h].get(m[h]);
+    b.v[h].get(v[h]);
+    update4<EIGHT>(a, gs, b.sm, b.su, g, w, m[h], v[h]);
+    Four<P>::store(p + i + h * 128, w);
+    if constexpr (sizeof(P) == 2) Four<float>::store(a.master + f + h * 128, w);
+    if constexpr (!EIGHT) {
+      Four<float>::store(static_cast<float*>(a.m) + f + h * 128, m[h]);
+      Four<float>::store(static_cast<float*>(a.v) + f + h * 128, v[h]);
+    }
+  }
+  if constexpr (EIGHT) store_codes(a, f, m, v);
+}
+
+// A tensor's ragged last block, or any of one that vectors cannot address: weights and gradients
+// one by one.  The flat buffers are padded to whole blocks; the padding stays 0.
+template <typename P, bool EIGHT>
+__device__ __noinline__ void odd_block(const Params& a, float gs, P* p, const P* gr, int64_t n, int64_t i, int64_t f) {
+  Block<P, EIGHT> b;
+  b.load_state(a, f);
+  float m[2][4], v[2][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float w[4], g[4];
+    const int64_t at = i + h * 128;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool in = at + k < n;
+      g[k] = in ? one<P>(gr[at + k]) : 0.f;
+      if constexpr (sizeof(P) == 4)
+        w[k] = in ? one<P>(p[at + k]) : 0.f;
+      else
+        w[k] = a.master[f + h * 128 + k];
+    }
+    b.m[h].get(m[h]);
+    b.v[h].get(v[h]);
+    update4<EIGHT>(a, gs, b.sm, b.su, g, w, m[h], v[h]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (at + k < n) {
+        p[at + k] = back<P>(w[k]);
+        if constexpr (sizeof(P) == 2) a.master[f + h * 128 + k] = w[k];
+      } else {
+        m[h][k] = v[h][k] = 0.f;
+      }
+    }
+    if constexpr (!EIGHT) {
+      Four<float>::store(static_cast<float*>(a.m) + f + h * 128, m[h]);
+      Four<float>::store(static_cast<float*>(a.v) + f + h * 128, v[h]);
+    }
+  }
+  if constexpr (EIGHT) store_codes(a, f, m, v);
+}
+
 template <typename P, bool EIGHT, int MOST>
-__global__ void __launch_bounds__(kWarps * 32) adamw_kernel(const __grid_constant__ Table<MOST> table,
-                                                            const __grid_constant__ Params a) {
-  constexpr bool kMaster = sizeof(P) == 2;
+__global__ void __launch_bounds__(kWarps * 32, EIGHT ? kCtas8 : 1)
+    adamw_kernel(const __grid_constant__ Table<MOST> table, const __grid_constant__ Params a) {
   int lo = 0, hi = a.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -145,102 +295,34 @@ __global__ void __launch_bounds__(kWarps * 32) adamw_kernel(const __grid_constan
       hi = mid - 1;
   }
   const Entry& e = table.e[lo];
-  const int64_t n = e.n;
   P* p = static_cast<P*>(e.p);
   const P* g = static_cast<const P*>(e.g);
-  const int lane = lane_id();
-  const bool wide = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) & (4 * sizeof(P) - 1)) == 0;
   const float gs = a.grad_scale ? *a.grad_scale : 1.0f;
-  const int64_t first = (int64_t)(blockIdx.x - e.chunk) * kChunk;
-  for (int64_t at = first + warp_id() * kBlock; at < min(first + kChunk, n); at += kWarps * kBlock) {
-    const int64_t s = (int64_t)e.at * kBlock + at;  // this block in the flat states
-    const bool whole = at + kBlock <= n;
-    float w[2][4], gr[2][4], m[2][4], v[2][4];
-    float sm = 0.f, su = 0.f;
-    if constexpr (EIGHT) sm = a.scale_m[s / kBlock], su = a.scale_u[s / kBlock];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int64_t i = at + h * 128 + lane * 4, f = s + h * 128 + lane * 4;
-      if (whole && wide) {
-        Four<P>::load(g + i, gr[h]);
-        if constexpr (!kMaster) Four<P>::load(p + i, w[h]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          gr[h][k] = i + k < n ? Four<P>::one(g[i + k]) : 0.f;
-          if constexpr (!kMaster) w[h][k] = i + k < n ? Four<P>::one(p[i + k]) : 0.f;
-        }
-      }
-      // the flat buffers are padded to whole blocks
-      if constexpr (kMaster) Four<float>::load(a.master + f, w[h]);
-      if constexpr (EIGHT) {
-        decode4(*reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.m) + f), m[h]);
-        decode4(*reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.v) + f), v[h]);
-      } else {
-        Four<float>::load(static_cast<const float*>(a.m) + f, m[h]);
-        Four<float>::load(static_cast<const float*>(a.v) + f, v[h]);
-      }
+  const bool wide = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) & (4 * sizeof(P) - 1)) == 0;
+  constexpr int kStep = kWarps * kBlock;
+  const int64_t first = (int64_t)(blockIdx.x - e.chunk) * kChunk, n = e.n;
+  int64_t at = first + warp_id() * kBlock;
+  const int64_t end = min(first + kChunk, n);
+  const int64_t fast = wide ? end - kBlock : at - 1;  // whole blocks begin up to here
+  const int64_t lane4 = lane_id() * 4, flat = (int64_t)e.at * kBlock + lane4;
+  if constexpr (EIGHT) {
+    // the next block's values are on their way while this one is computed: its scales wait for
+    // two warp maxima
+    Block<P, EIGHT> b;
+    if (at <= fast) b.load(a, p, g, at + lane4, flat + at);
+    for (; at <= fast; at += kStep) {
+      const Block<P, EIGHT> now = b;
+      if (at + kStep <= fast) b.load(a, p, g, at + kStep + lane4, flat + at + kStep);
+      whole_block<P, EIGHT>(a, gs, p, at + lane4, flat + at, now);
     }
-    float big_m = 0.f, big_u = 0.f;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if constexpr (EIGHT) {
-          m[h][k] = __fmul_rn(m[h][k], sm);
-          const float u = __fmul_rn(v[h][k], su);
-          v[h][k] = __fmul_rn(u, u);
-        }
-        float u;
-        update(a, gs, w[h][k], gr[h][k], m[h][k], v[h][k], u);
-        if constexpr (EIGHT) v[h][k] = u;
-        if (!whole && at + h * 128 + lane * 4 + k >= n) m[h][k] = v[h][k] = 0.f;  // padding stays 0
-        if constexpr (EIGHT) {
-          big_m = fmaxf(big_m, fabsf(m[h][k]));
-          big_u = fmaxf(big_u, v[h][k]);
-        }
-      }
-    float im = 0.f, iu = 0.f;
-    if constexpr (EIGHT) {
-      sm = __fmul_rn(warp_max(big_m), 1.0f / 448.0f);
-      su = __fmul_rn(warp_max(big_u), 1.0f / 448.0f);
-      im = inverse(sm), iu = inverse(su);
-      if (lane == 0) a.scale_m[s / kBlock] = sm, a.scale_u[s / kBlock] = su;
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int64_t i = at + h * 128 + lane * 4, f = s + h * 128 + lane * 4;
-      if (whole && wide) {
-        Four<P>::store(p + i, w[h]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (i + k < n) p[i + k] = Four<P>::back(w[h][k]);
-      }
-      if constexpr (kMaster) {
-        if (whole) {
-          Four<float>::store(a.master + f, w[h]);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (i + k < n) a.master[f + k] = w[h][k];
-        }
-      }
-      if constexpr (EIGHT) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          m[h][k] = __fmul_rn(m[h][k], im);
-          const float c = __fmul_rn(v[h][k], iu);
-          v[h][k] = v[h][k] > 0.f && iu > 0.f ? (c < 0x1p-9f ? 0x1p-9f : c) : c;
-        }
-        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.m) + f) = encode4(m[h]);
-        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.v) + f) = encode4(v[h]);
-      } else {
-        Four<float>::store(static_cast<float*>(a.m) + f, m[h]);
-        Four<float>::store(static_cast<float*>(a.v) + f, v[h]);
-      }
+  } else {
+    for (; at <= fast; at += kStep) {
+      Block<P, EIGHT> b;
+      b.load(a, p, g, at + lane4, flat + at);
+      whole_block<P, EIGHT>(a, gs, p, at + lane4, flat + at, b);
     }
   }
+  for (; at < end; at += kStep) odd_block<P, EIGHT>(a, gs, p, g, n, at + lane4, flat + at);
 }
 
 // Tables of two sizes: the parameters of a launch are copied with it, 2 KB for the usual handful
