@@ -111,45 +111,53 @@ struct Raw<T, 1> {
   }
 };
 
-// body(row, values of x[, values of dy]) for rows r, r + step, .. below end, U rows' loads in flight
+// body(row, values of x[, values of dy]) for rows r, r + step, .. below end.  The next U rows' loads
+// are in flight while U rows are computed.
 template <typename T, int V, int U, typename F>
 __device__ __forceinline__ void each_row(const T* x, int64_t stride, int r, int end, int step, F body) {
   Raw<T, V> a[U];
   float v[V];
-  for (; r + (U - 1) * step < end; r += U * step) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) a[u].load(x + (r + u * step) * stride);
+  for (int u = 0; u < U; ++u)
+    if (r + u * step < end) a[u].load(x + (r + u * step) * stride);
+  for (; r < end; r += U * step) {
+    Raw<T, V> now[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      a[u].get(v);
+      now[u] = a[u];
+      const int next = r + (U + u) * step;
+      if (next < end) a[u].load(x + next * stride);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (r + u * step >= end) break;
+      now[u].get(v);
       body(r + u * step, v);
     }
-  }
-  for (; r < end; r += step) {
-    a[0].load(x + r * stride);
-    a[0].get(v);
-    body(r, v);
   }
 }
 template <typename T, int V, int U, typename F>
 __device__ __forceinline__ void each_row(const T* x, const T* y, int64_t stride, int r, int end, int step, F body) {
   Raw<T, V> a[U], b[U];
   float v[V], w[V];
-  for (; r + (U - 1) * step < end; r += U * step) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) a[u].load(x + (r + u * step) * stride), b[u].load(y + (r + u * step) * stride);
+  for (int u = 0; u < U; ++u)
+    if (r + u * step < end) a[u].load(x + (r + u * step) * stride), b[u].load(y + (r + u * step) * stride);
+  for (; r < end; r += U * step) {
+    Raw<T, V> p[U], q[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      a[u].get(v);
-      b[u].get(w);
+      p[u] = a[u], q[u] = b[u];
+      const int next = r + (U + u) * step;
+      if (next < end) a[u].load(x + next * stride), b[u].load(y + next * stride);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (r + u * step >= end) break;
+      p[u].get(v);
+      q[u].get(w);
       body(r + u * step, v, w);
     }
-  }
-  for (; r < end; r += step) {
-    a[0].load(x + r * stride), b[0].load(y + r * stride);
-    a[0].get(v);
-    b[0].get(w);
-    body(r, v, w);
   }
 }
 
@@ -471,7 +479,7 @@ constexpr int kMaxGroups = 4096;  // a CTA holds a pair per group in shared memo
 
 // Chunks per SM: enough CTAs to fill the machine several times over (the last wave is short),
 // few enough that the partial sums stay small beside x.
-constexpr int kChunksPerSm = 8;
+constexpr int kChunksPerSm = 4;
 
 static Shape make_shape(const hi3d_group_norm_args* a, bool wide) {
   Shape s;

@@ -220,7 +220,13 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+# The current stream's handle without building a torch.cuda.Stream around it (a few microseconds).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream(t: torch.Tensor) -> int:
+    if _raw_stream is not None and t.is_cuda:
+        return _raw_stream(t.get_device())
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
@@ -229,7 +235,7 @@ _HERE = contextlib.nullcontext()
 
 def on_device(t: torch.Tensor):
     """Context in which the device of ``t`` is current: the library launches on the current device."""
-    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def require_cuda(*ts: torch.Tensor | None) -> None:

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import itertools
 import math
 
 import torch
@@ -319,8 +320,9 @@ def flash_attn_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
 # ---------------------------------------------------------------------------
 def _aligned(t: torch.Tensor) -> bool:
     """Whether the kernels' 16-byte loads and TMA boxes can address ``t`` as it lies."""
-    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-            and all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1])))
+    if t.data_ptr() & 15 or t.stride(-1) != 1:
+        return False
+    return t.is_contiguous() or all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1]))
 
 
 def _fit(t: torch.Tensor) -> torch.Tensor:
@@ -332,11 +334,12 @@ def _fit(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _steps(t: torch.Tensor, order: tuple[int, ...]) -> list[int]:
-    """Element strides of the (row, head[, batch]) axes ``order``.  An axis of one element may have
-    any stride, which the kernels would refuse: a row or head then steps by one head, a batch by 0
-    (one set for every sequence)."""
-    return [t.stride(i) if t.shape[i] != 1 else 0 if n == 2 else t.shape[-1] for n, i in enumerate(order)]
+def _steps(t: torch.Tensor, row: int, head: int, batch: int | None = None) -> tuple[int, int, int]:
+    """Element strides of these axes.  An axis of one element may have any stride, which the kernels
+    would refuse: a row or head then steps by one head, a batch by 0 (one set for every sequence)."""
+    n, s = t.shape, t.stride()
+    return (s[row] if n[row] != 1 else n[-1], s[head] if n[head] != 1 else n[-1],
+            0 if batch is None or n[batch] == 1 else s[batch])
 
 
 def _check_train(q, k, v, heads: int, kv_heads: int, dim: int, same_kv: bool) -> None:
@@ -404,14 +407,11 @@ def flash_attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale
         if nq == 0 or batch == 0:
             return out, lse
         q, k, v = _fit(q), _fit(k), _fit(v)
-        qr, qh, qb = _steps(q, (2, 1, 0) if q_layout == "bhnd" else (1, 2, 0))
-        kr, kh, kb = _steps(k, (2, 1, 0))
-        vr, vh, vb = _steps(v, (2, 1, 0))
         args = _lib.AttnArgs(
-            q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(),
-            q_row=qr, q_head=qh, q_batch=qb, k_row=kr, k_head=kh, k_batch=kb, v_row=vr, v_head=vh, v_batch=vb,
-            o_row=heads * dim, o_head=dim, o_batch=nq * heads * dim, nq=nq, nk=k.shape[2], max_seqlen_q=nq,
-            num_seqs=batch, heads=heads, head_dim=dim, dtype=_lib.dtype_code(q), scale=float(scale))
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+            *(_steps(q, 2, 1, 0) if q_layout == "bhnd" else _steps(q, 1, 2, 0)), *_steps(k, 2, 1, 0),
+            *_steps(v, 2, 1, 0), heads * dim, dim, nq * heads * dim, None, None, nq, k.shape[2], nq, batch, heads, dim,
+            _lib.dtype_code(q), float(scale))
         _forward_lse(args, k.shape[1], lse, k_splits)
     return out, lse
 
@@ -440,13 +440,10 @@ def flash_attn_varlen_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_
         if int(max_seqlen_q) < 1:
             raise ValueError("max_seqlen_q must be at least the longest query sequence")
         q, k, v = _fit(q), _fit(k), _fit(v)
-        (qr, qh), (kr, kh), (vr, vh) = (_steps(t, (0, 1)) for t in (q, k, v))
         args = _lib.AttnArgs(
-            q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(),
-            q_row=qr, q_head=qh, k_row=kr, k_head=kh, v_row=vr, v_head=vh, o_row=heads * dim, o_head=dim,
-            cu_seqlens_q=cu_q.data_ptr(), cu_seqlens_k=_lib.ptr(cu_k), nq=tq, nk=tk,
-            max_seqlen_q=min(int(max_seqlen_q), tq), num_seqs=num_seqs, heads=heads, head_dim=dim,
-            dtype=_lib.dtype_code(q), scale=float(scale))
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *_steps(q, 0, 1), *_steps(k, 0, 1),
+            *_steps(v, 0, 1), heads * dim, dim, 0, cu_q.data_ptr(), _lib.ptr(cu_k), tq, tk,
+            min(int(max_seqlen_q), tq), num_seqs, heads, dim, _lib.dtype_code(q), float(scale))
         _forward_lse(args, k.shape[1], lse, k_splits)
     return out, lse
 
@@ -462,34 +459,41 @@ def _varlen_shape(q, k, v, cu_seqlens_q, cu_seqlens_k):
     return cu_q, cu_k, heads, dim
 
 
-def _grads(out, like) -> list[torch.Tensor]:
+def _grads(given, like) -> list[torch.Tensor]:
     """The gradients' tensors: the caller's, checked, or new contiguous ones."""
     got = []
-    for name, given, t in zip(("dq", "dk", "dv"), out or (None, None, None), like):
-        if given is None:
-            given = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        elif given.shape != t.shape or given.dtype != t.dtype or given.device != t.device or not _aligned(given):
+    for name, g, t in zip(("dq", "dk", "dv"), given or (None, None, None), like):
+        if g is None:
+            g = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        elif g.shape != t.shape or g.dtype != t.dtype or g.device != t.device or not _aligned(g):
             raise ValueError(f"{name} must have the shape, dtype and device of its input, rows contiguous over the "
                              "head dimension and 16-byte aligned")
-        got.append(given)
+        got.append(g)
     return got
 
 
-def _backward(grad_out, q, k, v, out, lse, grads, strides, **sizes) -> None:
-    args = _lib.AttnBwdArgs(dtype=_lib.dtype_code(q), **sizes)
-    for name, t in zip(("q", "k", "v", "out", "dout", "lse", "dq", "dk", "dv"),
-                       (q, k, v, out, grad_out, lse, *grads)):
-        setattr(args, name, t.data_ptr())
-    for name, (row, head, batch) in strides.items():
-        setattr(args, f"{name}_row", row)
-        setattr(args, f"{name}_head", head)
-        setattr(args, f"{name}_batch", batch)
-    lib = _lib.load()
+@functools.lru_cache(maxsize=256)
+def _backward_workspace(packed_q: bool, packed_k: bool, shared: bool, sizes: tuple, device: int) -> int:
+    """Bytes of workspace for these sizes (asked once per sizes and device): only the presence of
+    pointers and the key batch stride count beside them."""
+    args = _lib.AttnBwdArgs(*[16] * 9, *[8] * 24, 16 if packed_q else None, 16 if packed_k else None, *sizes)
+    args.k_batch = 0 if shared else 8
     nbytes = ctypes.c_int64()
-    _lib.check(lib.hi3d_flash_attn_bwd_workspace_size(ctypes.byref(args), ctypes.byref(nbytes)),
+    _lib.check(_lib.load().hi3d_flash_attn_bwd_workspace_size(ctypes.byref(args), ctypes.byref(nbytes)),
                "flash_attention_backward workspace", launched=False)
-    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=q.device)
-    rc = lib.hi3d_flash_attn_bwd(ctypes.byref(args), ws.data_ptr(), ws.numel(), _lib.stream(q))
+    return nbytes.value
+
+
+def _backward(tensors, lse, strides, cu_q, cu_k, sizes) -> None:
+    """``tensors``: q, k, v, out, grad_out, dq, dk, dv with their ``strides``; ``sizes``: nq, nk, num_seqs,
+    heads, kv_heads, head_dim, dtype, scale."""
+    q, k, v, out, grad_out, dq, dk, dv = tensors
+    args = _lib.AttnBwdArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), grad_out.data_ptr(),
+                            lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                            *itertools.chain.from_iterable(strides), _lib.ptr(cu_q), _lib.ptr(cu_k), *sizes)
+    nbytes = _backward_workspace(cu_q is not None, cu_k is not None, args.k_batch == 0, sizes, q.get_device())
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    rc = _lib.load().hi3d_flash_attn_bwd(ctypes.byref(args), ws.data_ptr(), nbytes, _lib.stream(q))
     _lib.check(rc, "flash_attention_backward")
 
 
@@ -521,16 +525,15 @@ def flash_attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.T
             for t in grads:
                 t.zero_()
             return dq, dk, dv
-        q, k, v = _fit(q), _fit(k), _fit(v)
-        rows = lambda t: _fit(t.unflatten(2, (heads, dim)))  # noqa: E731
-        out, grad_out, lse = rows(out), rows(grad_out), lse.contiguous()
-        order = (2, 1, 0) if q_layout == "bhnd" else (1, 2, 0)
-        _backward(grad_out, q, k, v, out, lse, grads,
-                  {"q": _steps(q, order), "dq": _steps(dq, order), "o": _steps(out, (1, 2, 0)),
-                   "do": _steps(grad_out, (1, 2, 0)), "k": _steps(k, (2, 1, 0)), "v": _steps(v, (2, 1, 0)),
-                   "dk": _steps(dk, (2, 1, 0)), "dv": _steps(dv, (2, 1, 0))},
-                  nq=nq, nk=k.shape[2], num_seqs=batch, heads=heads, kv_heads=k.shape[1], head_dim=dim,
-                  scale=float(scale))
+        q, k, v, lse = _fit(q), _fit(k), _fit(v), lse.contiguous()
+        out = _fit(out.view(batch, nq, heads, dim) if out.is_contiguous() else out.unflatten(2, (heads, dim)))
+        grad_out = _fit(grad_out.view(batch, nq, heads, dim) if grad_out.is_contiguous()
+                        else grad_out.unflatten(2, (heads, dim)))
+        axes = (2, 1, 0) if q_layout == "bhnd" else (1, 2, 0)
+        _backward((q, k, v, out, grad_out, dq, dk, dv), lse,
+                  (_steps(q, *axes), _steps(k, 2, 1, 0), _steps(v, 2, 1, 0), _steps(out, 1, 2, 0),
+                   _steps(grad_out, 1, 2, 0), _steps(dq, *axes), _steps(dk, 2, 1, 0), _steps(dv, 2, 1, 0)),
+                  None, None, (nq, k.shape[2], batch, heads, k.shape[1], dim, _lib.dtype_code(q), float(scale)))
     return dq, dk, dv
 
 
@@ -551,11 +554,7 @@ def flash_attn_varlen_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch
             for t in grads:
                 t.zero_()
             return dq, dk, dv
-        q, k, v, out, grad_out, lse = _fit(q), _fit(k), _fit(v), _fit(out), _fit(grad_out), lse.contiguous()
-        step = lambda t: [*_steps(t, (0, 1)), 0]  # noqa: E731
-        _backward(grad_out, q, k, v, out, lse, grads,
-                  {"q": step(q), "k": step(k), "v": step(v), "o": step(out), "do": step(grad_out), "dq": step(dq),
-                   "dk": step(dk), "dv": step(dv)},
-                  cu_seqlens_q=cu_q.data_ptr(), cu_seqlens_k=_lib.ptr(cu_k), nq=tq, nk=k.shape[0],
-                  num_seqs=cu_q.numel() - 1, heads=heads, kv_heads=k.shape[1], head_dim=dim, scale=float(scale))
+        tensors = (_fit(q), _fit(k), _fit(v), _fit(out), _fit(grad_out), dq, dk, dv)
+        _backward(tensors, lse.contiguous(), [_steps(t, 0, 1) for t in tensors], cu_q, cu_k,
+                  (tq, k.shape[0], cu_q.numel() - 1, heads, k.shape[1], dim, _lib.dtype_code(q), float(scale)))
     return dq, dk, dv

@@ -62,11 +62,10 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor], exp_avg: t
     dtype, device = first.dtype, first.device
     if dtype not in DTYPES:
         raise ValueError(f"adamw_step takes float32, float16 or bfloat16 tensors, got {dtype}")
-    for p, g in zip(params, grads):
-        if (p.dtype is not dtype or g.dtype is not dtype or p.device != device or g.device != device
-                or p.shape != g.shape or not p.is_contiguous() or not g.is_contiguous()):
-            raise ValueError(f"params and grads must be contiguous, of one dtype and device and alike in pairs: "
-                             f"{tuple(p.shape)} {p.dtype} {p.device}, {tuple(g.shape)} {g.dtype} {g.device}")
+    both = [*params, *grads]
+    if ({t.dtype for t in both} != {dtype} or {t.get_device() for t in both} != {first.get_device()}
+            or not all(map(torch.Tensor.is_contiguous, both)) or any(p.shape != g.shape for p, g in zip(params, grads))):
+        raise ValueError("params and grads must be contiguous, of one dtype and device and alike in pairs")
     numels = [p.numel() for p in params]
     if offsets is None:
         offsets, total = state_layout(numels)
@@ -91,8 +90,8 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor], exp_avg: t
         return
     n = len(numels)
     args = _lib.AdamWArgs(
-        params=(ctypes.c_void_p * n)(*[p.data_ptr() for p in params]),
-        grads=(ctypes.c_void_p * n)(*[g.data_ptr() for g in grads]),
+        params=(ctypes.c_void_p * n)(*map(torch.Tensor.data_ptr, params)),
+        grads=(ctypes.c_void_p * n)(*map(torch.Tensor.data_ptr, grads)),
         numels=(ctypes.c_int64 * n)(*numels), offsets=(ctypes.c_int64 * n)(*offsets), master=_lib.ptr(master),
         exp_avg=exp_avg.data_ptr(), exp_avg_sq=exp_avg_sq.data_ptr(), scales=_lib.ptr(scales),
         grad_scale=_lib.ptr(grad_scale), total=total, step=int(step), lr=float(lr), beta1=float(betas[0]),

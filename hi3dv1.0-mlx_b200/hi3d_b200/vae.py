@@ -17,6 +17,7 @@ its helpers:
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import numpy as np
 import torch
@@ -97,20 +98,35 @@ def _norm_args(x, weight, bias, groups: int, act, eps: float, offsets, mean, rst
             raise ValueError("offsets must be a one-dimensional int32 (or int64) tensor of samples + 1 row offsets")
         offsets = offsets.to(torch.int32).contiguous()
         samples = offsets.numel() - 1
-    if any(t.device != x.device for t in (weight, bias, offsets, mean, rstd) if t is not None):
-        raise ValueError("all tensors must be on the device of x")
+    for t in (weight, bias, offsets, mean, rstd):
+        if t is not None and t.get_device() != x.get_device():
+            raise ValueError("all tensors must be on the device of x")
     return samples, offsets, _lib.GroupNormArgs(
         x=x.data_ptr(), weight=weight.data_ptr(), bias=bias.data_ptr(), offsets=_lib.ptr(offsets), rows=rows,
         channels=c, samples=samples, groups=groups, act=int(act is not None), dtype=_lib.dtype_code(x), eps=float(eps))
 
 
-def _norm_call(name: str, args, x) -> None:
-    lib = _lib.load()
+@functools.lru_cache(maxsize=256)
+def _norm_workspace(rows: int, channels: int, samples: int, groups: int, act: int, dtype: int, device: int) -> int:
+    """Bytes of workspace for these sizes (asked once per sizes and device)."""
+    args = _lib.GroupNormArgs(rows=rows, channels=channels, samples=samples, groups=groups, act=act, dtype=dtype, eps=1.0)
+    if rows % samples:
+        args.offsets = 1  # packed samples: only the pointer's presence counts here
     nb = ctypes.c_int64()
-    _lib.check(lib.hi3d_group_norm_act_workspace_size(ctypes.byref(args), ctypes.byref(nb)), name, launched=False)
-    ws = torch.empty(nb.value, dtype=torch.uint8, device=x.device)
-    rc = getattr(lib, name)(ctypes.byref(args), ws.data_ptr(), ws.numel(), _lib.stream(x))
+    _lib.check(_lib.load().hi3d_group_norm_act_workspace_size(ctypes.byref(args), ctypes.byref(nb)), "group_norm_act",
+               launched=False)
+    return nb.value
+
+
+def _norm_call(name: str, args, x) -> None:
+    size = _norm_workspace(args.rows, args.channels, args.samples, args.groups, args.act, args.dtype, x.get_device())
+    ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+    rc = getattr(_lib.load(), name)(ctypes.byref(args), ws.data_ptr(), size, _lib.stream(x))
     _lib.check(rc, name)
+
+
+def _fp32(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype is torch.float32 and t.is_contiguous() else t.detach().float().contiguous()
 
 
 def group_norm_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, groups: int, eps: float = 1e-6,
@@ -123,11 +139,12 @@ def group_norm_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, gr
     (some may be empty; they must cover all rows), or ``[samples, ..., C]``.  ``weight, bias`` ``[C]``.
     """
     _lib.require_cuda(x, weight, bias, offsets)
-    x, weight, bias = x.contiguous(), weight.detach().float().contiguous(), bias.detach().float().contiguous()
+    x, weight, bias = x.contiguous(), _fp32(weight), _fp32(bias)
     with _lib.on_device(x):
         samples, offsets, args = _norm_args(x, weight, bias, groups, act, eps, offsets, None, None)
         y = torch.empty_like(x)
-        mean, rstd = torch.empty((2, samples, groups), dtype=torch.float32, device=x.device)
+        mean = torch.empty((samples, groups), dtype=torch.float32, device=x.device)
+        rstd = torch.empty((samples, groups), dtype=torch.float32, device=x.device)
         if samples:
             args.y, args.mean, args.rstd = y.data_ptr(), mean.data_ptr(), rstd.data_ptr()
             _norm_call("hi3d_group_norm_act_fwd", args, x)
@@ -145,13 +162,14 @@ def group_norm_act_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tenso
     if mean.dim() != 2 or mean.shape != rstd.shape or mean.dtype != torch.float32 or rstd.dtype != torch.float32:
         raise ValueError("mean and rstd must be the float32 [samples, groups] of the forward pass")
     x, dy, mean, rstd = x.contiguous(), dy.contiguous(), mean.contiguous(), rstd.contiguous()
-    weight, bias = weight.detach().float().contiguous(), bias.detach().float().contiguous()
+    weight, bias = _fp32(weight), _fp32(bias)
     with _lib.on_device(x):
         samples, offsets, args = _norm_args(x, weight, bias, mean.shape[1], act, 1.0, offsets, mean, rstd)
         if mean.shape[0] != samples:
             raise ValueError(f"mean and rstd are of {mean.shape[0]} samples, x and offsets of {samples}")
         dx = torch.empty_like(x)
-        dweight, dbias = torch.empty((2, x.shape[-1]), dtype=torch.float32, device=x.device)
+        dweight = torch.empty(x.shape[-1], dtype=torch.float32, device=x.device)
+        dbias = torch.empty(x.shape[-1], dtype=torch.float32, device=x.device)
         if samples:
             args.mean, args.rstd, args.dy, args.dx = mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), dx.data_ptr()
             args.dweight, args.dbias = dweight.data_ptr(), dbias.data_ptr()
