@@ -36,7 +36,7 @@ constexpr int kRows = 128;           // stationary rows of a CTA
 constexpr float kLog2e = 1.4426950408889634f;
 // Of the 16 pairs of exponentials that a thread takes, those evaluated on the FMA pipe instead of
 // the MUFU unit.
-constexpr int kEmuPairs = 4;
+constexpr int kEmuPairs = 6;
 // fp16 only: P is stored times 2^kPShift (P <= 1, so at most 256), which keeps probabilities
 // down to 2^-22 normal numbers; dV is divided by it at the end.
 constexpr int kPShift = 8;
@@ -496,7 +496,7 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
           const uint64_t x =
               f2_fma(f2_pack(__uint_as_float(sv[u][2 * e]), __uint_as_float(sv[u][2 * e + 1])), scale2x2, bias);
           float p0, p1;
-          if (e % 4 == 0 && e < 4 * kEmuPairs) {
+          if (e * kEmuPairs % 16 < kEmuPairs) {  // spread over the 16
             f2_unpack(f2_exp2_poly(x), p0, p1);
           } else {
             f2_unpack(x, p0, p1);
