@@ -67,10 +67,17 @@ int encode_tmap(CUtensorMap* map, CUtensorMapDataType type, int rank, const void
   EncodeTiledFn fn = encode_fn();
   if (!fn) return set_error(HI3D_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   cuuint32_t elem_strides[5] = {1, 1, 1, 1, 1};
-  CUresult r = fn(map, type, (cuuint32_t)rank, const_cast<void*>(base), (const cuuint64_t*)dims,
-                  (const cuuint64_t*)strides_bytes, (const cuuint32_t*)box, elem_strides,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return fn(map, type, (cuuint32_t)rank, const_cast<void*>(base), (const cuuint64_t*)dims,
+              (const cuuint64_t*)strides_bytes, (const cuuint32_t*)box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  // A thread whose first CUDA call this is (autograd's, for one) has no context until the runtime
+  // binds its device's.
+  int dev = 0;
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess)
+    r = encode();
   if (r != CUDA_SUCCESS)
     return set_error(HI3D_ERR_INVALID_ARGUMENT, "cuTensorMapEncodeTiled failed (%d): rank %d dims %llu,%llu", (int)r,
                      rank, (unsigned long long)dims[0], (unsigned long long)(rank > 1 ? dims[1] : 0));

@@ -3,7 +3,8 @@
 Same signatures as the functions the upstream code calls
 (src/sparc3d/nn/sparse/attention/full_attn.py:56-76) and as the reference's CPU shim
 (src/hi3d_mac/torch_backend/attention.py:77-109), including its errors for causal or
-dropout attention.  Inputs are fp16/bf16 CUDA tensors, as for flash-attn itself.
+dropout attention.  Inputs are fp16/bf16 CUDA tensors, as for flash-attn itself.  Where a gradient is
+wanted they run the training pair (:mod:`hi3d_b200.training`), so the upstream model can be fine-tuned.
 """
 
 from __future__ import annotations
@@ -11,6 +12,11 @@ from __future__ import annotations
 import torch
 
 from .. import attention as _attn
+from .. import training as _train
+
+
+def _wants_grad(*ts: torch.Tensor) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in ts)
 
 
 def flash_attn_varlen_qkvpacked_func(qkv: torch.Tensor, cu_seqlens: torch.Tensor, max_seqlen: int,
@@ -19,8 +25,10 @@ def flash_attn_varlen_qkvpacked_func(qkv: torch.Tensor, cu_seqlens: torch.Tensor
     """Self-attention over packed ``[T, 3, H, D]`` sequences; returns ``[T, H, D]``."""
     if causal or dropout_p:
         raise NotImplementedError("causal or dropout attention is not used by Hi3D")
+    scale = qkv.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale
+    if _wants_grad(qkv):
+        return _train.flash_attn_varlen_qkvpacked(qkv, cu_seqlens.to(qkv.device), int(max_seqlen), scale)
     q, k, v = qkv.unbind(1)
-    scale = q.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale
     return _attn.flash_attn_varlen(q, k, v, cu_seqlens, cu_seqlens, int(max_seqlen), scale)
 
 
@@ -31,7 +39,10 @@ def flash_attn_varlen_kvpacked_func(q: torch.Tensor, kv: torch.Tensor, cu_seqlen
     """Cross-attention of packed queries ``[T, H, D]`` over packed ``[S, 2, H, D]``."""
     if causal or dropout_p:
         raise NotImplementedError("causal or dropout attention is not used by Hi3D")
-    k, v = kv.unbind(1)
     scale = q.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale
+    if _wants_grad(q, kv):
+        return _train.flash_attn_varlen_kvpacked(q, kv, cu_seqlens_q.to(q.device), cu_seqlens_k.to(q.device),
+                                                 int(max_seqlen_q), scale)
+    k, v = kv.unbind(1)
     return _attn.flash_attn_varlen(q, k, v, cu_seqlens_q.to(q.device), cu_seqlens_k.to(q.device),
                                    int(max_seqlen_q), scale)

@@ -1,0 +1,109 @@
+"""The training operators' refusals and host arithmetic, which need no GPU."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from hi3d_b200 import _lib, attention, optim, vae
+
+
+def _bwd(**kw):
+    a = _lib.AttnBwdArgs(*[16] * 9, *[64] * 24, None, None, 5, 7, 1, 2, 2, 64, _lib.F16, 0.125)
+    for name, value in kw.items():
+        setattr(a, name, value)
+    n = ctypes.c_int64(-1)
+    return _lib.load().hi3d_flash_attn_bwd_workspace_size(ctypes.byref(a), ctypes.byref(n)), n.value
+
+
+def test_attention_backward_arguments():
+    assert _bwd()[0] == _lib.OK and _bwd()[1] > 0
+    for kw in (dict(q=None), dict(lse=None), dict(dk=None), dict(dtype=_lib.F32), dict(nq=0), dict(nk=0),
+               dict(num_seqs=0), dict(kv_heads=0), dict(heads=3), dict(q=24), dict(dv_row=60), dict(k_head=-8),
+               dict(cu_seqlens_k=16), dict(nq=1 << 31)):
+        assert _bwd(**kw)[0] == _lib.ERR_INVALID_ARGUMENT, kw
+    assert _bwd(head_dim=80)[0] == _lib.ERR_UNSUPPORTED
+    a = _lib.AttnBwdArgs(*[16] * 9, *[64] * 24, None, None, 5, 7, 1, 2, 2, 64, _lib.F16, 0.125)
+    assert _lib.load().hi3d_flash_attn_bwd(ctypes.byref(a), None, 0, None) == _lib.ERR_CAPACITY
+    assert _lib.load().hi3d_flash_attn_bwd(ctypes.byref(a), 256, 64, None) == _lib.ERR_CAPACITY
+
+
+def test_attention_backward_workspace_covers_a_tile_per_sequence():
+    """Packed queries: each sequence's statistics begin at a 128-row tile of their own (8 bytes a row
+    and head, in tiles: rows / 128 + sequences of them)."""
+    rc, n = _bwd(cu_seqlens_q=16, cu_seqlens_k=16, nq=1000, nk=1000, num_seqs=6)
+    assert rc == _lib.OK and n >= (1000 // 128 + 6) * 128 * 8 * 2
+
+
+def test_attention_forward_lse_arguments():
+    lib = _lib.load()
+    a = _lib.AttnArgs(q=16, k=16, v=16, out=16, head_dim=64, dtype=0, heads=4, num_seqs=1, nq=1, nk=1)
+    call = lambda kv, lse, splits: lib.hi3d_flash_attn_fwd_lse(ctypes.byref(a), kv, lse, splits, None, 0, None)  # noqa: E731
+    assert call(3, 16, 1) == _lib.ERR_INVALID_ARGUMENT
+    assert call(4, None, 1) == _lib.ERR_INVALID_ARGUMENT
+    assert call(4, 16, 65) == _lib.ERR_INVALID_ARGUMENT
+    assert call(4, 16, 2) == _lib.ERR_CAPACITY
+    a.nk = 0
+    assert call(4, 16, 1) == _lib.ERR_INVALID_ARGUMENT
+
+
+def _norm(**kw):
+    a = _lib.GroupNormArgs(*[16] * 3, None, *[16] * 7, 10, 64, 1, 8, 1, _lib.F16, 1e-6)
+    for name, value in kw.items():
+        setattr(a, name, value)
+    n = ctypes.c_int64(-1)
+    return _lib.load().hi3d_group_norm_act_workspace_size(ctypes.byref(a), ctypes.byref(n)), n.value
+
+
+def test_group_norm_arguments():
+    assert _norm()[0] == _lib.OK and _norm()[1] > 0
+    for kw in (dict(rows=-1), dict(samples=0), dict(samples=3), dict(groups=7), dict(groups=0), dict(channels=0),
+               dict(dtype=_lib.I32), dict(act=2), dict(eps=0.0), dict(rows=0x7ff00001)):
+        assert _norm(**kw)[0] == _lib.ERR_INVALID_ARGUMENT, kw
+    for kw in (dict(channels=8192, groups=8192), dict(channels=1 << 21), dict(samples=70000, rows=70000)):
+        assert _norm(**kw)[0] == _lib.ERR_UNSUPPORTED, kw
+    a = _lib.GroupNormArgs(rows=10, channels=64, samples=1, groups=8, act=1, dtype=_lib.F16, eps=1e-6)
+    lib = _lib.load()
+    assert lib.hi3d_group_norm_act_fwd(ctypes.byref(a), None, 0, None) == _lib.ERR_INVALID_ARGUMENT
+    assert lib.hi3d_group_norm_act_bwd(ctypes.byref(a), None, 0, None) == _lib.ERR_INVALID_ARGUMENT
+    a.weight = a.bias = a.mean = a.rstd = a.x = a.y = 16
+    assert lib.hi3d_group_norm_act_fwd(ctypes.byref(a), None, 0, None) == _lib.ERR_CAPACITY
+
+
+def _adamw(numels=(300, 5), offsets=(0, 512), ptrs=(16, 32), **kw):
+    n = len(numels)
+    a = _lib.AdamWArgs((ctypes.c_void_p * n)(*ptrs), (ctypes.c_void_p * n)(*ptrs), (ctypes.c_int64 * n)(*numels),
+                       (ctypes.c_int64 * n)(*offsets), None, 16, 16, None, None, 768, 1, 1e-3, 0.9, 0.999, 1e-8, 0.01,
+                       n, _lib.F32, 32)
+    for name, value in kw.items():
+        setattr(a, name, value)
+    return _lib.load().hi3d_adamw_step(ctypes.byref(a), None)
+
+
+def test_adamw_arguments():
+    for kw in (dict(step=0), dict(lr=-1.0), dict(beta1=1.0), dict(beta2=-0.1), dict(eps=-1e-8), dict(weight_decay=-1.0),
+               dict(dtype=_lib.I32), dict(dtype=_lib.F16), dict(master=16), dict(state_bits=16), dict(state_bits=8),
+               dict(scales=16), dict(exp_avg=None), dict(exp_avg=20), dict(total=700), dict(total=512),
+               dict(offsets=(0, 500)), dict(offsets=(0, -256)), dict(offsets=(0, 1024)), dict(numels=(300, -1)),
+               dict(ptrs=(16, 30)), dict(ptrs=(16, None)), dict(lr=float("nan"))):
+        assert _adamw(**kw) == _lib.ERR_INVALID_ARGUMENT, kw
+    assert _adamw(count=0) == _lib.OK
+    assert _lib.load().hi3d_adamw_step(None, None) == _lib.ERR_INVALID_ARGUMENT
+
+
+def test_state_layout_aligns_each_tensor_to_a_block():
+    offsets, total = optim.state_layout([1, 256, 257, 0, 5])
+    assert offsets == [0, 256, 512, 1024, 1024] and total == 1280
+    assert optim.state_layout([]) == ([], 0)
+
+
+def test_no_cpu_path():
+    t = torch.zeros(1, 1, 4, 64, dtype=torch.float16)
+    with pytest.raises(ValueError):
+        attention.flash_attention_lse(t, t, t, 0.1)
+    with pytest.raises(ValueError):
+        vae.group_norm_act(torch.zeros(4, 8), torch.ones(8), torch.zeros(8), 2)
+    with pytest.raises(ValueError):
+        optim.adamw_step([torch.zeros(4)], [torch.zeros(4)], torch.zeros(256), torch.zeros(256), step=1, lr=1e-3)
