@@ -81,6 +81,12 @@ struct Cfg {
   static constexpr int STAGE = 2 * Y_BYTES;
   static constexpr int T_COL = 2 * BN;
   static constexpr int ACC_COL = 3 * BN;  // dK or dQ, then dV
+  // Stationary operands that fit beside them are copied into TMEM and read from there: a 64-column
+  // product with both operands in shared memory is bound by its reads (50 cycles a K step where
+  // 33 would do).  With room for one it is X2.
+  static constexpr int X_COL = ACC_COL + (KV ? 2 : 1) * D;
+  static constexpr int X_FIT = BN == 64 ? (512 - X_COL) / (D / 2) : 0;
+  static constexpr bool X1_TMEM = X_FIT >= 2, X2_TMEM = X_FIT >= 1;
   static constexpr int SMEM = 2 * X_BYTES + NST * STAGE + NST * BN * 8 + 1024 /*align*/ + 256 /*barriers*/;
   static_assert(ACC_COL + (KV ? 2 : 1) * D <= 512, "TMEM budget");
   static_assert(SMEM <= 232448, "shared memory budget");
@@ -88,6 +94,7 @@ struct Cfg {
 
 struct Barriers {
   uint64_t x_full;
+  uint64_t x_tmem;    // the stationary operands are in TMEM
   uint64_t full[4];
   uint64_t empty[4];
   uint64_t tail;      // a ragged block, before its rows past the end are cleared
@@ -314,6 +321,7 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
 
   if (threadIdx.x == 0) {
     mbar_init(&bar->x_full, 1);
+    mbar_init(&bar->x_tmem, 4 * kGroups);
     for (int s = 0; s < NST; ++s) {
       mbar_init(&bar->full[s], 1);
       mbar_init(&bar->empty[s], 1);
@@ -402,14 +410,22 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
       const uint64_t dY = smem_desc(smem_u32(sY), 16, 1024, kLayoutSW128);
       const uint64_t dYt = smem_desc(smem_u32(sY), C::Y_CHUNK, 1024, kLayoutSW128);  // rows as the K dimension
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-      auto product = [&](uint32_t d, uint64_t x, uint32_t y_off, uint64_t* done) {  // d = x y^T over the channels
+      // d = x y^T over the channels, x in TMEM (x_col) or in shared memory
+      auto product = [&](auto in_tmem, uint32_t d, uint64_t x, uint32_t x_col, uint32_t y_off, uint64_t* done) {
         if (!elect_one()) return;
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
-          mma_f16_ss(d, x + (((ks >> 2) * C::X_CHUNK + (ks & 3) * 32) >> 4),
-                     dY + ((y_off + (ks >> 2) * C::Y_CHUNK + (ks & 3) * 32) >> 4), idesc_s, ks > 0 ? 1u : 0u);
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint64_t y = dY + ((y_off + (ks >> 2) * C::Y_CHUNK + (ks & 3) * 32) >> 4);
+          if constexpr (decltype(in_tmem)::value)
+            mma_f16_ts(d, x_col + ks * 8, y, idesc_s, ks > 0 ? 1u : 0u);
+          else
+            mma_f16_ss(d, x + (((ks >> 2) * C::X_CHUNK + (ks & 3) * 32) >> 4), y, idesc_s, ks > 0 ? 1u : 0u);
+        }
         tc_commit(done);
       };
+      using X1InTmem = std::integral_constant<bool, C::X1_TMEM>;
+      using X2InTmem = std::integral_constant<bool, C::X2_TMEM>;
+      const uint32_t x2_col = tm + C::X_COL, x1_col = x2_col + D / 2;
       // acc += a y over the block's rows; a: HC / 2 TMEM columns in each group of the S buffer
       auto accumulate = [&](uint32_t d, uint32_t a, uint32_t y_off, bool more) {
 #pragma unroll
@@ -418,18 +434,19 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
           mma_f16_ts(d, a + group * HC + k * 8, dYt + ((y_off + ks * 2048) >> 4), idesc_acc, more || ks > 0 ? 1u : 0u);
         }
       };
-      bool ok = role_id == 2 || mbar_wait(&bar->x_full, 0, abort, 310);
+      bool ok = role_id == 2 || mbar_wait(C::X2_TMEM ? &bar->x_tmem : &bar->x_full, 0, abort, 310);
+      if (C::X2_TMEM && !C::X1_TMEM && ok && role_id == 0) ok = mbar_wait(&bar->x_full, 0, abort, 310);
       for (int j = 0; ok && j < n; ++j) {
         const uint32_t y = (j % NST) * C::STAGE;
         if (!(ok = mbar_wait(&bar->full[j % NST], (j / NST) & 1, abort, 311))) break;
         if (role_id == 0) {  // S(j), once the products that read P(j - 2), dS(j - 2) from this buffer are done
           if (j > 1 && !(ok = mbar_wait(&bar->acc_done[j & 1], ((j - 2) >> 1) & 1, abort, 314))) break;
           tc_fence_after();
-          product(tm + (j & 1) * BN, dX1, y, &bar->s_full[j & 1]);
+          product(X1InTmem(), tm + (j & 1) * BN, dX1, x1_col, y, &bar->s_full[j & 1]);
         } else if (role_id == 1) {  // T(j), once T(j - 1) has been read
           if (j > 0 && !(ok = mbar_wait(&bar->t_free, (j - 1) & 1, abort, 312))) break;
           tc_fence_after();
-          product(tm + C::T_COL, dX2, y + C::Y_BYTES, &bar->t_full);
+          product(X2InTmem(), tm + C::T_COL, dX2, x2_col, y + C::Y_BYTES, &bar->t_full);
         } else {  // the accumulators, once P(j), dS(j) are written
           if (!(ok = mbar_wait(&bar->pd_full[j & 1], (j >> 1) & 1, abort, 313))) break;
           tc_fence_after();
@@ -552,6 +569,31 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
       return true;
     };
     bool ok = true;
+    if constexpr (C::X2_TMEM) {
+      // this warp's rows of the stationary operands, the column groups one chunk of 64 channels each
+      if ((ok = mbar_wait(&bar->x_full, 0, abort, 324))) {
+#pragma unroll
+        for (int x = 0; x < (C::X1_TMEM ? 2 : 1); ++x)
+          for (int c = group; c < C::NCH; c += kGroups) {
+            const uint8_t* src = (x == 0 ? sX2 : sX1) + c * C::X_CHUNK + row * 128;
+            const uint32_t dst = tmem + lane_addr + C::X_COL + x * (D / 2) + c * 32;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              if (c * 64 + half * 32 >= D) break;
+              uint32_t v[16];
+#pragma unroll
+              for (int k = 0; k < 4; ++k)  // 128-byte swizzle: 16-byte unit u of row r lies at u ^ (r % 8)
+                *reinterpret_cast<uint4*>(&v[4 * k]) =
+                    *reinterpret_cast<const uint4*>(src + (((half * 4 + k) ^ (row & 7)) << 4));
+              tmem_st16(dst + half * 16, v);
+            }
+          }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar->x_tmem);
+      }
+    }
     for (int j = 0; ok && j < n;) {
       // the blocks of one sequence and head; its last may be ragged
       const int m = min(n - j, it.nblk - it.blk), whole = (int)(it.len / BN) - it.blk;

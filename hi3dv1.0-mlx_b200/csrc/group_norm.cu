@@ -9,8 +9,8 @@
 //   1. chunks of rows, one CTA each: per-channel sums of the chunk (forward: mean and squared
 //      deviations about it, from sums shifted by the first value, so a large mean costs no bits;
 //      backward: sum du and sum du xh);
-//   2. per sample and channel, the chunks in order (forward: pooled deviations; backward: sums,
-//      and dw, db over all samples), 32 channels a CTA;
+//   2. per sample and channel, the chunks in order (forward: pooled deviations; backward: sums, and
+//      dw, db, over several samples by one more launch), 32 channels a CTA;
 //   3. the chunks again, last first: a CTA folds the channels of each group (shared memory) and
 //      writes y or dx.  The last chunks of pass 1 are the ones still in L2.
 // Fixed orders everywhere: no atomics.  A chunk belongs to one sample; sample s begins at chunk
@@ -27,7 +27,7 @@ namespace hi3d {
 namespace gn {
 
 constexpr int kThreads = 256;
-constexpr int kInFlight = 4;  // rows whose loads a thread has in flight (two tensors: half)
+constexpr int kInFlight = 6;  // rows whose loads a thread has in flight (two tensors: half)
 
 struct Shape {
   int rows;                // all samples' rows
@@ -82,20 +82,22 @@ __device__ __forceinline__ float fold_sum(const Shape& s, float v) {
   return v;
 }
 
-// V consecutive channels: 16 bytes of any type, or one value; unpacked to fp32 when used, so that
-// rows in flight hold 4 registers each.
+// V consecutive channels: 16 bytes of any type, or one value.  They are unpacked to fp32 pairs when
+// used (so that rows in flight hold 4 registers each) and computed on with two-lane instructions: in
+// 16 bits these kernels are bound by issue and the MUFU unit as much as by memory.  One value is a
+// pair of itself.
+template <int V>
+constexpr int kPairs = V == 1 ? 1 : V / 2;
+
 template <typename T, int V>
 struct Raw {
   uint4 u;
   __device__ __forceinline__ void load(const T* p) { u = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void get(float (&v)[V]) const {
+  __device__ __forceinline__ void get(uint64_t (&v)[kPairs<V>]) const {
     if constexpr (sizeof(T) == 4) {
-      v[0] = __uint_as_float(u.x), v[1] = __uint_as_float(u.y), v[2] = __uint_as_float(u.z), v[3] = __uint_as_float(u.w);
+      v[0] = f2_pack(__uint_as_float(u.x), __uint_as_float(u.y)), v[1] = f2_pack(__uint_as_float(u.z), __uint_as_float(u.w));
     } else {
-      f2_unpack(Cvt<T>::to_f2(u.x), v[0], v[1]);
-      f2_unpack(Cvt<T>::to_f2(u.y), v[2], v[3]);
-      f2_unpack(Cvt<T>::to_f2(u.z), v[4], v[5]);
-      f2_unpack(Cvt<T>::to_f2(u.w), v[6], v[7]);
+      v[0] = Cvt<T>::to_f2(u.x), v[1] = Cvt<T>::to_f2(u.y), v[2] = Cvt<T>::to_f2(u.z), v[3] = Cvt<T>::to_f2(u.w);
     }
   }
 };
@@ -103,20 +105,46 @@ template <typename T>
 struct Raw<T, 1> {
   T u;
   __device__ __forceinline__ void load(const T* p) { u = *p; }
-  __device__ __forceinline__ void get(float (&v)[1]) const {
+  __device__ __forceinline__ void get(uint64_t (&v)[1]) const {
     if constexpr (sizeof(T) == 4)
-      v[0] = u;
+      v[0] = f2_splat(u);
     else
-      v[0] = Cvt<T>::to_f(u);
+      v[0] = f2_splat(Cvt<T>::to_f(u));
   }
 };
 
-// body(row, values of x[, values of dy]) for rows r, r + step, .. below end.  The next U rows' loads
-// are in flight while U rows are computed.
+// What channels ch .. ch + V - 1 have of a per-channel array, as pairs
+template <int V, typename F>
+__device__ __forceinline__ void channel_pairs(uint64_t (&v)[kPairs<V>], F value) {
+#pragma unroll
+  for (int i = 0; i < kPairs<V>; ++i) v[i] = V == 1 ? f2_splat(value(0)) : f2_pack(value(2 * i), value(2 * i + 1));
+}
+// The same of what a group has, one pair where the channels share a group
+template <int V, bool UNI, typename F>
+__device__ __forceinline__ void group_pairs(uint64_t (&v)[UNI ? 1 : kPairs<V>], F value) {
+  if constexpr (UNI)
+    v[0] = f2_splat(value(0));
+  else
+    channel_pairs<V>(v, value);
+}
+__device__ __forceinline__ float low(uint64_t v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return a;
+}
+__device__ __forceinline__ float lane_of(uint64_t v, int i) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return i ? b : a;
+}
+
+// body(row, values of x[, values of dy]) for rows r, r + step, .. below end; the next U rows' loads are
+// in flight while U rows are computed.  (A shared-memory ring of bulk copies measured the same:
+// 100k x 512 bf16, all six kernels, 214 us against 201.)
 template <typename T, int V, int U, typename F>
 __device__ __forceinline__ void each_row(const T* x, int64_t stride, int r, int end, int step, F body) {
   Raw<T, V> a[U];
-  float v[V];
+  uint64_t v[kPairs<V>];
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (r + u * step < end) a[u].load(x + (r + u * step) * stride);
@@ -139,7 +167,7 @@ __device__ __forceinline__ void each_row(const T* x, int64_t stride, int r, int 
 template <typename T, int V, int U, typename F>
 __device__ __forceinline__ void each_row(const T* x, const T* y, int64_t stride, int r, int end, int step, F body) {
   Raw<T, V> a[U], b[U];
-  float v[V], w[V];
+  uint64_t v[kPairs<V>], w[kPairs<V>];
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (r + u * step < end) a[u].load(x + (r + u * step) * stride), b[u].load(y + (r + u * step) * stride);
@@ -162,33 +190,45 @@ __device__ __forceinline__ void each_row(const T* x, const T* y, int64_t stride,
 }
 
 template <typename T, int V>
-__device__ __forceinline__ void store(T* p, const float (&v)[V]) {
+__device__ __forceinline__ void store(T* p, const uint64_t (&v)[kPairs<V>]) {
   if constexpr (V == 1) {
     if constexpr (sizeof(T) == 4)
-      *p = v[0];
+      *p = low(v[0]);
     else
-      *p = Cvt<T>::from_f(v[0]);
+      *p = Cvt<T>::from_f(low(v[0]));
   } else if constexpr (sizeof(T) == 4) {
-    __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
+    __stcs(reinterpret_cast<float4*>(p), make_float4(lane_of(v[0], 0), lane_of(v[0], 1), lane_of(v[1], 0), lane_of(v[1], 1)));
   } else {
-    __stcs(reinterpret_cast<uint4*>(p), make_uint4(Cvt<T>::pack2(v[0], v[1]), Cvt<T>::pack2(v[2], v[3]),
-                                                   Cvt<T>::pack2(v[4], v[5]), Cvt<T>::pack2(v[6], v[7])));
+    __stcs(reinterpret_cast<uint4*>(p), make_uint4(Cvt<T>::from_f2(v[0]), Cvt<T>::from_f2(v[1]),
+                                                   Cvt<T>::from_f2(v[2]), Cvt<T>::from_f2(v[3])));
   }
 }
 
-// sigmoid with exp and the reciprocal on the MUFU unit (relative error about 2^-21); below -80,
-// where it is under 2^-115, it is held there: the reciprocal's range ends soon after.
-__device__ __forceinline__ float sigmoid(float u) { return __fdividef(1.0f, 1.0f + __expf(-fmaxf(u, -80.0f))); }
+// sigmoid(u) = 1 / (1 + exp(-u)) of a pair: two exponentials and one reciprocal, of the product
+// (relative error about 2^-21).  Below -40, where it is under 2^-57, it is held there: the product
+// of two denominators then stays finite.
+__device__ __forceinline__ uint64_t sigmoid2(uint64_t u) {
+  float a, b;
+  f2_unpack(u, a, b);
+  f2_unpack(f2_mul(f2_pack(fmaxf(a, -40.0f), fmaxf(b, -40.0f)), f2_splat(-1.4426950408889634f)), a, b);
+  const uint64_t d = f2_add(f2_pack(ex2_approx(a), ex2_approx(b)), f2_splat(1.0f));
+  f2_unpack(d, a, b);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
+  return f2_mul(f2_pack(b, a), f2_splat(r));
+}
 
 template <bool ACT>
-__device__ __forceinline__ float act(float u) {
-  return ACT ? u * sigmoid(u) : u;
+__device__ __forceinline__ uint64_t act2(uint64_t u) {
+  return ACT ? f2_mul(u, sigmoid2(u)) : u;
 }
+// d act'(u)
 template <bool ACT>
-__device__ __forceinline__ float act_grad(float u) {
-  if (!ACT) return 1.0f;
-  const float s = sigmoid(u);
-  return s * (1.0f + u * (1.0f - s));
+__device__ __forceinline__ uint64_t act_grad2(uint64_t u, uint64_t d) {
+  if (!ACT) return d;
+  const uint64_t s = sigmoid2(u), one = f2_splat(1.0f);
+  const uint64_t g = f2_fma(u, f2_fma(s, f2_splat(-1.0f), one), one);  // 1 + u (1 - s)
+  return f2_mul(d, f2_mul(s, g));
 }
 
 // ---------------------------------------------------------------- pass 1
@@ -202,26 +242,28 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const T* __restrict__ x
   const int lanes = kThreads / s.cols, cx = threadIdx.x % s.cols, y = threadIdx.x / s.cols;
   const int ch = (blockIdx.y * s.cols + cx) * V;
   const bool on = y < lanes && ch < s.channels;
-  float k[V], a[V] = {}, b[V] = {};
-  const int r = t.r0 + y, n = y < lanes && r < t.r1 ? (t.r1 - r + lanes - 1) / lanes : 0;
-  if (on) {
-    if (n) {
-      Raw<T, V> first;
-      first.load(x + ch + (int64_t)r * s.channels);
-      first.get(k);
-    }
-    each_row<T, V, kInFlight>(x + ch, s.channels, r, t.r1, lanes, [&](int, const float (&v)[V]) {
+  uint64_t k[kPairs<V>], a[kPairs<V>] = {}, b[kPairs<V>] = {};
+  int n = 0;
+  // sums about the thread's first value
+  auto add = [&](int, const uint64_t (&v)[kPairs<V>]) {
+    if (n++ == 0) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float d = v[i] - k[i];
-        a[i] += d;
-        b[i] = fmaf(d, d, b[i]);
-      }
-    });
+      for (int i = 0; i < kPairs<V>; ++i) k[i] = v[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kPairs<V>; ++i) {
+      const uint64_t d = f2_fma(k[i], f2_splat(-1.0f), v[i]);
+      a[i] = f2_add(a[i], d);
+      b[i] = f2_fma(d, d, b[i]);
+    }
+  };
+  if (on) {
+    each_row<T, V, kInFlight>(x + ch, s.channels, t.r0 + y, t.r1, lanes, add);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float m = n ? a[i] / n : 0.f;  // mean - k
-      sh[(y * s.cols + cx) * V + i] = n ? make_float2(k[i] + m, fmaxf(0.f, fmaf(-a[i], m, b[i]))) : make_float2(0.f, 0.f);
+      const float sum = lane_of(a[i / 2], i & 1), m = n ? sum / n : 0.f;  // mean - k
+      sh[(y * s.cols + cx) * V + i] =
+          n ? make_float2(lane_of(k[i / 2], i & 1) + m, fmaxf(0.f, fmaf(-sum, m, lane_of(b[i / 2], i & 1)))) : make_float2(0.f, 0.f);
     }
   }
   if (cx == 0 && y < lanes) count[y] = n;
@@ -253,30 +295,31 @@ __global__ void __launch_bounds__(kThreads) sums_kernel(const T* __restrict__ x,
   const Chunk t = find_chunk(s, blockIdx.x);
   const int lanes = kThreads / s.cols, cx = threadIdx.x % s.cols, y = threadIdx.x / s.cols;
   const int ch = (blockIdx.y * s.cols + cx) * V;
-  if (y < lanes && ch < s.channels) {
-    constexpr int G = UNI ? 1 : V;
-    const int width = s.channels / s.groups;
-    float mu[G], rs[G], ww[V], bb[V], a[V] = {}, c[V] = {};
+  const bool on = y < lanes && ch < s.channels;
+  constexpr int P = kPairs<V>, G = UNI ? 1 : P;
+  const int width = s.channels / s.groups;
+  uint64_t mu[G], rs[G], ww[P], bb[P], a[P] = {}, c[P] = {};
+  if (on) {
+    const float *m = mean + (int64_t)t.sample * s.groups, *r = rstd + (int64_t)t.sample * s.groups;
+    group_pairs<V, UNI>(mu, [&](int i) { return -m[(ch + i) / width]; });
+    group_pairs<V, UNI>(rs, [&](int i) { return r[(ch + i) / width]; });
+    channel_pairs<V>(ww, [&](int i) { return w[ch + i]; });
+    channel_pairs<V>(bb, [&](int i) { return b[ch + i]; });
+  }
+  auto add = [&](int, const uint64_t (&v)[P], const uint64_t (&d)[P]) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      if (i < G) {
-        const int64_t g = (int64_t)t.sample * s.groups + (ch + i) / width;
-        mu[i] = mean[g], rs[i] = rstd[g];
-      }
-      ww[i] = w[ch + i], bb[i] = b[ch + i];
+    for (int i = 0; i < P; ++i) {
+      const uint64_t xh = f2_mul(f2_add(v[i], mu[i % G]), rs[i % G]);
+      const uint64_t du = act_grad2<ACT>(f2_fma(xh, ww[i], bb[i]), d[i]);
+      a[i] = f2_add(a[i], du);
+      c[i] = f2_fma(du, xh, c[i]);
     }
-    each_row<T, V, kInFlight / 2>(x + ch, dy + ch, s.channels, t.r0 + y, t.r1, lanes,
-                                  [&](int, const float (&v)[V], const float (&d)[V]) {
+  };
+  if (on) {
+    each_row<T, V, kInFlight / 2>(x + ch, dy + ch, s.channels, t.r0 + y, t.r1, lanes, add);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float xh = (v[i] - mu[i % G]) * rs[i % G];
-        const float du = d[i] * act_grad<ACT>(fmaf(xh, ww[i], bb[i]));
-        a[i] += du;
-        c[i] = fmaf(du, xh, c[i]);
-      }
-    });
-#pragma unroll
-    for (int i = 0; i < V; ++i) sh[(y * s.cols + cx) * V + i] = make_float2(a[i], c[i]);
+    for (int i = 0; i < V; ++i)
+      sh[(y * s.cols + cx) * V + i] = make_float2(lane_of(a[i / 2], i & 1), lane_of(c[i / 2], i & 1));
   }
   __syncthreads();
   for (int e = threadIdx.x; e < s.cols * V; e += kThreads) {
@@ -330,37 +373,48 @@ __global__ void __launch_bounds__(1024) pool_kernel(const float2* __restrict__ p
   }
 }
 
-// Backward: sums of each sample and channel, dw and db over the samples in order.
+// {sum of k = 0 .. n - 1 of p[k stride]} of 32 channels by 32 lanes, lane y the terms y, y + 32, ..; the
+// lanes in order.  Every thread calls it; lane 0 gets the sum.
+__device__ __forceinline__ float2 column_sum(const float2* p, int64_t stride, int n, bool on) {
+  __shared__ float2 red[32][33];
+  float2 a = make_float2(0.f, 0.f);
+  if (on) {
+#pragma unroll 8
+    for (int k = threadIdx.y; k < n; k += 32) {
+      const float2 q = p[k * stride];
+      a.x += q.x, a.y += q.y;
+    }
+  }
+  red[threadIdx.y][threadIdx.x] = a;
+  __syncthreads();
+  float2 t = make_float2(0.f, 0.f);
+  if (threadIdx.y == 0) {
+#pragma unroll
+    for (int y = 0; y < 32; ++y) t.x += red[y][threadIdx.x].x, t.y += red[y][threadIdx.x].y;
+  }
+  return t;
+}
+
+// Backward: sums of each sample and channel over the sample's chunks; dw and db of a single sample.
 __global__ void __launch_bounds__(1024) total_kernel(const float2* __restrict__ part, const Shape s,
                                                      float2* __restrict__ chan, float* __restrict__ dw,
                                                      float* __restrict__ db) {
-  __shared__ float2 red[32][33];
-  const int c = blockIdx.x * 32 + threadIdx.x;
-  float2 all = make_float2(0.f, 0.f);
-  for (int smp = 0; smp < s.samples; ++smp) {
-    const int lo = offset(s, smp), len = max(offset(s, smp + 1) - lo, 0);
-    const int64_t base = lo / s.chunk + smp;
-    const int chunks = (len + s.chunk - 1) / s.chunk;
-    float2 a = make_float2(0.f, 0.f);
-    if (c < s.channels) {
-#pragma unroll 8
-      for (int k = threadIdx.y; k < chunks; k += 32) {
-        const float2 p = part[(base + k) * s.channels + c];
-        a.x += p.x, a.y += p.y;
-      }
-    }
-    red[threadIdx.y][threadIdx.x] = a;
-    __syncthreads();
-    if (threadIdx.y == 0 && c < s.channels) {
-      float2 t = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int y = 0; y < 32; ++y) t.x += red[y][threadIdx.x].x, t.y += red[y][threadIdx.x].y;
-      chan[(int64_t)smp * s.channels + c] = t;
-      all.x += t.x, all.y += t.y;
-    }
-    __syncthreads();
+  const int c = blockIdx.x * 32 + threadIdx.x, smp = blockIdx.y;
+  const int lo = offset(s, smp), len = max(offset(s, smp + 1) - lo, 0);
+  const int64_t base = lo / s.chunk + smp;
+  const float2 t = column_sum(part + base * s.channels + c, s.channels, (len + s.chunk - 1) / s.chunk, c < s.channels);
+  if (threadIdx.y == 0 && c < s.channels) {
+    chan[(int64_t)smp * s.channels + c] = t;
+    if (s.samples == 1) db[c] = t.x, dw[c] = t.y;
   }
-  if (threadIdx.y == 0 && c < s.channels) db[c] = all.x, dw[c] = all.y;
+}
+
+// dw and db over several samples
+__global__ void __launch_bounds__(1024) join_kernel(const float2* __restrict__ chan, const Shape s,
+                                                    float* __restrict__ dw, float* __restrict__ db) {
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  const float2 t = column_sum(chan + c, s.channels, s.samples, c < s.channels);
+  if (threadIdx.y == 0 && c < s.channels) db[c] = t.x, dw[c] = t.y;
 }
 
 // ---------------------------------------------------------------- pass 3
@@ -402,20 +456,21 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(const T* __restrict__ x
   __syncthreads();
   const int lanes = kThreads / s.cols, cx = threadIdx.x % s.cols, y = threadIdx.x / s.cols;
   const int ch = (blockIdx.y * s.cols + cx) * V;
-  if (y >= lanes || ch >= s.channels) return;
-  constexpr int G = UNI ? 1 : V;
-  float mu[G], ww[V], bb[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const float2 st = sh[(ch + i) / width];
-    mu[i % G] = st.x, ww[i] = st.y * w[ch + i], bb[i] = b[ch + i];
+  const bool on = y < lanes && ch < s.channels;
+  constexpr int P = kPairs<V>, G = UNI ? 1 : P;
+  uint64_t mu[G], ww[P], bb[P];
+  if (on) {
+    group_pairs<V, UNI>(mu, [&](int i) { return -sh[(ch + i) / width].x; });
+    channel_pairs<V>(ww, [&](int i) { return sh[(ch + i) / width].y * w[ch + i]; });
+    channel_pairs<V>(bb, [&](int i) { return b[ch + i]; });
   }
-  each_row<T, V, kInFlight>(x + ch, s.channels, t.r0 + y, t.r1, lanes, [&](int r, const float (&v)[V]) {
-    float o[V];
+  auto put = [&](int r, const uint64_t (&v)[P]) {
+    uint64_t o[P];
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = act<ACT>(fmaf(v[i] - mu[i % G], ww[i], bb[i]));
+    for (int i = 0; i < P; ++i) o[i] = act2<ACT>(f2_fma(f2_add(v[i], mu[i % G]), ww[i], bb[i]));
     store<T, V>(out + (int64_t)r * s.channels + ch, o);
-  });
+  };
+  if (on) each_row<T, V, kInFlight>(x + ch, s.channels, t.r0 + y, t.r1, lanes, put);
 }
 
 // sh[g]: {mean(du w), mean(du w xh)} over the sample and group
@@ -447,29 +502,29 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const T* __restrict__ x,
   __syncthreads();
   const int lanes = kThreads / s.cols, cx = threadIdx.x % s.cols, y = threadIdx.x / s.cols;
   const int ch = (blockIdx.y * s.cols + cx) * V;
-  if (y >= lanes || ch >= s.channels) return;
-  constexpr int G = UNI ? 1 : V;
-  float mu[G], rs[G], c1[G], c2[G], ww[V], bb[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if (i < G) {
-      const int g = (ch + i) / width;
-      mu[i] = mean[(int64_t)smp * s.groups + g], rs[i] = rstd[(int64_t)smp * s.groups + g];
-      c1[i] = sh[g].x, c2[i] = sh[g].y;
-    }
-    ww[i] = w[ch + i], bb[i] = b[ch + i];
+  const bool on = y < lanes && ch < s.channels;
+  constexpr int P = kPairs<V>, G = UNI ? 1 : P;
+  uint64_t mu[G], rs[G], c1[G], c2[G], ww[P], bb[P];
+  if (on) {
+    const float *m = mean + (int64_t)smp * s.groups, *r = rstd + (int64_t)smp * s.groups;
+    group_pairs<V, UNI>(mu, [&](int i) { return -m[(ch + i) / width]; });
+    group_pairs<V, UNI>(rs, [&](int i) { return r[(ch + i) / width]; });
+    group_pairs<V, UNI>(c1, [&](int i) { return -sh[(ch + i) / width].x; });
+    group_pairs<V, UNI>(c2, [&](int i) { return -sh[(ch + i) / width].y; });
+    channel_pairs<V>(ww, [&](int i) { return w[ch + i]; });
+    channel_pairs<V>(bb, [&](int i) { return b[ch + i]; });
   }
-  each_row<T, V, kInFlight / 2>(x + ch, dy + ch, s.channels, t.r0 + y, t.r1, lanes,
-                                [&](int r, const float (&v)[V], const float (&d)[V]) {
-    float o[V];
+  auto put = [&](int r, const uint64_t (&v)[P], const uint64_t (&d)[P]) {
+    uint64_t o[P];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float xh = (v[i] - mu[i % G]) * rs[i % G];
-      const float du = d[i] * act_grad<ACT>(fmaf(xh, ww[i], bb[i]));
-      o[i] = rs[i % G] * (fmaf(du, ww[i], -c1[i % G]) - xh * c2[i % G]);
+    for (int i = 0; i < P; ++i) {
+      const uint64_t xh = f2_mul(f2_add(v[i], mu[i % G]), rs[i % G]);
+      const uint64_t du = act_grad2<ACT>(f2_fma(xh, ww[i], bb[i]), d[i]);
+      o[i] = f2_mul(rs[i % G], f2_fma(xh, c2[i % G], f2_fma(du, ww[i], c1[i % G])));
     }
     store<T, V>(dx + (int64_t)r * s.channels + ch, o);
-  });
+  };
+  if (on) each_row<T, V, kInFlight / 2>(x + ch, dy + ch, s.channels, t.r0 + y, t.r1, lanes, put);
 }
 
 // ---------------------------------------------------------------------------
@@ -477,8 +532,8 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const T* __restrict__ x,
 // ---------------------------------------------------------------------------
 constexpr int kMaxGroups = 4096;  // a CTA holds a pair per group in shared memory
 
-// Chunks per SM: enough CTAs to fill the machine several times over (the last wave is short),
-// few enough that the partial sums stay small beside x.
+// Chunks per SM: as many CTAs as run at once with the registers of the gradient kernels, so that no
+// second wave of a few CTAs follows, and the partial sums stay small beside x.
 constexpr int kChunksPerSm = 4;
 
 static Shape make_shape(const hi3d_group_norm_args* a, bool wide) {
@@ -488,7 +543,8 @@ static Shape make_shape(const hi3d_group_norm_args* a, bool wide) {
   const int vec = wide ? (a->dtype == HI3D_F32 ? 4 : 8) : 1;
   const int across = (s.channels + vec - 1) / vec;
   s.cols = across < kThreads ? across : kThreads;
-  const int lanes = kThreads / s.cols, ctas = kChunksPerSm * sm_count();
+  const int lanes = kThreads / s.cols, most = kChunksPerSm * sm_count();
+  const int ctas = a->samples < most / 2 ? most - a->samples : most;  // each sample may add one
   const int want = (int)((a->rows + ctas - 1) / ctas), least = kInFlight * lanes;
   s.chunk = want < least ? least : want;
   s.chunks = (int)(a->rows / s.chunk) + a->samples;
@@ -557,8 +613,13 @@ static int backward(const hi3d_group_norm_args* a, const Shape& s, float2* part,
   sums_kernel<T, V, ACT, UNI><<<grid, kThreads, (size_t)(kThreads / s.cols) * s.cols * V * 8, st>>>(
       x, dy, s, a->mean, a->rstd, a->weight, a->bias, part);
   if ((rc = check_launch("group_norm gradient sums"))) return rc;
-  total_kernel<<<(unsigned)((s.channels + 31) / 32), dim3(32, 32), 0, st>>>(part, s, chan, a->dweight, a->dbias);
+  const unsigned columns = (unsigned)((s.channels + 31) / 32);
+  total_kernel<<<dim3(columns, (unsigned)s.samples), dim3(32, 32), 0, st>>>(part, s, chan, a->dweight, a->dbias);
   if ((rc = check_launch("group_norm gradient totals"))) return rc;
+  if (s.samples > 1) {
+    join_kernel<<<columns, dim3(32, 32), 0, st>>>(chan, s, a->dweight, a->dbias);
+    if ((rc = check_launch("group_norm parameter gradients"))) return rc;
+  }
   grad_kernel<T, V, ACT, UNI><<<grid, kThreads, (size_t)s.groups * 8, st>>>(
       x, dy, s, chan, a->mean, a->rstd, a->weight, a->bias, static_cast<T*>(a->dx));
   return check_launch("group_norm gradient");
