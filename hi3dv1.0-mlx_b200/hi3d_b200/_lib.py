@@ -225,9 +225,10 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def stream(t: torch.Tensor) -> int:
-    if _raw_stream is not None and t.is_cuda:
-        return _raw_stream(t.get_device())
-    return torch.cuda.current_stream(t.device).cuda_stream
+    device = t.device
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 _HERE = contextlib.nullcontext()
