@@ -33,6 +33,16 @@ int check_launch(const char* what) {
   return HI3D_OK;
 }
 
+int allow_shared(const void* kernel, int bytes, bool (&done)[64], const char* what) {
+  int dev = -1;
+  const bool known = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64;
+  if (known && done[dev]) return HI3D_OK;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return set_error(HI3D_ERR_CUDA, "%s: smem attribute: %s", what, cudaGetErrorString(e));
+  if (known) done[dev] = true;
+  return HI3D_OK;
+}
+
 int sm_count() {
   static int counts[64] = {};
   int dev = 0;

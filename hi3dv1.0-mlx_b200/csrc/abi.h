@@ -15,6 +15,10 @@ int set_error(int code, const char* fmt, ...);
 // HI3D_OK, or HI3D_ERR_CUDA with the launch error recorded.
 int check_launch(const char* what);
 
+// Lets `kernel` use `bytes` of dynamic shared memory, once per kernel and device (`done`: the
+// caller's flags for this kernel); HI3D_OK or HI3D_ERR_CUDA.
+int allow_shared(const void* kernel, int bytes, bool (&done)[64], const char* what);
+
 // Streaming multiprocessors of the current device (cached per device).
 int sm_count();
 

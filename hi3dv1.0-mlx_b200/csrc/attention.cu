@@ -695,6 +695,8 @@ static int launch_attn(const hi3d_attn_args* a, cudaStream_t st, int k_splits = 
   const int64_t qlen_max = varlen_q ? a->max_seqlen_q : a->nq;
   p.tiles_per_seq = (int)((qlen_max + 2 * attn::kRowsPerTile - 1) / (2 * attn::kRowsPerTile));
   p.scale2 = a->scale * 1.4426950408889634f;
+  // a scale of 0 attends evenly; masked scores are -inf and have to stay it
+  if (LSE && p.scale2 < 1.2e-38f) p.scale2 = 1.2e-38f;
   p.k_splits = k_splits;
   p.slot0 = slot0;
   p.part_o = part_o;
@@ -708,8 +710,9 @@ static int launch_attn(const hi3d_attn_args* a, cudaStream_t st, int k_splits = 
   if (grid == 0) return HI3D_OK;
   if (grid > 0x7fffffff) return set_error(HI3D_ERR_INVALID_ARGUMENT, "flash_attn: too many tiles");
   auto kern = part_o ? attn::flash_fwd_kernel<T, D, true, LSE> : attn::flash_fwd_kernel<T, D, false, LSE>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-  if (e != cudaSuccess) return set_error(HI3D_ERR_CUDA, "flash_attn: smem attribute: %s", cudaGetErrorString(e));
+  static bool allowed[2][64];  // whole and partial
+  if (int bad = allow_shared(reinterpret_cast<const void*>(kern), C::SMEM, allowed[part_o ? 1 : 0], "flash_attn"))
+    return bad;
   kern<<<(unsigned)grid, attn::kThreads, C::SMEM, st>>>(mq, mk, mv, p);
   return check_launch("flash_attn_fwd");
 }
@@ -899,6 +902,8 @@ extern "C" int hi3d_flash_attn_fwd_lse(const hi3d_attn_args* a, int kv_heads, fl
                      kv_heads, a->heads);
   if (!lse) return set_error(HI3D_ERR_INVALID_ARGUMENT, "flash_attn_fwd_lse: null lse");
   if (a->nk == 0) return set_error(HI3D_ERR_INVALID_ARGUMENT, "flash_attn_fwd_lse: no keys");
+  if (!(a->scale >= 0.f) || a->scale > 3.0e38f)
+    return set_error(HI3D_ERR_INVALID_ARGUMENT, "flash_attn_fwd_lse: scale must be finite and not negative");
   if (a->nq == 0 || a->num_seqs == 0) return HI3D_OK;
   if (k_splits > 1 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
     return set_error(HI3D_ERR_CAPACITY, "flash_attn_fwd_lse: workspace %lld bytes, need %lld (16-byte aligned)",

@@ -880,6 +880,8 @@ static int check_args(const hi3d_attn_bwd_args* a) {
                              a->dk_row, a->dk_head, a->dk_batch, a->dv_row, a->dv_head, a->dv_batch};
   for (int64_t s : strides)
     if (s < 0 || s % 8) return set_error(HI3D_ERR_INVALID_ARGUMENT, "flash_attn_bwd: strides must be multiples of 8");
+  if (!(a->scale >= 0.f) || a->scale > 3.0e38f)
+    return set_error(HI3D_ERR_INVALID_ARGUMENT, "flash_attn_bwd: scale must be finite and not negative");
   if (!a->cu_seqlens_q && a->cu_seqlens_k)
     return set_error(HI3D_ERR_INVALID_ARGUMENT, "flash_attn_bwd: packed keys need packed queries");
   if (a->nq > 0x7ffffff0 || a->nk > 0x7ffffff0)
@@ -950,8 +952,8 @@ static int launch(const hi3d_attn_bwd_args* a, const Plan& n, uint8_t* ws, cudaS
   if ((rc = check_launch("flash_attn_bwd statistics"))) return rc;
 
   auto kern = bwd_kernel<T, D>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, CK::SMEM);
-  if (e != cudaSuccess) return set_error(HI3D_ERR_CUDA, "flash_attn_bwd: smem attribute: %s", cudaGetErrorString(e));
+  static bool allowed[64];
+  if ((rc = allow_shared(reinterpret_cast<const void*>(kern), CK::SMEM, allowed, "flash_attn_bwd"))) return rc;
   kern<<<(unsigned)(n.kv_ctas + n.q_ctas), CK::THREADS, CK::SMEM, st>>>(mq, md, mk, mv, mqs, mds, mks, mvs, p);
   if ((rc = check_launch("flash_attn_bwd"))) return rc;
 

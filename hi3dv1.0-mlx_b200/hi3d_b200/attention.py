@@ -20,6 +20,7 @@ import ctypes
 import functools
 import itertools
 import math
+from typing import NamedTuple
 
 import torch
 
@@ -318,50 +319,98 @@ def flash_attn_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
 # ---------------------------------------------------------------------------
 # training: the forward pass with its log-sum-exp, and the gradients
 # ---------------------------------------------------------------------------
-def _aligned(t: torch.Tensor) -> bool:
-    """Whether the kernels' 16-byte loads and TMA boxes can address ``t`` as it lies."""
-    if t.data_ptr() & 15 or t.stride(-1) != 1:
-        return False
-    return t.is_contiguous() or all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+# A call's checks and strides depend on shapes, strides, types and devices alone, so they are worked
+# out once for each combination (a plan) and kept; addresses are looked at on every call.
+def _lies(shape, stride) -> bool:
+    """Whether the kernels' 16-byte loads and TMA boxes can address these strides."""
+    return stride[-1] == 1 and all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(shape[:-1], stride[:-1]))
 
 
 def _fit(t: torch.Tensor) -> torch.Tensor:
     """``t`` itself, or a contiguous copy where its strides or address do not fit the kernels
     (an expanded gradient, an odd slice)."""
-    if _aligned(t):
+    if t.data_ptr() % 16 == 0 and _lies(t.shape, t.stride()):
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _steps(t: torch.Tensor, row: int, head: int, batch: int | None = None) -> tuple[int, int, int]:
+def _steps(shape, stride, row: int, head: int, batch: int | None = None) -> tuple[int, int, int]:
     """Element strides of these axes.  An axis of one element may have any stride, which the kernels
     would refuse: a row or head then steps by one head, a batch by 0 (one set for every sequence)."""
-    n, s = t.shape, t.stride()
-    return (s[row] if n[row] != 1 else n[-1], s[head] if n[head] != 1 else n[-1],
-            0 if batch is None or n[batch] == 1 else s[batch])
+    return (stride[row] if shape[row] != 1 else shape[-1], stride[head] if shape[head] != 1 else shape[-1],
+            0 if batch is None or shape[batch] == 1 else stride[batch])
 
 
-def _check_train(q, k, v, heads: int, kv_heads: int, dim: int, same_kv: bool) -> None:
+def _contiguous(shape) -> tuple[int, ...]:
+    return tuple(itertools.accumulate(reversed(shape[1:]), lambda a, b: a * max(b, 1), initial=1))[::-1]
+
+
+class _Plan(NamedTuple):
+    batch: int      # dense: sequences; packed: 1
+    heads: int
+    nq: int         # rows of a sequence, packed: of all
+    nk: int
+    kv_heads: int
+    dim: int
+    dtype: int
+    q_axes: tuple   # (row, head[, batch]) of q and dq
+    k_axes: tuple
+    steps: tuple    # nine strides of q, k, v
+    fits: bool
+    out_shape: tuple
+    lse_shape: tuple
+    out_steps: tuple
+
+
+@functools.lru_cache(maxsize=512)
+def _plan(layout: str, qs, qt, ks, kt, vs, vt, types: tuple, devices: tuple) -> _Plan:
+    """Checks and strides of queries, keys and values; layout ``bhnd``, ``bnhd`` or ``packed``."""
+    if min(devices) < 0:
+        raise ValueError("hi3d_b200 operators take CUDA tensors")
+    if layout not in ("bhnd", "bnhd", "packed"):
+        raise ValueError(f"unknown q layout {layout!r}")
+    rank = 3 if layout == "packed" else 4
+    if len(qs) != rank or len(ks) != rank:
+        raise ValueError(f"unsupported shapes q {tuple(qs)} k {tuple(ks)} v {tuple(vs)}")
+    q_axes = {"bhnd": (2, 1, 0), "bnhd": (1, 2, 0), "packed": (0, 1)}[layout]
+    k_axes = (0, 1) if layout == "packed" else (2, 1, 0)
+    nq, heads, batch = qs[q_axes[0]], qs[q_axes[1]], 1 if rank == 3 else qs[0]
+    nk, kv_heads, dim = ks[k_axes[0]], ks[k_axes[1]], qs[-1]
     if dim not in SUPPORTED_HEAD_DIMS:
         raise NotImplementedError(f"head_dim {dim} not supported {SUPPORTED_HEAD_DIMS}")
-    if not same_kv or kv_heads < 1 or heads < 1 or heads % kv_heads:
-        raise ValueError(f"unsupported shapes q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)}")
-    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+    if (ks != vs or ks[-1] != dim or (rank == 4 and ks[0] not in (1, batch)) or kv_heads < 1 or heads < 1
+            or heads % kv_heads):
+        raise ValueError(f"unsupported shapes q {tuple(qs)} k {tuple(ks)} v {tuple(vs)}")
+    if types[0] not in (torch.float16, torch.bfloat16) or len(set(types)) != 1:
         raise ValueError("flash attention takes float16 or bfloat16 inputs of one dtype")
-    if k.device != q.device or v.device != q.device:
+    if len(set(devices)) != 1:
         raise ValueError("q, k and v must be on one device")
+    return _Plan(batch, heads, nq, nk, kv_heads, dim, _lib.F16 if types[0] == torch.float16 else _lib.BF16, q_axes,
+                 k_axes, (*_steps(qs, qt, *q_axes), *_steps(ks, kt, *k_axes), *_steps(vs, vt, *k_axes)),
+                 _lies(qs, qt) and _lies(ks, kt) and _lies(vs, vt),
+                 (nq, heads, dim) if rank == 3 else (batch, nq, heads * dim),
+                 (heads, nq) if rank == 3 else (batch, heads, nq),
+                 (heads * dim, dim, 0 if rank == 3 else nq * heads * dim))
 
 
-def _dense_shape(q, k, v, q_layout: str) -> tuple[int, int, int, int]:
-    if q_layout not in ("bhnd", "bnhd"):
-        raise ValueError(f"unknown q layout {q_layout!r}")
-    if q.dim() != 4 or k.dim() != 4:
-        raise ValueError(f"unsupported shapes q {tuple(q.shape)} k {tuple(k.shape)}")
-    batch, heads, nq, dim = q.shape if q_layout == "bhnd" else (q.shape[0], q.shape[2], q.shape[1], q.shape[3])
-    _check_train(q, k, v, heads, k.shape[1], dim,
-                 k.shape == v.shape and k.shape[3] == dim and k.shape[0] in (1, batch))
-    return batch, heads, nq, dim
+def _planned(layout: str, q, k, v):
+    """The plan of these tensors, and they or copies that fit the kernels."""
+    for _ in range(2):
+        p = _plan(layout, q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), (q.dtype, k.dtype, v.dtype),
+                  (q.get_device(), k.get_device(), v.get_device()))
+        if p.nq == 0 or p.nk == 0 or p.batch == 0 or (
+                p.fits and not (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15):
+            break
+        q, k, v = _fit(q), _fit(k), _fit(v)
+    return p, q, k, v
+
+
+def _scale(scale) -> float:
+    scale = float(scale)
+    if not 0.0 <= scale < math.inf:
+        raise ValueError(f"scale must be finite and not negative, got {scale}")
+    return scale
 
 
 def _cu(cu: torch.Tensor | None, like: torch.Tensor, name: str) -> torch.Tensor | None:
@@ -369,23 +418,43 @@ def _cu(cu: torch.Tensor | None, like: torch.Tensor, name: str) -> torch.Tensor 
         return None
     if cu.dim() != 1 or cu.numel() < 1 or cu.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be a one-dimensional int32 (or int64) tensor of num_seqs + 1 offsets")
-    if cu.device != like.device:
+    if cu.get_device() != like.get_device():
         raise ValueError(f"{name} must be on the device of q")
-    return cu.to(torch.int32).contiguous()
+    return cu if cu.dtype is torch.int32 and cu.is_contiguous() else cu.to(torch.int32).contiguous()
 
 
-def _forward_lse(args: _lib.AttnArgs, kv_heads: int, lse: torch.Tensor, k_splits) -> None:
-    splits = _resolve_splits(k_splits, args, lse)
-    lib = _lib.load()
-    ws = None
-    if splits > 1:
-        nbytes = ctypes.c_int64()
-        _lib.check(lib.hi3d_flash_attn_split_workspace_size(ctypes.byref(args), splits, ctypes.byref(nbytes)),
-                   "flash_attention split workspace", launched=False)
-        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=lse.device)
-    rc = lib.hi3d_flash_attn_fwd_lse(ctypes.byref(args), kv_heads, lse.data_ptr(), splits, _lib.ptr(ws),
-                                     0 if ws is None else ws.numel(), _lib.stream(lse))
-    _lib.check(rc, "flash_attention_lse")
+def _offsets(cu_seqlens_q, cu_seqlens_k, q):
+    cu_q, cu_k = _cu(cu_seqlens_q, q, "cu_seqlens_q"), _cu(cu_seqlens_k, q, "cu_seqlens_k")
+    if cu_k is not None and cu_k.numel() != cu_q.numel():
+        raise ValueError("cu_seqlens_q and cu_seqlens_k must have the same length")
+    return cu_q, cu_k
+
+
+_cached_splits = functools.lru_cache(maxsize=512)(auto_splits)
+
+
+def _forward_lse(p: _Plan, q, k, v, cu_q, cu_k, num_seqs: int, longest: int, scale: float, k_splits):
+    with _lib.on_device(q):
+        if p.nk == 0:
+            return q.new_zeros(p.out_shape), torch.full(p.lse_shape, -math.inf, device=q.device)
+        out, lse = q.new_empty(p.out_shape), q.new_empty(p.lse_shape, dtype=torch.float32)
+        if p.nq == 0 or num_seqs == 0:
+            return out, lse
+        args = _lib.AttnArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *p.steps, *p.out_steps,
+                             _lib.ptr(cu_q), _lib.ptr(cu_k), p.nq, p.nk, longest, num_seqs, p.heads, p.dim, p.dtype,
+                             scale)
+        if k_splits == "auto":
+            k_splits = _cached_splits(math.ceil(longest / 256) * num_seqs * p.heads,
+                                      math.ceil(p.nk / (128 if p.dim == 64 else 64)), _sm_count(q.get_device()))
+        lib, ws, nbytes = _lib.load(), None, ctypes.c_int64()
+        if k_splits > 1:
+            _lib.check(lib.hi3d_flash_attn_split_workspace_size(ctypes.byref(args), k_splits, ctypes.byref(nbytes)),
+                       "flash_attention split workspace", launched=False)
+            ws = q.new_empty(nbytes.value, dtype=torch.uint8)
+        rc = lib.hi3d_flash_attn_fwd_lse(ctypes.byref(args), p.kv_heads, lse.data_ptr(), int(k_splits), _lib.ptr(ws),
+                                         nbytes.value, _lib.stream(q))
+        _lib.check(rc, "flash_attention_lse")
+    return out, lse
 
 
 def flash_attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, q_layout: str = "bhnd",
@@ -396,24 +465,10 @@ def flash_attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale
     ``k, v`` ``[B or 1, Hk, Nk, D]`` with ``Hk`` dividing ``H``: query head ``h`` reads key head
     ``h // (H // Hk)``.  Without keys (``Nk = 0``) the output is 0 and ``lse`` is ``-inf``.
     """
-    _lib.require_cuda(q, k, v)
-    batch, heads, nq, dim = _dense_shape(q, k, v, q_layout)
-    with _lib.on_device(q):
-        if k.shape[2] == 0:
-            return (torch.zeros((batch, nq, heads * dim), dtype=q.dtype, device=q.device),
-                    torch.full((batch, heads, nq), -math.inf, device=q.device))
-        out = torch.empty((batch, nq, heads * dim), dtype=q.dtype, device=q.device)
-        lse = torch.empty((batch, heads, nq), dtype=torch.float32, device=q.device)
-        if nq == 0 or batch == 0:
-            return out, lse
-        q, k, v = _fit(q), _fit(k), _fit(v)
-        args = _lib.AttnArgs(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-            *(_steps(q, 2, 1, 0) if q_layout == "bhnd" else _steps(q, 1, 2, 0)), *_steps(k, 2, 1, 0),
-            *_steps(v, 2, 1, 0), heads * dim, dim, nq * heads * dim, None, None, nq, k.shape[2], nq, batch, heads, dim,
-            _lib.dtype_code(q), float(scale))
-        _forward_lse(args, k.shape[1], lse, k_splits)
-    return out, lse
+    if q_layout == "packed":
+        raise ValueError(f"unknown q layout {q_layout!r}")
+    p, q, k, v = _planned(q_layout, q, k, v)
+    return _forward_lse(p, q, k, v, None, None, p.batch, p.nq, _scale(scale), k_splits)
 
 
 def flash_attn_varlen_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
@@ -423,86 +478,96 @@ def flash_attn_varlen_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_
 
     ``k, v`` ``[Tk, Hk, D]`` with ``Hk`` dividing ``H``.  A sequence without keys gets an output of 0
     and ``lse = -inf``.  Sequences never see each other's rows, NaN and infinities included.  The
-    offsets must cover all rows of ``q``.
+    offsets must cover all rows of ``q``, and no sequence may be longer than ``max_seqlen_q``.
     """
-    _lib.require_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k)
-    cu_q, cu_k, heads, dim = _varlen_shape(q, k, v, cu_seqlens_q, cu_seqlens_k)
-    tq, tk = q.shape[0], k.shape[0]
-    with _lib.on_device(q):
-        if tk == 0:
-            return (torch.zeros((tq, heads, dim), dtype=q.dtype, device=q.device),
-                    torch.full((heads, tq), -math.inf, device=q.device))
-        out = torch.empty((tq, heads, dim), dtype=q.dtype, device=q.device)
-        lse = torch.empty((heads, tq), dtype=torch.float32, device=q.device)
-        num_seqs = cu_q.numel() - 1
-        if tq == 0 or num_seqs == 0:
-            return out, lse
-        if int(max_seqlen_q) < 1:
-            raise ValueError("max_seqlen_q must be at least the longest query sequence")
-        q, k, v = _fit(q), _fit(k), _fit(v)
-        args = _lib.AttnArgs(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *_steps(q, 0, 1), *_steps(k, 0, 1),
-            *_steps(v, 0, 1), heads * dim, dim, 0, cu_q.data_ptr(), _lib.ptr(cu_k), tq, tk,
-            min(int(max_seqlen_q), tq), num_seqs, heads, dim, _lib.dtype_code(q), float(scale))
-        _forward_lse(args, k.shape[1], lse, k_splits)
-    return out, lse
+    p, q, k, v = _planned("packed", q, k, v)
+    cu_q, cu_k = _offsets(cu_seqlens_q, cu_seqlens_k, q)
+    num_seqs = cu_q.numel() - 1
+    if int(max_seqlen_q) < 1 and p.nq and num_seqs:
+        raise ValueError("max_seqlen_q must be at least the longest query sequence")
+    return _forward_lse(p, q, k, v, cu_q, cu_k, num_seqs, min(int(max_seqlen_q), p.nq), _scale(scale), k_splits)
 
 
-def _varlen_shape(q, k, v, cu_seqlens_q, cu_seqlens_k):
-    if q.dim() != 3 or k.dim() != 3:
-        raise ValueError(f"unsupported shapes q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)}")
-    _, heads, dim = q.shape
-    _check_train(q, k, v, heads, k.shape[1], dim, k.shape == v.shape and k.shape[2] == dim)
-    cu_q, cu_k = _cu(cu_seqlens_q, q, "cu_seqlens_q"), _cu(cu_seqlens_k, q, "cu_seqlens_k")
-    if cu_k is not None and cu_k.numel() != cu_q.numel():
-        raise ValueError("cu_seqlens_q and cu_seqlens_k must have the same length")
-    return cu_q, cu_k, heads, dim
+@functools.lru_cache(maxsize=512)
+def _saved_plan(p: _Plan, os, ot, gs, gt, ls, types: tuple, devices: tuple) -> tuple:
+    """Checks of what the backward pass is given beside q, k, v, and the strides of out and its
+    gradient, or None where a copy has to be made."""
+    for name, shape, kind, device in zip(("out", "grad_out"), (os, gs), types, devices):
+        if shape != p.out_shape or kind != types[3] or device != devices[3]:
+            raise ValueError(f"{name} must be {p.out_shape} in the dtype and on the device of q, got {tuple(shape)}")
+    if ls != p.lse_shape or types[2] != torch.float32 or devices[2] != devices[3]:
+        raise ValueError(f"lse must be the float32 {p.lse_shape} of the forward pass, got {tuple(ls)}")
+    steps = []
+    for shape, stride in ((os, ot), (gs, gt)):
+        if len(shape) == 3 and len(p.q_axes) == 3:  # [B, Nq, H * D] as [B, Nq, H, D]
+            shape, stride = (*shape[:2], p.heads, p.dim), (*stride[:2], p.dim * stride[2], stride[2])
+        axes = (0, 1) if len(shape) == 3 else (1, 2, 0)
+        steps.append(_steps(shape, stride, *axes) if _lies(shape, stride) else None)
+    return tuple(steps)
 
 
-def _grads(given, like) -> list[torch.Tensor]:
-    """The gradients' tensors: the caller's, checked, or new contiguous ones."""
-    got = []
-    for name, g, t in zip(("dq", "dk", "dv"), given or (None, None, None), like):
-        if g is None:
-            g = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        elif g.shape != t.shape or g.dtype != t.dtype or g.device != t.device or not _aligned(g):
-            raise ValueError(f"{name} must have the shape, dtype and device of its input, rows contiguous over the "
-                             "head dimension and 16-byte aligned")
-        got.append(g)
-    return got
-
-
-@functools.lru_cache(maxsize=256)
-def _backward_workspace(packed_q: bool, packed_k: bool, shared: bool, sizes: tuple, device: int) -> int:
-    """Bytes of workspace for these sizes (asked once per sizes and device): only the presence of
-    pointers and the key batch stride count beside them."""
-    args = _lib.AttnBwdArgs(*[16] * 9, *[8] * 24, 16 if packed_q else None, 16 if packed_k else None, *sizes)
-    args.k_batch = 0 if shared else 8
+@functools.lru_cache(maxsize=512)
+def _backward_plan(p: _Plan, qs, ks, steps: tuple, packed_k: bool, num_seqs: int, scale: float, device: int) -> tuple:
+    """(the argument structure's strides with contiguous gradients, its sizes, bytes of workspace)."""
+    dq, dk = _steps(qs, _contiguous(qs), *p.q_axes), _steps(ks, _contiguous(ks), *p.k_axes)
+    sizes = (p.nq, p.nk, num_seqs, p.heads, p.kv_heads, p.dim, p.dtype, scale)
+    packed = len(p.q_axes) == 2
+    # only the presence of pointers counts for the workspace
+    args = _lib.AttnBwdArgs(*[16] * 9, *p.steps, *steps, *dq, *dk, *dk, 16 if packed else None,
+                            16 if packed_k else None, *sizes)
     nbytes = ctypes.c_int64()
     _lib.check(_lib.load().hi3d_flash_attn_bwd_workspace_size(ctypes.byref(args), ctypes.byref(nbytes)),
                "flash_attention_backward workspace", launched=False)
-    return nbytes.value
+    return (*p.steps, *steps, *dq, *dk, *dk), sizes, nbytes.value
 
 
-def _backward(tensors, lse, strides, cu_q, cu_k, sizes) -> None:
-    """``tensors``: q, k, v, out, grad_out, dq, dk, dv with their ``strides``; ``sizes``: nq, nk, num_seqs,
-    heads, kv_heads, head_dim, dtype, scale."""
-    q, k, v, out, grad_out, dq, dk, dv = tensors
-    args = _lib.AttnBwdArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), grad_out.data_ptr(),
-                            lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                            *itertools.chain.from_iterable(strides), _lib.ptr(cu_q), _lib.ptr(cu_k), *sizes)
-    nbytes = _backward_workspace(cu_q is not None, cu_k is not None, args.k_batch == 0, sizes, q.get_device())
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    rc = _lib.load().hi3d_flash_attn_bwd(ctypes.byref(args), ws.data_ptr(), nbytes, _lib.stream(q))
-    _lib.check(rc, "flash_attention_backward")
+def _given(grads, like, p: _Plan) -> tuple[list, tuple]:
+    """The caller's gradient tensors, checked, with new ones for None, and their strides."""
+    got, steps = [], []
+    for name, g, t, axes in zip(("dq", "dk", "dv"), grads, like, (p.q_axes, p.k_axes, p.k_axes)):
+        if g is None:
+            g = t.new_empty(t.shape)
+        elif (g.shape != t.shape or g.dtype != t.dtype or g.device != t.device or g.data_ptr() % 16
+              or not _lies(g.shape, g.stride())):
+            raise ValueError(f"{name} must have the shape, dtype and device of its input, rows contiguous over the "
+                             "head dimension and 16-byte aligned")
+        got.append(g)
+        steps += _steps(g.shape, g.stride(), *axes)
+    return got, tuple(steps)
 
 
-def _check_saved(grad_out, out, lse, q, out_shape, lse_shape) -> None:
-    for name, t in (("grad_out", grad_out), ("out", out)):
-        if tuple(t.shape) != out_shape or t.dtype != q.dtype or t.device != q.device:
-            raise ValueError(f"{name} must be {out_shape} in the dtype and on the device of q, got {tuple(t.shape)}")
-    if tuple(lse.shape) != lse_shape or lse.dtype != torch.float32 or lse.device != q.device:
-        raise ValueError(f"lse must be the float32 {lse_shape} of the forward pass, got {tuple(lse.shape)}")
+def _backward(p: _Plan, grad_out, q, k, v, out, lse, cu_q, cu_k, num_seqs: int, scale: float, grads):
+    for _ in range(2):
+        steps = _saved_plan(p, out.shape, out.stride(), grad_out.shape, grad_out.stride(), lse.shape,
+                            (out.dtype, grad_out.dtype, lse.dtype, q.dtype),
+                            (out.get_device(), grad_out.get_device(), lse.get_device(), q.get_device()))
+        if None not in steps and not (out.data_ptr() | grad_out.data_ptr()) & 15:
+            break
+        if p.nq == 0 or p.nk == 0 or p.batch == 0 or num_seqs == 0:
+            break
+        out, grad_out = _fit(out), _fit(grad_out)
+    with _lib.on_device(q):
+        if grads is None:
+            dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+            given = None
+        else:
+            (dq, dk, dv), given = _given(grads, (q, k, v), p)
+        if p.nq == 0 or p.nk == 0 or p.batch == 0 or num_seqs == 0:
+            for t in (dq, dk, dv):
+                t.zero_()
+            return dq, dk, dv
+        strides, sizes, nbytes = _backward_plan(p, q.shape, k.shape, steps[0] + steps[1], cu_k is not None, num_seqs,
+                                                scale, q.get_device())
+        if given is not None:
+            strides = strides[:15] + given
+        lse = lse.contiguous()
+        args = _lib.AttnBwdArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), grad_out.data_ptr(),
+                                lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *strides, _lib.ptr(cu_q),
+                                _lib.ptr(cu_k), *sizes)
+        ws = q.new_empty(nbytes, dtype=torch.uint8)
+        rc = _lib.load().hi3d_flash_attn_bwd(ctypes.byref(args), ws.data_ptr(), nbytes, _lib.stream(q))
+        _lib.check(rc, "flash_attention_backward")
+    return dq, dk, dv
 
 
 def flash_attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -516,25 +581,10 @@ def flash_attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.T
     once.  ``grads``: optional ``(dq, dk, dv)`` tensors to write, e.g. views of one fused gradient
     (None entries are allocated).
     """
-    _lib.require_cuda(grad_out, q, k, v, out, lse)
-    batch, heads, nq, dim = _dense_shape(q, k, v, q_layout)
-    _check_saved(grad_out, out, lse, q, (batch, nq, heads * dim), (batch, heads, nq))
-    with _lib.on_device(q):
-        dq, dk, dv = grads = _grads(grads, (q, k, v))
-        if nq == 0 or batch == 0 or k.shape[2] == 0:
-            for t in grads:
-                t.zero_()
-            return dq, dk, dv
-        q, k, v, lse = _fit(q), _fit(k), _fit(v), lse.contiguous()
-        out = _fit(out.view(batch, nq, heads, dim) if out.is_contiguous() else out.unflatten(2, (heads, dim)))
-        grad_out = _fit(grad_out.view(batch, nq, heads, dim) if grad_out.is_contiguous()
-                        else grad_out.unflatten(2, (heads, dim)))
-        axes = (2, 1, 0) if q_layout == "bhnd" else (1, 2, 0)
-        _backward((q, k, v, out, grad_out, dq, dk, dv), lse,
-                  (_steps(q, *axes), _steps(k, 2, 1, 0), _steps(v, 2, 1, 0), _steps(out, 1, 2, 0),
-                   _steps(grad_out, 1, 2, 0), _steps(dq, *axes), _steps(dk, 2, 1, 0), _steps(dv, 2, 1, 0)),
-                  None, None, (nq, k.shape[2], batch, heads, k.shape[1], dim, _lib.dtype_code(q), float(scale)))
-    return dq, dk, dv
+    if q_layout == "packed":
+        raise ValueError(f"unknown q layout {q_layout!r}")
+    p, q, k, v = _planned(q_layout, q, k, v)
+    return _backward(p, grad_out, q, k, v, out, lse, None, None, p.batch, _scale(scale), grads)
 
 
 def flash_attn_varlen_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -544,17 +594,6 @@ def flash_attn_varlen_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch
     """``(dq, dk, dv)`` of :func:`flash_attn_varlen_lse` in the shapes of ``q, k, v``, as
     :func:`flash_attention_backward`; with ``cu_seqlens_k=None`` ``dk, dv`` sum over all sequences.
     No longest length is needed.  The offsets must cover all rows."""
-    _lib.require_cuda(grad_out, q, k, v, out, lse, cu_seqlens_q, cu_seqlens_k)
-    cu_q, cu_k, heads, dim = _varlen_shape(q, k, v, cu_seqlens_q, cu_seqlens_k)
-    tq = q.shape[0]
-    _check_saved(grad_out, out, lse, q, (tq, heads, dim), (heads, tq))
-    with _lib.on_device(q):
-        dq, dk, dv = grads = _grads(grads, (q, k, v))
-        if tq == 0 or k.shape[0] == 0 or cu_q.numel() < 2:
-            for t in grads:
-                t.zero_()
-            return dq, dk, dv
-        tensors = (_fit(q), _fit(k), _fit(v), _fit(out), _fit(grad_out), dq, dk, dv)
-        _backward(tensors, lse.contiguous(), [_steps(t, 0, 1) for t in tensors], cu_q, cu_k,
-                  (tq, k.shape[0], cu_q.numel() - 1, heads, k.shape[1], dim, _lib.dtype_code(q), float(scale)))
-    return dq, dk, dv
+    p, q, k, v = _planned("packed", q, k, v)
+    cu_q, cu_k = _offsets(cu_seqlens_q, cu_seqlens_k, q)
+    return _backward(p, grad_out, q, k, v, out, lse, cu_q, cu_k, cu_q.numel() - 1, _scale(scale), grads)

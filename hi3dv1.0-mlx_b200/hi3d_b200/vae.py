@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 
 import numpy as np
 import torch
@@ -77,56 +78,48 @@ def conv_gn_swish(x: torch.Tensor, level: sparse.Level, norm_weight: torch.Tenso
                        tap_mask=level.tap_mask)
 
 
-def _norm_args(x, weight, bias, groups: int, act, eps: float, offsets, mean, rstd):
-    if x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+@functools.lru_cache(maxsize=512)
+def _norm_plan(shape, dtype, weight_shape, bias_shape, groups: int, act, eps: float, packed: int | None, devices: tuple):
+    """What follows from shapes, types and devices alone, worked out once for each combination: the
+    number of samples, the argument structure's sizes, bytes of workspace.  ``packed``: offsets given."""
+    if min(devices) < 0:
+        raise ValueError("hi3d_b200 operators take CUDA tensors")
+    if dtype not in (torch.float16, torch.bfloat16, torch.float32):
         raise ValueError("group_norm_act takes float16, bfloat16 or float32 features")
-    if x.dim() < 2:
-        raise ValueError(f"x must be [rows, C] or [samples, ..., C], got {tuple(x.shape)}")
-    c = x.shape[-1]
+    if len(shape) < 2:
+        raise ValueError(f"x must be [rows, C] or [samples, ..., C], got {tuple(shape)}")
     if act not in (None, "swish"):
         raise ValueError(f"unknown activation {act!r}")
+    if packed is not None and (len(shape) != 2 or packed < 2):
+        raise ValueError("offsets are samples + 1 row offsets of packed rows [rows, C]")
+    c = shape[-1]
     if groups < 1 or c < 1 or c % groups:
         raise ValueError(f"{c} channels do not divide into {groups} groups")
-    if weight.shape != (c,) or bias.shape != (c,):
+    if weight_shape != (c,) or bias_shape != (c,):
         raise ValueError(f"weight and bias must be [{c}]")
-    rows = x.numel() // c
-    samples = 1 if x.dim() == 2 else x.shape[0]
-    if offsets is not None:
-        if x.dim() != 2:
-            raise ValueError("offsets are for packed rows [rows, C]")
-        if offsets.dim() != 1 or offsets.numel() < 2 or offsets.dtype not in (torch.int32, torch.int64):
-            raise ValueError("offsets must be a one-dimensional int32 (or int64) tensor of samples + 1 row offsets")
-        offsets = offsets.to(torch.int32).contiguous()
-        samples = offsets.numel() - 1
-    for t in (weight, bias, offsets, mean, rstd):
-        if t is not None and t.get_device() != x.get_device():
-            raise ValueError("all tensors must be on the device of x")
-    return samples, offsets, _lib.GroupNormArgs(
-        x=x.data_ptr(), weight=weight.data_ptr(), bias=bias.data_ptr(), offsets=_lib.ptr(offsets), rows=rows,
-        channels=c, samples=samples, groups=groups, act=int(act is not None), dtype=_lib.dtype_code(x), eps=float(eps))
-
-
-@functools.lru_cache(maxsize=256)
-def _norm_workspace(rows: int, channels: int, samples: int, groups: int, act: int, dtype: int, device: int) -> int:
-    """Bytes of workspace for these sizes (asked once per sizes and device)."""
-    args = _lib.GroupNormArgs(rows=rows, channels=channels, samples=samples, groups=groups, act=act, dtype=dtype, eps=1.0)
-    if rows % samples:
-        args.offsets = 1  # packed samples: only the pointer's presence counts here
+    if len(set(devices)) != 1:
+        raise ValueError("all tensors must be on the device of x")
+    samples = packed - 1 if packed else 1 if len(shape) == 2 else shape[0]
+    code = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}[dtype]
+    sizes = (math.prod(shape[:-1]), c, samples, groups, int(act is not None), code, eps)
     nb = ctypes.c_int64()
-    _lib.check(_lib.load().hi3d_group_norm_act_workspace_size(ctypes.byref(args), ctypes.byref(nb)), "group_norm_act",
-               launched=False)
-    return nb.value
-
-
-def _norm_call(name: str, args, x) -> None:
-    size = _norm_workspace(args.rows, args.channels, args.samples, args.groups, args.act, args.dtype, x.get_device())
-    ws = torch.empty(size, dtype=torch.uint8, device=x.device)
-    rc = getattr(_lib.load(), name)(ctypes.byref(args), ws.data_ptr(), size, _lib.stream(x))
-    _lib.check(rc, name)
+    if samples:
+        args = _lib.GroupNormArgs(*[16] * 3, 16 if packed else None, *[16] * 7, *sizes)
+        _lib.check(_lib.load().hi3d_group_norm_act_workspace_size(ctypes.byref(args), ctypes.byref(nb)),
+                   "group_norm_act", launched=False)
+    return samples, sizes, nb.value
 
 
 def _fp32(t: torch.Tensor) -> torch.Tensor:
     return t if t.dtype is torch.float32 and t.is_contiguous() else t.detach().float().contiguous()
+
+
+def _int32(offsets: torch.Tensor | None) -> torch.Tensor | None:
+    if offsets is None or (offsets.dtype is torch.int32 and offsets.is_contiguous() and offsets.dim() == 1):
+        return offsets
+    if offsets.dim() != 1 or offsets.dtype != torch.int32 and offsets.dtype != torch.int64:
+        raise ValueError("offsets must be a one-dimensional int32 (or int64) tensor of samples + 1 row offsets")
+    return offsets.to(torch.int32).contiguous()
 
 
 def group_norm_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, groups: int, eps: float = 1e-6,
@@ -138,16 +131,19 @@ def group_norm_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, gr
     ``x`` is one sample ``[rows, C]``, packed samples ``[rows, C]`` with row ``offsets [samples + 1]``
     (some may be empty; they must cover all rows), or ``[samples, ..., C]``.  ``weight, bias`` ``[C]``.
     """
-    _lib.require_cuda(x, weight, bias, offsets)
+    offsets = _int32(offsets)
+    samples, sizes, nbytes = _norm_plan(
+        x.shape, x.dtype, weight.shape, bias.shape, groups, act, float(eps), None if offsets is None else offsets.numel(),
+        (x.get_device(), weight.get_device(), bias.get_device(), (x if offsets is None else offsets).get_device()))
     x, weight, bias = x.contiguous(), _fp32(weight), _fp32(bias)
     with _lib.on_device(x):
-        samples, offsets, args = _norm_args(x, weight, bias, groups, act, eps, offsets, None, None)
-        y = torch.empty_like(x)
-        mean = torch.empty((samples, groups), dtype=torch.float32, device=x.device)
-        rstd = torch.empty((samples, groups), dtype=torch.float32, device=x.device)
+        y, mean, rstd = torch.empty_like(x), weight.new_empty((samples, groups)), weight.new_empty((samples, groups))
         if samples:
-            args.y, args.mean, args.rstd = y.data_ptr(), mean.data_ptr(), rstd.data_ptr()
-            _norm_call("hi3d_group_norm_act_fwd", args, x)
+            ws = x.new_empty(nbytes, dtype=torch.uint8)
+            args = _lib.GroupNormArgs(x.data_ptr(), weight.data_ptr(), bias.data_ptr(), _lib.ptr(offsets),
+                                      mean.data_ptr(), rstd.data_ptr(), y.data_ptr(), None, None, None, None, *sizes)
+            rc = _lib.load().hi3d_group_norm_act_fwd(ctypes.byref(args), ws.data_ptr(), nbytes, _lib.stream(x))
+            _lib.check(rc, "group_norm_act")
     return y, mean, rstd
 
 
@@ -156,24 +152,29 @@ def group_norm_act_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tenso
                             offsets: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``(dx, dweight, dbias)`` of :func:`group_norm_act`: ``dx`` in the type of ``x``, the others fp32
     ``[C]``, summed over all samples in a fixed order."""
-    _lib.require_cuda(dy, x, mean, rstd, weight, bias, offsets)
-    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
-        raise ValueError(f"dy must be like x {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
+    offsets = _int32(offsets)
     if mean.dim() != 2 or mean.shape != rstd.shape or mean.dtype != torch.float32 or rstd.dtype != torch.float32:
         raise ValueError("mean and rstd must be the float32 [samples, groups] of the forward pass")
+    # eps went into rstd: any positive number passes the checks
+    samples, sizes, nbytes = _norm_plan(
+        x.shape, x.dtype, weight.shape, bias.shape, mean.shape[1], act, 1.0, None if offsets is None else offsets.numel(),
+        (x.get_device(), weight.get_device(), bias.get_device(), (x if offsets is None else offsets).get_device(),
+         dy.get_device(), mean.get_device(), rstd.get_device()))
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError(f"dy must be like x {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
+    if mean.shape[0] != samples:
+        raise ValueError(f"mean and rstd are of {mean.shape[0]} samples, x and offsets of {samples}")
     x, dy, mean, rstd = x.contiguous(), dy.contiguous(), mean.contiguous(), rstd.contiguous()
     weight, bias = _fp32(weight), _fp32(bias)
     with _lib.on_device(x):
-        samples, offsets, args = _norm_args(x, weight, bias, mean.shape[1], act, 1.0, offsets, mean, rstd)
-        if mean.shape[0] != samples:
-            raise ValueError(f"mean and rstd are of {mean.shape[0]} samples, x and offsets of {samples}")
-        dx = torch.empty_like(x)
-        dweight = torch.empty(x.shape[-1], dtype=torch.float32, device=x.device)
-        dbias = torch.empty(x.shape[-1], dtype=torch.float32, device=x.device)
+        dx, dweight, dbias = torch.empty_like(x), weight.new_empty(x.shape[-1]), weight.new_empty(x.shape[-1])
         if samples:
-            args.mean, args.rstd, args.dy, args.dx = mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), dx.data_ptr()
-            args.dweight, args.dbias = dweight.data_ptr(), dbias.data_ptr()
-            _norm_call("hi3d_group_norm_act_bwd", args, x)
+            ws = x.new_empty(nbytes, dtype=torch.uint8)
+            args = _lib.GroupNormArgs(x.data_ptr(), weight.data_ptr(), bias.data_ptr(), _lib.ptr(offsets),
+                                      mean.data_ptr(), rstd.data_ptr(), None, dy.data_ptr(), dx.data_ptr(),
+                                      dweight.data_ptr(), dbias.data_ptr(), *sizes)
+            rc = _lib.load().hi3d_group_norm_act_bwd(ctypes.byref(args), ws.data_ptr(), nbytes, _lib.stream(x))
+            _lib.check(rc, "group_norm_act_backward")
         else:
             dweight.zero_()
             dbias.zero_()

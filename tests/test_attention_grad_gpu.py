@@ -306,6 +306,30 @@ def test_no_keys_no_queries_no_batch():
     assert out.shape == q.shape and lse.shape == (2, 0)
 
 
+def test_a_scale_of_zero_attends_evenly():
+    q, k, v, do = (_rand((1, 2, 40 + 9 * i, 64), torch.bfloat16, 60 + i) for i in range(4))
+    v, do = v[:, :, :49], do[:, :, :40]
+    out, lse, dq, dk, dv = dense(q, k, v, do, 0.0)
+    assert torch.allclose(lse, torch.tensor(math.log(49.0), device=DEV), rtol=1e-6)
+    assert not dq.any() and not dk.any()
+    check("dv", dv, (do.double().sum(2, keepdim=True) / 49).expand_as(dv), torch.bfloat16)
+
+
+def test_saved_tensors_in_other_layouts():
+    """out and its gradient as views of wider rows, lse with strides of its own: the same bits."""
+    q, k, v, do = (_rand((2, 3, 50, 64), torch.float16, 70 + i) for i in range(4))
+    want = dense(q, k, v, do, 0.125)
+    out, lse = attention.flash_attention_lse(q, k, v, 0.125)
+    wide = torch.zeros((2, 50, 400), dtype=torch.float16, device=DEV)
+    wide[..., 8:200], wide[..., 200:392] = out, do.transpose(1, 2).flatten(2)
+    apart = torch.empty((50, 2, 3), device=DEV).permute(1, 2, 0).copy_(lse)
+    got = attention.flash_attention_backward(wide[..., 200:392], q, k, v, wide[..., 8:200], apart, 0.125)
+    assert all(torch.equal(a, b) for a, b in zip(got, want[2:]))
+    slow = torch.empty((192, 2, 50), dtype=torch.float16, device=DEV).permute(1, 2, 0).copy_(out)
+    got = attention.flash_attention_backward(wide[..., 200:392], q, k, v, slow, lse, 0.125)
+    assert all(torch.equal(a, b) for a, b in zip(got, want[2:]))
+
+
 def test_another_stream_and_odd_alignment():
     q, k, v, do = (_rand((1, 2, 200, 64), torch.float16, 45 + i) for i in range(4))
     want = dense(q, k, v, do, 0.125)
@@ -328,8 +352,13 @@ def test_refusals():
         attention.flash_attention_lse(q, k64, k64, 0.1)        # two dtypes
     with pytest.raises(ValueError):
         attention.flash_attention_lse(q.float(), q.float(), q.float(), 0.1)
+    for scale in (-0.1, math.nan, math.inf):
+        with pytest.raises(ValueError):
+            attention.flash_attention_lse(q, q, q, scale)
     with pytest.raises(ValueError):
         attention.flash_attention_lse(q, q, q, 0.1, "hbnd")
+    with pytest.raises(ValueError):
+        attention.flash_attention_lse(q, q, q, 0.1, "packed")
     with pytest.raises(NotImplementedError):
         attention.flash_attention_lse(q[..., :32], q[..., :32], q[..., :32], 0.1)
     with pytest.raises(ValueError):

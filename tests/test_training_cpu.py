@@ -22,7 +22,7 @@ def test_attention_backward_arguments():
     assert _bwd()[0] == _lib.OK and _bwd()[1] > 0
     for kw in (dict(q=None), dict(lse=None), dict(dk=None), dict(dtype=_lib.F32), dict(nq=0), dict(nk=0),
                dict(num_seqs=0), dict(kv_heads=0), dict(heads=3), dict(q=24), dict(dv_row=60), dict(k_head=-8),
-               dict(cu_seqlens_k=16), dict(nq=1 << 31)):
+               dict(cu_seqlens_k=16), dict(nq=1 << 31), dict(scale=-1.0), dict(scale=float("nan"))):
         assert _bwd(**kw)[0] == _lib.ERR_INVALID_ARGUMENT, kw
     assert _bwd(head_dim=80)[0] == _lib.ERR_UNSUPPORTED
     a = _lib.AttnBwdArgs(*[16] * 9, *[64] * 24, None, None, 5, 7, 1, 2, 2, 64, _lib.F16, 0.125)
@@ -45,7 +45,9 @@ def test_attention_forward_lse_arguments():
     assert call(4, None, 1) == _lib.ERR_INVALID_ARGUMENT
     assert call(4, 16, 65) == _lib.ERR_INVALID_ARGUMENT
     assert call(4, 16, 2) == _lib.ERR_CAPACITY
-    a.nk = 0
+    a.scale = -0.5
+    assert call(4, 16, 1) == _lib.ERR_INVALID_ARGUMENT
+    a.scale, a.nk = 0.5, 0
     assert call(4, 16, 1) == _lib.ERR_INVALID_ARGUMENT
 
 
