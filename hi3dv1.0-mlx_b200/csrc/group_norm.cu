@@ -16,8 +16,11 @@
 // Fixed orders everywhere: no atomics.  A chunk belongs to one sample; sample s begins at chunk
 // offsets[s] / R + s, which covers every sample's rows without a host copy of the offsets.
 //
-// Bound by HBM: x is read twice forward, x and dy twice backward (once each where they stay in
-// L2), y and dx written once with a streaming hint.  Four rows' loads are in flight per thread.
+// Bound by HBM for fp32 (200k x 256: 282 us for 1.64 GB of passes, 5.8 TB/s, 89 % of the measured
+// copy rate): x is read twice forward, x and dy twice backward, y and dx written once with a
+// streaming hint.  In 16 bits (100k x 512 bf16: 171 us for 0.82 GB, 4.8 TB/s) instruction issue
+// (55-59 %) and the MUFU unit come close beside it.  A floor of one reading each (62 and 125 us)
+// would need the chunks to stay on chip between the passes; they are 3 to 7 times what L2 keeps.
 #include <type_traits>
 
 #include "abi.h"
@@ -27,7 +30,9 @@ namespace hi3d {
 namespace gn {
 
 constexpr int kThreads = 256;
-constexpr int kInFlight = 6;  // rows whose loads a thread has in flight (two tensors: half)
+// Rows whose loads a thread has in flight (two tensors: half).  100k x 512 bf16, all kernels: four
+// rows 201 us, six 184, eight 217.
+constexpr int kInFlight = 6;
 
 struct Shape {
   int rows;                // all samples' rows
@@ -532,9 +537,11 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const T* __restrict__ x,
 // ---------------------------------------------------------------------------
 constexpr int kMaxGroups = 4096;  // a CTA holds a pair per group in shared memory
 
-// Chunks per SM: as many CTAs as run at once with the registers of the gradient kernels, so that no
-// second wave of a few CTAs follows, and the partial sums stay small beside x.
-constexpr int kChunksPerSm = 4;
+// Chunks per SM: as many CTAs as run at once with the rows in flight in registers (110-127 of them a
+// thread), so that no second wave follows and the partial sums stay small beside x.  100k x 512 bf16,
+// all kernels: two 171 us, four 184, three 208 (a second wave of a third of the SMs); holding the
+// registers to 85 or 64 for more CTAs spills (400 us and more).
+constexpr int kChunksPerSm = 2;
 
 static Shape make_shape(const hi3d_group_norm_args* a, bool wide) {
   Shape s;
