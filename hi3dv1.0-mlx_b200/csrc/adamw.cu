@@ -16,9 +16,13 @@
 // step would divide by it.
 //
 // Bound by HBM: 28 bytes an element (32-bit states; fp32 weights, or 16-bit with their master),
-// 16 with 8-bit states.  One warp takes a block at a time, lane l elements 4 l .. 4 l + 3 and
-// 128 + 4 l .. + 3, so every load and store of a warp is one contiguous run, 16 bytes a lane in
-// fp32, and the block's maxima are warp shuffles.  One launch takes up to kMost tensors: their
+// 16 with 8-bit states.  67M bf16 weights with 32-bit states: 281 us, 6.7 TB/s; 403M with 8-bit
+// states: 1247 us, 5.2 TB/s (79 % of the measured copy rate; 64 registers for two blocks a warp, four
+// CTAs an SM; without the block ahead 1853 us, with three or five CTAs 1413 or 1445).
+//
+// One warp takes a block at a time, lane l elements 4 l .. 4 l + 3 and 128 + 4 l .. + 3, so every
+// load and store of a warp is one contiguous run, 16 bytes a lane in fp32, and the block's maxima
+// are warp shuffles.  One launch takes up to kMost tensors: their
 // addresses travel in the kernel's parameters, so no table is copied to the device and the
 // launch can be captured.  A CTA finds its tensor by a binary search over the first chunks.
 #include <math.h>

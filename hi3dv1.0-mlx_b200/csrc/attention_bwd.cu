@@ -16,14 +16,25 @@
 // only lengthen the key CTAs' stream: the sum over the heads of a group and over the batch is
 // the same accumulation.
 //
-// CTA (640 threads; head dims over 64: 384): warp 0 loads (TMA ring of NST stages) and owns the TMEM; warps 1-3 issue the
+// CTA (384 threads): warp 0 loads (TMA ring of NST stages) and owns the TMEM; warps 1-3 issue the
 // MMAs, one each for S, T and the accumulators, so that none queues behind another's waits (a
-// wait costs 80-100 cycles even when it is over); the others compute, each four of them 32 of a
-// block's columns.
+// wait costs 80-100 cycles even when it is over); the other eight compute, each four of them half
+// of a block's columns.
 // TMEM: S is double-buffered, T single, then the accumulators.  P and dS (16-bit) are written
 // over the S columns that the same warp has read, and are the A operands of the last products.
 // S(j+2) runs when the accumulator products of j are done with its buffer, T(j+1) as soon as T(j)
 // has been read, so a compute warp finds the next block ready.
+//
+// What bounds it.  8192 x 16 x 64 bf16: 878 us, 783 TFLOP/s of the five products that a backward
+// pass cannot do without, 1096 of the seven done (67 % of the measured burst rate, and near the
+// power limit: a sustained loop runs at 1.55-1.7 GHz).  Counters at 4096: tensor pipe 47 %, FMA pipe
+// 49 %, MUFU 34 %, issue 51 %, DRAM 2 %: a scheduler's two compute warps take the exponentials, then
+// the products' elementwise part, in step, so no pipe is busy throughout.  Measured and not kept
+// (same size): 16 compute warps of half the columns 970 us; two CTAs an SM with 64-row blocks
+// 950-990 (a 64-column product reads 50 cycles' worth of shared memory in 33, and S, T and the
+// accumulators then form one chain); column sets with T, or S and T, of their own so that they drift
+// apart 905-935; T read before the exponentials 1044; barriers asked ahead of need 920-945.
+// 2049 x 16 over 4 heads of 128: 118 us, 1020 TFLOP/s of the seven products, tensor pipe 59 %.
 #include <type_traits>
 
 #include "abi.h"
@@ -35,7 +46,7 @@ namespace attn_bwd {
 constexpr int kRows = 128;           // stationary rows of a CTA
 constexpr float kLog2e = 1.4426950408889634f;
 // Of the 16 pairs of exponentials that a thread takes, those evaluated on the FMA pipe instead of
-// the MUFU unit.
+// the MUFU unit.  8192 x 16 x 64 bf16 on one box: four 910 us, five 916, six 871, seven 889, eight 912.
 constexpr int kEmuPairs = 6;
 // fp16 only: P is stored times 2^kPShift (P <= 1, so at most 256), which keeps probabilities
 // down to 2^-22 normal numbers; dV is divided by it at the end.
@@ -54,7 +65,7 @@ struct Params {
   int kv_seqs;    // key sets: num_seqs, or 1 when all sequences share one
   int q_tiles;    // row tiles of one query head: per sequence (dense) or over all (varlen)
   int kv_tiles;   // the same of one key head
-  int kv_ctas;    // key CTAs come first in the grid
+  int kv_ctas, kv_first, q_first;  // key CTAs, and where each kind begins in the grid
   int kv_splits, q_splits;
   float* part_kv;  // splits > 1: [split][2][key set][kv head][kv row][D] (dK, dV) in fp32
   float* part_q;   // [split][query batch][head][query row][D]
@@ -83,7 +94,7 @@ struct Cfg {
   static constexpr int ACC_COL = 3 * BN;  // dK or dQ, then dV
   // Stationary operands that fit beside them are copied into TMEM and read from there: a 64-column
   // product with both operands in shared memory is bound by its reads (50 cycles a K step where
-  // 33 would do).  With room for one it is X2.
+  // 33 would do).  With room for one it is X2.  2049 x 16 over 4 heads of 128: 119 us, without 130.
   static constexpr int X_COL = ACC_COL + (KV ? 2 : 1) * D;
   static constexpr int X_FIT = BN == 64 ? (512 - X_COL) / (D / 2) : 0;
   static constexpr bool X1_TMEM = X_FIT >= 2, X2_TMEM = X_FIT >= 1;
@@ -664,17 +675,19 @@ __global__ void __launch_bounds__(Cfg<D, true>::THREADS, 1)
                const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  if ((int)blockIdx.x < p.kv_ctas)
-    role<T, D, true>(&tmK, &tmV, &tmQs, &tmDOs, p, blockIdx.x, smem);
+  const int keys = (int)blockIdx.x - p.kv_first;
+  if (keys >= 0 && keys < p.kv_ctas)
+    role<T, D, true>(&tmK, &tmV, &tmQs, &tmDOs, p, keys, smem);
   else
-    role<T, D, false>(&tmQ, &tmDO, &tmKs, &tmVs, p, blockIdx.x - p.kv_ctas, smem);
+    role<T, D, false>(&tmQ, &tmDO, &tmKs, &tmVs, p, blockIdx.x - p.q_first, smem);
 }
 
 // Row statistics {-L log2e, -delta} in tiles of 128 rows, delta = rowsum(dO O) in fp32.  Blocks
 // [0, stat_blocks): one (tile, head, sequence) each; rows past the sequence's end get
 // probability 0.  fp16: these blocks also take the largest finite |dO|, and the blocks after
 // them the largest finite |V| (integer maxima of the bits: order does not matter).
-// Bound by HBM: reads O and dO once.
+// Reads O and dO once: 4096 x 16 x 64 bf16 6.8 us, 8192 11 us (3.1 TB/s; short, so its launch, the
+// first loads' latency and the tail count as much as the bytes).
 struct StatParams {
   const void *o, *d_o, *v;
   Strides so, sdo, sv;
@@ -763,7 +776,8 @@ __global__ void __launch_bounds__(256) stat_kernel(const Params p, const StatPar
   }
 }
 
-// Sums the fp32 partials of the splits in order and rounds them: out[batch][row][head][D].
+// Sums the fp32 partials of the splits in order and rounds them: out[batch][row][head][D].  8 bytes
+// of partials a split and value of dK, dV: two splits of 2049 x 4 x 128, 5.5 us.
 struct ReduceJob {
   const float* part;
   void* out;
@@ -806,6 +820,9 @@ __global__ void __launch_bounds__(256) reduce_kernel(const ReduceJob j0, const R
 struct Plan {
   int q_tiles, kv_tiles, kv_seqs, q_batches, kv_batches;
   int64_t kv_ctas, q_ctas;
+  // The kind with the longer streams starts first, so that none begins late.  64 queries on 8192
+  // keys, 16 heads of 64, bf16: 58 us, with the key CTAs first 101.
+  bool q_first;
   int kv_splits, q_splits;
   int64_t stat_bytes, kv_part, q_part;  // floats of one split's partials
   int64_t bytes;
@@ -814,13 +831,16 @@ struct Plan {
 static int64_t round256(int64_t b) { return (b + 255) & ~int64_t(255); }
 
 // How many CTAs share one tile's stream.  A CTA should not take longer than the mean load of an
-// SM (a CTA's stream counts one per block, its set-up and epilogue kSetup blocks): a short key
-// set under many queries (cross-attention), or a handful of tiles, would otherwise leave most
-// SMs idle behind a few long streams.  Each split costs a read and a write of fp32 partials, so
-// a part keeps at least kMinBlocks blocks.
+// SM (`ideal`, in blocks): a short key set under many queries (cross-attention), or a handful of
+// tiles, would otherwise leave most SMs idle behind a few long streams.  Each split costs a write
+// and a read of fp32 partials and one more launch, so a stream may be kSlack longer, and a part
+// keeps at least kMinBlocks blocks.  Whole backward pass in bf16, split against never split: 8192
+// queries on 77 keys, 16 heads of 64, 61 us against 77; 4 heads 26 against 72; 2049 x 8 over one key
+// head of 64 50 against 149; 2049 x 16 over 4 heads of 64 (kept whole) 81, split 86.
 static int split_count(int64_t steps, double ideal) {
   constexpr int kMinBlocks = 4;
-  if (steps <= ideal || steps < 2 * kMinBlocks) return 1;
+  constexpr double kSlack = 1.1;
+  if (steps <= kSlack * ideal || steps < 2 * kMinBlocks) return 1;
   const int64_t want = (int64_t)(steps / (ideal > kMinBlocks ? ideal : kMinBlocks) + 0.999);
   return (int)(want < 1 ? 1 : want > 64 ? 64 : want);
 }
@@ -843,13 +863,15 @@ static Plan make_plan(const hi3d_attn_bwd_args* a) {
   const int64_t q_steps = vk ? (k_blocks + a->num_seqs - 1) / a->num_seqs : k_blocks;
   const int64_t kv_tiles = (int64_t)n.kv_tiles * a->kv_heads * n.kv_batches;
   const int64_t q_tiles = (int64_t)n.q_tiles * a->heads * n.q_batches;
-  constexpr double kSetup = 3.0, kQueryCost = 0.8;  // a query block has 3 products where a key block has 4
-  const double load = kv_tiles * (kv_steps + kSetup) + q_tiles * (kQueryCost * q_steps + kSetup);
+  constexpr double kQueryCost = 0.8;       // a query block has 3 products where a key block has 4
+  const double setup = bn == 128 ? 6 : 8;  // a CTA's set-up and epilogue, about 7 us
+  const double load = kv_tiles * (kv_steps + setup) + q_tiles * (kQueryCost * q_steps + setup);
   const double ideal = load / sm_count();
   n.kv_splits = split_count(kv_steps, ideal);
   n.q_splits = split_count(q_steps, ideal / kQueryCost);
   n.kv_ctas = kv_tiles * n.kv_splits;
   n.q_ctas = q_tiles * n.q_splits;
+  n.q_first = kQueryCost * q_steps / n.q_splits > (double)kv_steps / n.kv_splits;
   const int64_t stat_tiles = (int64_t)n.q_tiles * a->heads * n.q_batches;
   n.stat_bytes = round256(stat_tiles * kRows * 8);
   n.kv_part = (int64_t)n.kv_batches * a->kv_heads * a->nk * a->head_dim;
@@ -923,7 +945,8 @@ static int launch(const hi3d_attn_bwd_args* a, const Plan& n, uint8_t* ws, cudaS
   p.num_seqs = a->num_seqs, p.heads = a->heads, p.kv_heads = a->kv_heads, p.group = a->heads / a->kv_heads;
   p.kv_seqs = n.kv_seqs;
   p.q_tiles = n.q_tiles, p.kv_tiles = n.kv_tiles;
-  p.kv_ctas = (int)n.kv_ctas, p.kv_splits = n.kv_splits, p.q_splits = n.q_splits;
+  p.kv_ctas = (int)n.kv_ctas, p.kv_first = n.q_first ? (int)n.q_ctas : 0, p.q_first = n.q_first ? 0 : (int)n.kv_ctas;
+  p.kv_splits = n.kv_splits, p.q_splits = n.q_splits;
   p.scale = a->scale, p.scale2 = a->scale * kLog2e;
   p.amax = reinterpret_cast<const unsigned*>(ws);
   p.stat = reinterpret_cast<const float4*>(ws + 256);

@@ -155,41 +155,6 @@ static __device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parit
   return false;
 }
 
-// The same wait parked in hardware: each poll may suspend the warp for up to kParkNs until the
-// phase completes, so a waiting warp takes no issue slots from the computing ones.  For kernels
-// whose many waiting warps share schedulers with compute warps.
-constexpr uint32_t kParkNs = 20000;
-
-__device__ __forceinline__ bool mbar_try_wait_parked(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity), "r"(kParkNs)
-      : "memory");
-  return ok != 0;
-}
-
-static __device__ __noinline__ bool mbar_wait_parked_slow(uint64_t* bar, uint32_t parity, volatile int* abort,
-                                                          int where) {
-  const uint64_t t0 = global_ns();
-  for (uint32_t i = 0; i < kSpinLimit; ++i) {
-    if (mbar_try_wait_parked(bar, parity)) return true;
-    if (*abort) return false;
-    if (global_ns() - t0 > kWaitNs) break;
-  }
-  report_error(HI3D_ERR_DEVICE_TIMEOUT, where, (int)parity);
-  *abort = 1;
-  return false;
-}
-
-__device__ __forceinline__ bool mbar_wait_parked(uint64_t* bar, uint32_t parity, volatile int* abort, int where) {
-  if (mbar_try_wait_parked(bar, parity)) return true;
-  return mbar_wait_parked_slow(bar, parity, abort, where);
-}
-
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int where) {
   if (mbar_try_wait(bar, parity)) return true;
   return mbar_wait_slow(bar, parity, abort, where);
@@ -389,12 +354,6 @@ __device__ __forceinline__ void tmem_st_16x256b_x4(uint32_t taddr, const uint32_
 __device__ __forceinline__ void tmem_st_16x128b_x4(uint32_t taddr, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
                "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
-}
-
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
-               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
 

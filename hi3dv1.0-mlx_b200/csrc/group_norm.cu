@@ -584,7 +584,8 @@ static int check_args(const hi3d_group_norm_args* a) {
   return HI3D_OK;
 }
 
-// 16-byte accesses: whole vectors in a row, and aligned addresses
+// 16-byte accesses: whole vectors in a row, and aligned addresses.  100k x 512 bf16, the four passes:
+// 162 us, 357 one value at a time; 200k x 256 fp32 274 and 520.  (512 x 256 fp16: 18 and 13.)
 static bool is_wide(const hi3d_group_norm_args* a, const void* p, const void* q, const void* r) {
   const int vec = a->dtype == HI3D_F32 ? 4 : 8;
   return a->channels % vec == 0 && aligned16(p) && aligned16(q) && aligned16(r);
@@ -646,6 +647,8 @@ static int run(const hi3d_group_norm_args* a, const Shape& s, bool wide, uint8_t
   float2* part = reinterpret_cast<float2*>(ws);
   float2* chan = reinterpret_cast<float2*>(ws + round256((int64_t)s.chunks * s.channels * 8));
   if (!wide) return pick_act<T, FWD, 1, true>(a, s, part, chan, st);
+  // A vector inside one group keeps one mean and factor instead of V: the gradient's two passes at
+  // 100k x 512 bf16 take 100 us against 129.
   return s.channels / s.groups % V == 0 ? pick_act<T, FWD, V, true>(a, s, part, chan, st)
                                         : pick_act<T, FWD, V, false>(a, s, part, chan, st);
 }
