@@ -4,10 +4,10 @@
 //   p <- p - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // all in fp32.  The moments' products and sums are rounded one by one (no contraction), so the
-// 8-bit codes do not depend on how a compiler fuses; the root and the quotient are the MUFU
-// unit's (2 units in the last place each, on an update that is itself a small part of p): with
-// correctly rounded ones the 8-bit step was bound by issue, not by HBM.  16-bit weights are the
-// rounded copy of an fp32 master.
+// 8-bit codes do not depend on how a compiler fuses; the root and the quotient of the update are
+// the MUFU unit's (2 units in the last place each, on an update that is itself a small part of p):
+// with a correctly rounded quotient the 8-bit step was bound by issue, not by HBM.  What is coded
+// is the correctly rounded root.  16-bit weights are the rounded copy of an fp32 master.
 //
 // The states of all tensors lie in flat buffers, each tensor beginning at a multiple of kBlock
 // elements.  8 bits: a block of kBlock values of m, and of u = sqrt(v), is stored as e4m3 codes
@@ -134,13 +134,11 @@ __device__ __forceinline__ float root_approx(float x) {
   return r;
 }
 
-// u: the root of the new v
-__device__ __forceinline__ void update(const Params& a, float gs, float& p, float g, float& m, float& v, float& u) {
+__device__ __forceinline__ void update(const Params& a, float gs, float& p, float g, float& m, float& v) {
   g = __fmul_rn(g, gs);
   m = __fadd_rn(__fmul_rn(m, a.b1), __fmul_rn(g, a.b1c));
   v = __fadd_rn(__fmul_rn(v, a.b2), __fmul_rn(__fmul_rn(g, g), a.b2c));
-  u = root_approx(v);
-  const float den = __fadd_rn(__fmul_rn(u, a.root), a.eps);
+  const float den = __fadd_rn(__fmul_rn(root_approx(v), a.root), a.eps);
   p = __fsub_rn(__fmul_rn(p, a.decay), __fmul_rn(__fdividef(m, den), a.step));
 }
 
@@ -184,7 +182,7 @@ struct Block {
   }
 };
 
-// New moments of four values in m and v (8 bits: v holds its root) and weights in w.
+// New moments of four values in m and v (8 bits: v comes in as its root's codes) and weights in w.
 template <bool EIGHT>
 __device__ __forceinline__ void update4(const Params& a, float gs, float sm, float su, const float (&g)[4],
                                         float (&w)[4], float (&m)[4], float (&v)[4]) {
@@ -195,32 +193,35 @@ __device__ __forceinline__ void update4(const Params& a, float gs, float sm, flo
       const float u = __fmul_rn(v[k], su);
       v[k] = __fmul_rn(u, u);
     }
-    float u;
-    update(a, gs, w[k], g[k], m[k], v[k], u);
-    if constexpr (EIGHT) v[k] = u;
+    update(a, gs, w[k], g[k], m[k], v[k]);
   }
 }
 
-// The states of a block whose lane holds m and v (its root), written with their scales.
+// The states of a block whose lane holds m and v, written with their scales.  The root is taken
+// again, correctly rounded: beside the middle of two codes the MUFU unit's would get the other one,
+// a sixteenth of the value, once in 3 million values.
 __device__ __forceinline__ void store_codes(const Params& a, int64_t f, float (&m)[2][4], float (&v)[2][4]) {
-  float big_m = 0.f, big_u = 0.f;
+  float big_m = 0.f, big_v = 0.f;
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) big_m = fmaxf(big_m, fabsf(m[h][k])), big_u = fmaxf(big_u, v[h][k]);
-  const float sm = __fmul_rn(warp_max(big_m), 1.0f / 448.0f), su = __fmul_rn(warp_max(big_u), 1.0f / 448.0f);
+    for (int k = 0; k < 4; ++k) big_m = fmaxf(big_m, fabsf(m[h][k])), big_v = fmaxf(big_v, v[h][k]);
+  const float sm = __fmul_rn(warp_max(big_m), 1.0f / 448.0f);
+  const float su = __fmul_rn(__fsqrt_rn(warp_max(big_v)), 1.0f / 448.0f);
   const float im = inverse(sm), iu = inverse(su);
   if (lane_id() == 0) a.scale_m[f / kBlock] = sm, a.scale_u[f / kBlock] = su;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      m[h][k] = __fmul_rn(m[h][k], im);
-      const float c = __fmul_rn(v[h][k], iu);
-      v[h][k] = v[h][k] > 0.f && iu > 0.f ? (c < 0x1p-9f ? 0x1p-9f : c) : c;
-    }
+    for (int k = 0; k < 4; ++k) m[h][k] = __fmul_rn(m[h][k], im);
     *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.m) + f + h * 128) = encode4(m[h]);
-    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.v) + f + h * 128) = encode4(v[h]);
+    float c[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      c[k] = __fmul_rn(__fsqrt_rn(v[h][k]), iu);
+      if (v[h][k] > 0.f && iu > 0.f) c[k] = fmaxf(c[k], 0x1p-9f);
+    }
+    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.v) + f + h * 128) = encode4(c);
   }
 }
 
@@ -330,7 +331,8 @@ __global__ void __launch_bounds__(kWarps * 32, EIGHT ? kCtas8 : 1)
 }
 
 // Tables of two sizes: the parameters of a launch are copied with it, 2 KB for the usual handful
-// of tensors, 24 KB for a model's hundreds.
+// of tensors, 24 KB for a model's hundreds (12 tensors of 9216: a step takes 53 us on the host, with
+// the large table 56).
 constexpr int kFew = 64, kMost = 768;
 
 template <typename P, bool EIGHT, int MOST>

@@ -160,6 +160,32 @@ def test_zero_tiny_and_huge_gradients(bits):
     assert torch.isfinite(f.params[0]).all()
 
 
+def test_8_bit_codes_are_those_of_correctly_rounded_operations():
+    """The states' operations one by one in fp32, each rounded to nearest: every code and scale equal.
+
+    No tolerance: where a root off by one in its last place crosses the middle of two codes, its
+    code differs, about once in 3 million values, so ten times here.
+    """
+    flat = Flat([(1 << 25,)], torch.float32, 8, seed=31)
+    f32 = lambda x: torch.tensor(x, dtype=torch.float32)  # noqa: E731
+    b1, b2 = HYPER["betas"]
+    blocks = lambda t: t.view(-1, optim.BLOCK)  # noqa: E731
+    scales, g = flat.scales.cpu(), flat.grads[0].cpu()
+    m = (blocks(flat.m.cpu().float()) * scales[0][:, None]).view(-1)
+    v = (blocks(flat.v.cpu().float()) * scales[1][:, None]).square().view(-1)
+    m = m * f32(b1) + g * f32(1 - b1)
+    v = v * f32(b2) + (g * g) * f32(1 - b2)
+    u = v.double().sqrt().float()  # float32 roots of the CPU may be off by one
+    scales = torch.stack([blocks(m).abs().amax(1), blocks(u).amax(1)]) * f32(1 / 448)
+    inv = scales.reciprocal()
+    c = torch.where(blocks(u) > 0, (blocks(u) * inv[1][:, None]).clamp_min(2.0 ** -9), 0.0)
+    flat.step(3)
+    assert torch.equal(flat.scales.cpu(), scales)
+    code = lambda t: t.to(torch.float8_e4m3fn).view(torch.uint8).view(-1)  # noqa: E731
+    assert torch.equal(flat.m.cpu().view(torch.uint8), code(blocks(m) * inv[0][:, None]))
+    assert torch.equal(flat.v.cpu().view(torch.uint8), code(c))
+
+
 def test_a_nan_gradient_spoils_its_own_value_only():
     for bits in (32, 8):
         a, b = Flat([(600,)], torch.float32, bits, seed=12), Flat([(600,)], torch.float32, bits, seed=12)
