@@ -16,9 +16,9 @@
 // step would divide by it.
 //
 // Bound by HBM: 28 bytes an element (32-bit states; fp32 weights, or 16-bit with their master),
-// 16 with 8-bit states.  67M bf16 weights with 32-bit states: 281 us, 6.7 TB/s; 403M with 8-bit
-// states: 1247 us, 5.2 TB/s (79 % of the measured copy rate; 64 registers for two blocks a warp, four
-// CTAs an SM; without the block ahead 1853 us, with three or five CTAs 1413 or 1445).
+// 16 with 8-bit states.  67M bf16 weights with 32-bit states: 274 us, 6.9 TB/s; 403M with 8-bit
+// states: 1126 us, 5.7 TB/s (88 % of the measured copy rate; 64 registers a thread hold two blocks of
+// a warp, 32 warps an SM; with 28 warps 1180 us, with 40, which spill, 1363).
 //
 // One warp takes a block at a time, lane l elements 4 l .. 4 l + 3 and 128 + 4 l .. + 3, so every
 // load and store of a warp is one contiguous run, 16 bytes a lane in fp32, and the block's maxima
@@ -36,9 +36,14 @@ namespace hi3d {
 namespace adamw {
 
 constexpr int kBlock = HI3D_ADAMW_BLOCK;
-constexpr int kWarps = 8;
-constexpr int kChunk = 4 * kWarps * kBlock;  // elements of a CTA
-constexpr int kCtas8 = 4;                    // CTAs an SM holds with 8-bit states (at most 64 registers)
+// Warps of a CTA: 403M bf16 weights with 8-bit states, two 1131 us, four 1126, eight 1153.
+constexpr int kWarps = 4;
+constexpr int kCtas8 = 8;  // CTAs an SM holds with 8-bit states (at most 64 registers)
+// Elements of a CTA: a block a warp, with 8-bit states two, the second of which is loaded while the
+// first is computed.  (8 bits, eight warps: one 1261 us, two 1145, three 1197, four 1208; 32 bits,
+// 67M weights: one 273, two 278, four 281.)
+template <bool EIGHT>
+constexpr int kChunk = (EIGHT ? 2 : 1) * kWarps * kBlock;
 
 struct Entry {
   void* p;
@@ -305,9 +310,9 @@ __global__ void __launch_bounds__(kWarps * 32, EIGHT ? kCtas8 : 1)
   const float gs = a.grad_scale ? *a.grad_scale : 1.0f;
   const bool wide = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) & (4 * sizeof(P) - 1)) == 0;
   constexpr int kStep = kWarps * kBlock;
-  const int64_t first = (int64_t)(blockIdx.x - e.chunk) * kChunk, n = e.n;
+  const int64_t first = (int64_t)(blockIdx.x - e.chunk) * kChunk<EIGHT>, n = e.n;
   int64_t at = first + warp_id() * kBlock;
-  const int64_t end = min(first + kChunk, n);
+  const int64_t end = min(first + kChunk<EIGHT>, n);
   const int64_t fast = wide ? end - kBlock : at - 1;  // whole blocks begin up to here
   const int64_t lane4 = lane_id() * 4, flat = (int64_t)e.at * kBlock + lane4;
   if constexpr (EIGHT) {
@@ -347,7 +352,7 @@ static int launch(const hi3d_adamw_args* a, const Params& base, int from, int co
     e.p = a->params[i], e.g = a->grads[i], e.n = a->numels[i];
     e.at = (uint32_t)(a->offsets[i] / kBlock);
     e.chunk = (uint32_t)chunks;
-    chunks += (uint64_t)((a->numels[i] + kChunk - 1) / kChunk);
+    chunks += (uint64_t)((a->numels[i] + kChunk<EIGHT> - 1) / kChunk<EIGHT>);
     if (chunks > 0x7fffffffu) return set_error(HI3D_ERR_INVALID_ARGUMENT, "adamw_step: too many elements");
   }
   if (p.count == 0) return HI3D_OK;
