@@ -18,7 +18,8 @@
 // Bound by HBM: 28 bytes an element (32-bit states; fp32 weights, or 16-bit with their master),
 // 16 with 8-bit states.  67M bf16 weights with 32-bit states: 274 us, 6.9 TB/s; 403M with 8-bit
 // states: 1126 us, 5.7 TB/s (88 % of the measured copy rate; 64 registers a thread hold two blocks of
-// a warp, 32 warps an SM; with 28 warps 1180 us, with 40, which spill, 1363).
+// a warp, 32 warps an SM; with 28 warps 1180 us, with 40, which spill, 1363); there instruction issue
+// (79 %) is as near its limit as HBM.
 //
 // One warp takes a block at a time, lane l elements 4 l .. 4 l + 3 and 128 + 4 l .. + 3, so every
 // load and store of a warp is one contiguous run, 16 bytes a lane in fp32, and the block's maxima

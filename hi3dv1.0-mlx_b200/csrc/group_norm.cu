@@ -19,7 +19,7 @@
 // Bound by HBM for fp32 (200k x 256: 282 us for 1.64 GB of passes, 5.8 TB/s, 89 % of the measured
 // copy rate): x is read twice forward, x and dy twice backward, y and dx written once with a
 // streaming hint.  In 16 bits (100k x 512 bf16: 171 us for 0.82 GB, 4.8 TB/s) instruction issue
-// (55-59 %) and the MUFU unit come close beside it.  A floor of one reading each (62 and 125 us)
+// (54-60 %) and the MUFU unit come close beside it.  A floor of one reading each (62 and 125 us)
 // would need the chunks to stay on chip between the passes; they are 3 to 7 times what L2 keeps.
 #include <type_traits>
 
