@@ -682,15 +682,24 @@ __global__ void __launch_bounds__(Cfg<D, true>::THREADS, 1)
     role<T, D, false>(&tmQ, &tmDO, &tmKs, &tmVs, p, blockIdx.x - p.q_first, smem);
 }
 
-// Row statistics {-L log2e, -delta} in tiles of 128 rows, delta = rowsum(dO O) in fp32.  Blocks
+// Over this many keys or fewer delta is summed from P and dP (below).
+constexpr int kFewKeys = 16;
+// CTAs an SM: the kernel is short and waits for its loads.  8192 x 16 x 64 bf16: eight 8.4 us (32
+// registers, a little spilled), six 11.4, unbounded (74 registers) 15.3.
+constexpr int kStatCtas = 8;
+
+// Row statistics {-L log2e, -delta} in tiles of 128 rows, delta = rowsum(dO O) in fp32.  Over few
+// keys delta nearly cancels dP, and O's rounding in it would be most of dS's error (dQ in bf16, 512
+// queries: 2 keys 0.0040 relative, 5 0.0029, 16 and more 0.0025): there delta = sum P dP / sum P,
+// the products done again here, 16 FMAs a key and 8 channels (then 0.0024 throughout).  Blocks
 // [0, stat_blocks): one (tile, head, sequence) each; rows past the sequence's end get
 // probability 0.  fp16: these blocks also take the largest finite |dO|, and the blocks after
 // them the largest finite |V| (integer maxima of the bits: order does not matter).
-// Reads O and dO once: 4096 x 16 x 64 bf16 6.8 us, 8192 11 us (3.1 TB/s; short, so its launch, the
+// Reads O and dO once: 4096 x 16 x 64 bf16 7.2 us, 8192 8.4 us (4.0 TB/s; short, so its launch, the
 // first loads' latency and the tail count as much as the bytes).
 struct StatParams {
-  const void *o, *d_o, *v;
-  Strides so, sdo, sv;
+  const void *o, *d_o, *q, *k, *v;
+  Strides so, sdo, sq, sk, sv;
   const float* lse;
   float* stat;
   unsigned* amax;
@@ -712,8 +721,74 @@ __device__ __forceinline__ float abs_max8(uint4 u, float m) {
   return m;
 }
 
+// Products of 8 channels, summed
+template <typename T>
+__device__ __forceinline__ float dot8(uint4 a, uint4 b) {
+  uint64_t sum = f2_mul(Cvt<T>::to_f2(a.x), Cvt<T>::to_f2(b.x));
+  sum = f2_fma(Cvt<T>::to_f2(a.y), Cvt<T>::to_f2(b.y), sum);
+  sum = f2_fma(Cvt<T>::to_f2(a.z), Cvt<T>::to_f2(b.z), sum);
+  sum = f2_fma(Cvt<T>::to_f2(a.w), Cvt<T>::to_f2(b.w), sum);
+  float x, y;
+  f2_unpack(sum, x, y);
+  return x + y;
+}
+
+// One value pair of a tile's row
+__device__ __forceinline__ void put_stat(const StatParams& q, int64_t tile, int r, float l, float delta) {
+  float* dst = q.stat + (tile * kRows + (r & ~1)) * 2 + (r & 1);
+  dst[0] = l, dst[2] = delta;
+}
+
+// The statistics of a tile whose sequence has at most kFewKeys keys.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) stat_kernel(const Params p, const StatParams q) {
+__device__ __forceinline__ void few_keys(const Params& p, const StatParams& q, int t, int h, int b, int64_t tile,
+                                      float& big) {
+  constexpr bool kHalf = std::is_same<T, __half>::value;
+  constexpr int L = D == 64 ? 8 : 16;
+  constexpr float shift = kHalf ? (float)kPShift : 0.f;
+  const int sub = threadIdx.x % L, batch = p.cu_q ? 0 : b, kb = p.cu_k || p.kv_seqs == 1 ? 0 : b;
+  int64_t start, len, k_start, keys;
+  seq_range(p.cu_q, b, p.nq, start, len);
+  seq_range(p.cu_k, b, p.nk, k_start, keys);
+  const T* x = static_cast<const T*>(q.q) + batch * q.sq.batch + (int64_t)h * q.sq.head + sub * 8;
+  const T* d = static_cast<const T*>(q.d_o) + batch * q.sdo.batch + (int64_t)h * q.sdo.head + sub * 8;
+  const T* k = static_cast<const T*>(q.k) + kb * q.sk.batch + (int64_t)(h / p.group) * q.sk.head + sub * 8;
+  const T* v = static_cast<const T*>(q.v) + kb * q.sv.batch + (int64_t)(h / p.group) * q.sv.head + sub * 8;
+#pragma unroll 1
+  for (int r = threadIdx.x / L; r < kRows; r += 256 / L) {
+    const int64_t row = (int64_t)t * kRows + r;
+    const bool in = row < len && sub * 8 < D;
+    uint4 a = make_uint4(0, 0, 0, 0), g = a;
+    if (in) {
+      a = *reinterpret_cast<const uint4*>(x + (start + row) * q.sq.row);
+      g = *reinterpret_cast<const uint4*>(d + (start + row) * q.sdo.row);
+    }
+    const float l = row < len ? q.lse[((int64_t)batch * p.heads + h) * p.nq + start + row] * kLog2e : 0.f;
+    if constexpr (kHalf) big = abs_max8<T, D>(g, big);
+    float sum = 0.f, delta = 0.f;
+#pragma unroll 1
+    for (int j = 0; j < (int)keys; ++j) {
+      float s = 0.f, dp = 0.f;
+      if (in) {
+        s = dot8<T>(a, *reinterpret_cast<const uint4*>(k + (k_start + j) * q.sk.row));
+        dp = dot8<T>(g, *reinterpret_cast<const uint4*>(v + (k_start + j) * q.sv.row));
+      }
+#pragma unroll
+      for (int m = L / 2; m > 0; m >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, m);
+        dp += __shfl_xor_sync(0xffffffffu, dp, m);
+      }
+      const float e = exp2f(fmaf(s, p.scale2, -l));
+      sum += e, delta = fmaf(e, dp, delta);
+    }
+    // sum is 1 up to the log-sum-exp's rounding, which must not part delta from dP
+    if (sub == 0) put_stat(q, tile, r, row < len ? shift - l : -INFINITY, row < len && keys > 0 ? -delta / sum : 0.f);
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256, kStatCtas)
+    stat_kernel(const __grid_constant__ Params p, const __grid_constant__ StatParams q) {
   constexpr bool kHalf = std::is_same<T, __half>::value;
   constexpr int L = D == 64 ? 8 : 16;  // lanes of a row, 8 channels each (96: 12 of 16 work)
   const int sub = threadIdx.x % L;
@@ -735,29 +810,27 @@ __global__ void __launch_bounds__(256) stat_kernel(const Params p, const StatPar
     if (t < 0 || (int64_t)t * kRows >= len) return;
     const T* o = static_cast<const T*>(q.o) + batch * q.so.batch + (int64_t)h * q.so.head + sub * 8;
     const T* d = static_cast<const T*>(q.d_o) + batch * q.sdo.batch + (int64_t)h * q.sdo.head + sub * 8;
+    int64_t k_start, keys;
+    seq_range(p.cu_k, b, p.nk, k_start, keys);
+    if (keys <= kFewKeys) {
+      few_keys<T, D>(p, q, t, h, b, tile, big);
+    } else {
 #pragma unroll 4
-    for (int r = threadIdx.x / L; r < kRows; r += 256 / L) {
-      const int64_t row = (int64_t)t * kRows + r;
-      float acc = 0.f;
-      if (row < len && on) {
-        const uint4 a = *reinterpret_cast<const uint4*>(o + (start + row) * q.so.row);
-        const uint4 g = *reinterpret_cast<const uint4*>(d + (start + row) * q.sdo.row);
-        uint64_t sum = f2_mul(Cvt<T>::to_f2(a.x), Cvt<T>::to_f2(g.x));
-        sum = f2_fma(Cvt<T>::to_f2(a.y), Cvt<T>::to_f2(g.y), sum);
-        sum = f2_fma(Cvt<T>::to_f2(a.z), Cvt<T>::to_f2(g.z), sum);
-        sum = f2_fma(Cvt<T>::to_f2(a.w), Cvt<T>::to_f2(g.w), sum);
-        float x, y;
-        f2_unpack(sum, x, y);
-        acc = x + y;
-        if constexpr (kHalf) big = abs_max8<T, D>(g, big);
-      }
+      for (int r = threadIdx.x / L; r < kRows; r += 256 / L) {
+        const int64_t row = (int64_t)t * kRows + r;
+        float acc = 0.f;
+        if (row < len && on) {
+          const uint4 a = *reinterpret_cast<const uint4*>(o + (start + row) * q.so.row);
+          const uint4 g = *reinterpret_cast<const uint4*>(d + (start + row) * q.sdo.row);
+          acc = dot8<T>(a, g);
+          if constexpr (kHalf) big = abs_max8<T, D>(g, big);
+        }
 #pragma unroll
-      for (int m = L / 2; m > 0; m >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, m);
-      if (sub == 0) {
-        float* dst = q.stat + (tile * kRows + (r & ~1)) * 2 + (r & 1);
-        dst[0] = row < len ? -q.lse[((int64_t)batch * p.heads + h) * p.nq + start + row] * kLog2e + shift
-                               : -INFINITY;
-        dst[2] = row < len ? -acc : 0.f;
+        for (int m = L / 2; m > 0; m >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, m);
+        if (sub == 0)
+          put_stat(q, tile, r,
+                   row < len ? shift - q.lse[((int64_t)batch * p.heads + h) * p.nq + start + row] * kLog2e : -INFINITY,
+                   row < len ? -acc : 0.f);
       }
     }
   } else {
@@ -954,9 +1027,11 @@ static int launch(const hi3d_attn_bwd_args* a, const Plan& n, uint8_t* ws, cudaS
   p.part_q = p.part_kv + (n.kv_splits > 1 ? round256(n.kv_part * 2 * n.kv_splits * 4) / 4 : 0);
 
   StatParams q;
-  q.o = a->out, q.d_o = a->dout, q.v = a->v;
+  q.o = a->out, q.d_o = a->dout, q.q = a->q, q.k = a->k, q.v = a->v;
   q.so = {a->o_row, a->o_head, a->o_batch};
   q.sdo = {a->do_row, a->do_head, a->do_batch};
+  q.sq = {a->q_row, a->q_head, a->q_batch};
+  q.sk = {a->k_row, a->k_head, a->k_batch};
   q.sv = {a->v_row, a->v_head, a->v_batch};
   q.lse = a->lse;
   q.stat = reinterpret_cast<float*>(ws + 256);

@@ -129,6 +129,33 @@ def test_one_key_has_no_score_gradient():
     assert torch.equal(out, v.expand_as(out))
 
 
+@pytest.mark.parametrize("dim,dtype", [(64, torch.bfloat16), (96, torch.float16), (128, torch.bfloat16)])
+@pytest.mark.parametrize("nk", [2, 3, 7, 16, 17])
+def test_few_keys_keep_their_bits(dim, dtype, nk):
+    """Over a few keys delta nearly cancels dP, so that the saved output's rounding would be most of
+    dS's error.  Without it a score gradient carries two roundings, of dS and its own: 0.64 u in
+    quadrature, checked at 0.8 u.  From 17 keys on the output's is small beside them.  A dense set,
+    and a sequence beside others of one and no key."""
+    q, do = _rand((2, 3, 700, dim), dtype, 41), _rand((2, 3, 700, dim), dtype, 42)
+    k, v = _rand((2, 3, nk, dim), dtype, 43), _rand((2, 3, nk, dim), dtype, 44)
+
+    def close(name, got, want):
+        err, tol = (got.double() - want).norm(), 0.8 * U[dtype] * want.norm()
+        assert err <= tol, f"{name}: {err:.3e} > {tol:.3e}"
+
+    out, lse, dq, dk, dv = dense(q, k, v, do, dim ** -0.5)
+    e = exact(q, k, v, do, dim ** -0.5)
+    close("dq", dq, e[2])
+    close("dk", dk, e[3])
+    one = lambda t: t[0].transpose(0, 1).contiguous()  # noqa: E731
+    cu_q, cu_k = [0, 5, 5, 700], [0, 1, 1, nk + 1]
+    kk, vv = (torch.cat([one(t)[:1], one(t)]) for t in (k, v))
+    got = packed(one(q), kk, vv, one(do), cu_q, cu_k, dim ** -0.5)
+    e = exact(q[:1, :, 5:], k[:1], v[:1], do[:1, :, 5:], dim ** -0.5)
+    close("packed dq", got[2][5:], e[2][0].transpose(0, 1))
+    close("packed dk", got[3][1:], e[3][0].transpose(0, 1))
+
+
 @pytest.mark.parametrize("mul", [1e-4, 1e-2, 300.0])
 def test_fp16_gradients_of_any_size_keep_their_bits(mul):
     """dS = P (dP - delta) is far below fp16's normal range for small gradients over many keys and
