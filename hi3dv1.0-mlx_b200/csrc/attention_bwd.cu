@@ -685,13 +685,16 @@ __global__ void __launch_bounds__(Cfg<D, true>::THREADS, 1)
 // Over this many keys or fewer delta is summed from P and dP (below).
 constexpr int kFewKeys = 16;
 // CTAs an SM: the kernel is short and waits for its loads.  8192 x 16 x 64 bf16: eight 8.4 us (32
-// registers, a little spilled), six 11.4, unbounded (74 registers) 15.3.
-constexpr int kStatCtas = 8;
+// registers, a little spilled), six 11.4, unbounded 15.3.  The form for few keys needs registers:
+// 16384 x 16 queries on 16 keys, the whole pass, four 200 us, five 202, six 211; packed 5873 x 22 x 96
+// fp16, this kernel, 23.2, 21.8, 21.0.
+constexpr int kStatCtas = 8, kFewCtas = 5;
 
 // Row statistics {-L log2e, -delta} in tiles of 128 rows, delta = rowsum(dO O) in fp32.  Over few
 // keys delta nearly cancels dP, and O's rounding in it would be most of dS's error (dQ in bf16, 512
 // queries: 2 keys 0.0040 relative, 5 0.0029, 16 and more 0.0025): there delta = sum P dP / sum P,
-// the products done again here, 16 FMAs a key and 8 channels (then 0.0024 throughout).  Blocks
+// the products done again here, 16 FMAs a key and 8 channels (then 0.0024 throughout; 4096 x 16 queries,
+// the whole pass: 4 keys 45 us, 16 keys 62, 36 without).  Blocks
 // [0, stat_blocks): one (tile, head, sequence) each; rows past the sequence's end get
 // probability 0.  fp16: these blocks also take the largest finite |dO|, and the blocks after
 // them the largest finite |V| (integer maxima of the bits: order does not matter).
@@ -739,14 +742,18 @@ __device__ __forceinline__ void put_stat(const StatParams& q, int64_t tile, int 
   dst[0] = l, dst[2] = delta;
 }
 
-// The statistics of a tile whose sequence has at most kFewKeys keys.
+// The statistics of a tile whose sequence has at most kFewKeys keys.  Four keys at a time: their
+// eight products are summed across a row's lanes by a transposing exchange (8 shuffles where a sum
+// each would take 24), after which a lane has one key.
 template <typename T, int D>
 __device__ __forceinline__ void few_keys(const Params& p, const StatParams& q, int t, int h, int b, int64_t tile,
-                                      float& big) {
+                                         float& big) {
   constexpr bool kHalf = std::is_same<T, __half>::value;
   constexpr int L = D == 64 ? 8 : 16;
   constexpr float shift = kHalf ? (float)kPShift : 0.f;
+  constexpr uint32_t kAll = 0xffffffffu;
   const int sub = threadIdx.x % L, batch = p.cu_q ? 0 : b, kb = p.cu_k || p.kv_seqs == 1 ? 0 : b;
+  const bool dp_lane = sub & 4, high2 = sub & 2, high1 = sub & 1;
   int64_t start, len, k_start, keys;
   seq_range(p.cu_q, b, p.nq, start, len);
   seq_range(p.cu_k, b, p.nk, k_start, keys);
@@ -758,36 +765,52 @@ __device__ __forceinline__ void few_keys(const Params& p, const StatParams& q, i
   for (int r = threadIdx.x / L; r < kRows; r += 256 / L) {
     const int64_t row = (int64_t)t * kRows + r;
     const bool in = row < len && sub * 8 < D;
-    uint4 a = make_uint4(0, 0, 0, 0), g = a;
-    if (in) {
-      a = *reinterpret_cast<const uint4*>(x + (start + row) * q.sq.row);
-      g = *reinterpret_cast<const uint4*>(d + (start + row) * q.sdo.row);
-    }
-    const float l = row < len ? q.lse[((int64_t)batch * p.heads + h) * p.nq + start + row] * kLog2e : 0.f;
-    if constexpr (kHalf) big = abs_max8<T, D>(g, big);
-    float sum = 0.f, delta = 0.f;
+    float sum = 0.f, delta = 0.f, l = 0.f;
+    if (__any_sync(kAll, in)) {
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      const uint4 a = in ? *reinterpret_cast<const uint4*>(x + (start + row) * q.sq.row) : zero;
+      const uint4 g = in ? *reinterpret_cast<const uint4*>(d + (start + row) * q.sdo.row) : zero;
+      if (row < len) l = q.lse[((int64_t)batch * p.heads + h) * p.nq + start + row] * kLog2e;
+      if constexpr (kHalf) big = abs_max8<T, D>(g, big);
 #pragma unroll 1
-    for (int j = 0; j < (int)keys; ++j) {
-      float s = 0.f, dp = 0.f;
-      if (in) {
-        s = dot8<T>(a, *reinterpret_cast<const uint4*>(k + (k_start + j) * q.sk.row));
-        dp = dot8<T>(g, *reinterpret_cast<const uint4*>(v + (k_start + j) * q.sv.row));
+      for (int j = 0; j < (int)keys; j += 4) {
+        float e8[8], e4[4], e2[2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool have = in && j + i < (int)keys;
+          e8[i] = dot8<T>(a, have ? *reinterpret_cast<const uint4*>(k + (k_start + j + i) * q.sk.row) : zero);
+          e8[i + 4] = dot8<T>(g, have ? *reinterpret_cast<const uint4*>(v + (k_start + j + i) * q.sv.row) : zero);
+        }
+        if constexpr (L == 16) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) e8[i] += __shfl_xor_sync(kAll, e8[i], 8);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          e4[i] = (dp_lane ? e8[i + 4] : e8[i]) + __shfl_xor_sync(kAll, dp_lane ? e8[i] : e8[i + 4], 4);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          e2[i] = (high2 ? e4[i + 2] : e4[i]) + __shfl_xor_sync(kAll, high2 ? e4[i] : e4[i + 2], 2);
+        const float mine = (high1 ? e2[1] : e2[0]) + __shfl_xor_sync(kAll, high1 ? e2[0] : e2[1], 1);
+        const float other = __shfl_xor_sync(kAll, mine, 4);
+        const float pr =
+            j + (sub & 3) < (int)keys ? exp2f(fmaf(dp_lane ? other : mine, p.scale2, -l)) : 0.f;
+        sum += pr, delta = fmaf(pr, dp_lane ? mine : other, delta);
       }
 #pragma unroll
-      for (int m = L / 2; m > 0; m >>= 1) {
-        s += __shfl_xor_sync(0xffffffffu, s, m);
-        dp += __shfl_xor_sync(0xffffffffu, dp, m);
+      for (int m = 2; m > 0; m >>= 1) {
+        sum += __shfl_xor_sync(kAll, sum, m);
+        delta += __shfl_xor_sync(kAll, delta, m);
       }
-      const float e = exp2f(fmaf(s, p.scale2, -l));
-      sum += e, delta = fmaf(e, dp, delta);
     }
     // sum is 1 up to the log-sum-exp's rounding, which must not part delta from dP
     if (sub == 0) put_stat(q, tile, r, row < len ? shift - l : -INFINITY, row < len && keys > 0 ? -delta / sum : 0.f);
   }
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(256, kStatCtas)
+// FEW: some sequence may have that few keys.
+template <typename T, int D, bool FEW>
+__global__ void __launch_bounds__(256, FEW ? kFewCtas : kStatCtas)
     stat_kernel(const __grid_constant__ Params p, const __grid_constant__ StatParams q) {
   constexpr bool kHalf = std::is_same<T, __half>::value;
   constexpr int L = D == 64 ? 8 : 16;  // lanes of a row, 8 channels each (96: 12 of 16 work)
@@ -810,9 +833,9 @@ __global__ void __launch_bounds__(256, kStatCtas)
     if (t < 0 || (int64_t)t * kRows >= len) return;
     const T* o = static_cast<const T*>(q.o) + batch * q.so.batch + (int64_t)h * q.so.head + sub * 8;
     const T* d = static_cast<const T*>(q.d_o) + batch * q.sdo.batch + (int64_t)h * q.sdo.head + sub * 8;
-    int64_t k_start, keys;
-    seq_range(p.cu_k, b, p.nk, k_start, keys);
-    if (keys <= kFewKeys) {
+    int64_t k_start, keys = p.nk;
+    if (FEW) seq_range(p.cu_k, b, p.nk, k_start, keys);
+    if (FEW && keys <= kFewKeys) {
       few_keys<T, D>(p, q, t, h, b, tile, big);
     } else {
 #pragma unroll 4
@@ -1046,7 +1069,10 @@ static int launch(const hi3d_attn_bwd_args* a, const Plan& n, uint8_t* ws, cudaS
     cudaError_t e = cudaMemsetAsync(ws, 0, 8, st);
     if (e != cudaSuccess) return set_error(HI3D_ERR_CUDA, "flash_attn_bwd: %s", cudaGetErrorString(e));
   }
-  stat_kernel<T, D><<<(unsigned)blocks, 256, 0, st>>>(p, q);
+  if (a->cu_seqlens_k || a->nk <= kFewKeys)
+    stat_kernel<T, D, true><<<(unsigned)blocks, 256, 0, st>>>(p, q);
+  else
+    stat_kernel<T, D, false><<<(unsigned)blocks, 256, 0, st>>>(p, q);
   if ((rc = check_launch("flash_attn_bwd statistics"))) return rc;
 
   auto kern = bwd_kernel<T, D>;

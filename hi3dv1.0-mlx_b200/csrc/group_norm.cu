@@ -330,12 +330,12 @@ __global__ void __launch_bounds__(kThreads) sums_kernel(const T* __restrict__ x,
   for (int e = threadIdx.x; e < s.cols * V; e += kThreads) {
     const int c = blockIdx.y * s.cols * V + e;
     if (c >= s.channels) break;
-    float2 t = make_float2(0.f, 0.f);
+    double tx = 0, ty = 0;  // few channels leave up to 256 lanes to one long sum
     for (int l = 0; l < lanes; ++l) {
       const float2 o = sh[l * s.cols * V + e];
-      t.x += o.x, t.y += o.y;
+      tx += o.x, ty += o.y;
     }
-    part[(int64_t)blockIdx.x * s.channels + c] = t;
+    part[(int64_t)blockIdx.x * s.channels + c] = make_float2((float)tx, (float)ty);
   }
 }
 
@@ -392,12 +392,12 @@ __device__ __forceinline__ float2 column_sum(const float2* p, int64_t stride, in
   }
   red[threadIdx.y][threadIdx.x] = a;
   __syncthreads();
-  float2 t = make_float2(0.f, 0.f);
+  double x = 0, y = 0;
   if (threadIdx.y == 0) {
 #pragma unroll
-    for (int y = 0; y < 32; ++y) t.x += red[y][threadIdx.x].x, t.y += red[y][threadIdx.x].y;
+    for (int l = 0; l < 32; ++l) x += red[l][threadIdx.x].x, y += red[l][threadIdx.x].y;
   }
-  return t;
+  return make_float2((float)x, (float)y);
 }
 
 // Backward: sums of each sample and channel over the sample's chunks; dw and db of a single sample.
