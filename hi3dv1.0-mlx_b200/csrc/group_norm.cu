@@ -276,17 +276,22 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const T* __restrict__ x
   for (int e = threadIdx.x; e < s.cols * V; e += kThreads) {
     const int c = blockIdx.y * s.cols * V + e;
     if (c >= s.channels) break;
-    float mean = 0.f, dev = 0.f, have = 0.f;
+    // the lanes' means about the first one's; few channels leave up to 256 lanes to one sum
+    const float first = sh[e].x;
+    double sum = 0, square = 0, dev = 0;
+    int have = 0;
     for (int l = 0; l < lanes; ++l) {
-      const float m = (float)count[l];
-      if (m == 0.f) break;
+      const int m = count[l];
+      if (m == 0) break;
       const float2 o = sh[l * s.cols * V + e];
-      const float d = o.x - mean, f = m / (have + m);
-      mean = fmaf(d, f, mean);
-      dev += o.y + d * d * have * f;
+      const double d = (double)o.x - first;
+      sum = fma(d, m, sum), square = fma(d * d, m, square), dev += o.y;
       have += m;
     }
-    part[(int64_t)blockIdx.x * s.channels + c] = make_float2(mean, dev);
+    const double mean = have ? sum / have : 0, between = fma(-sum, mean, square);
+    part[(int64_t)blockIdx.x * s.channels + c] =
+        have ? make_float2((float)(first + mean), (float)(dev + (between < 0 ? 0 : between)))  // a NaN stays one
+             : make_float2(0.f, 0.f);
   }
 }
 
