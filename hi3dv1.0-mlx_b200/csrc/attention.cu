@@ -10,8 +10,8 @@
 // CTA layout (352 threads):
 //   warp 0      TMA producer (one lane): Q tiles once, then K/V blocks into
 //               an NST-stage ring
-//   warp 1      MMA issuer of query tile 0 (one lane); owns the TMEM allocation
-//   warp 10     MMA issuer of query tile 1 (one lane)
+//   warp 1      MMA issuer of query tile 0 (an elected lane); owns the TMEM allocation
+//   warp 10     MMA issuer of query tile 1 (an elected lane)
 //   warps 2-5   softmax + O correction + epilogue of query tile 0
 //   warps 6-9   the same for query tile 1
 // A warp reaches TMEM lanes 32*(warp % 4) .. +31, so each group of four
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (__shfl_sync(0xffffffffu, tail_issued, 0)) {  // the last copy: cleared by the warp, then published
         uint8_t* v = sV + (tail_block % C::NST) * C::KV_STAGE;
         volatile int no_abort = 0;
-        mbar_wait(&bar->v_tail, 0, &no_abort, 4);
+        warp_wait(&bar->v_tail, 0, &no_abort, 4);
         for (int c = 0; c < C::NCH; ++c)
           for (int e = tail_rows * 8 + lane; e < C::BK * 8; e += 32)
             *reinterpret_cast<uint4*>(v + c * C::KV_CHUNK + e * 16) = make_uint4(0, 0, 0, 0);
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_commit(&bar->s_full[i]);
       };
       const int i = warp == 1 ? 0 : 1;
-      bool ok = mbar_wait(&bar->q_full, 0, abort, 10) && mbar_wait(&bar->k_full[0], 0, abort, 11);
+      bool ok = warp_wait(&bar->q_full, 0, abort, 10) && warp_wait(&bar->k_full[0], 0, abort, 11);
       if (ok) {
         tc_fence_after();
         issue_s(i, 0);
@@ -362,13 +362,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int s = j % C::NST, n = j / C::NST;
         const int s1 = (j + 1) % C::NST, n1 = (j + 1) / C::NST;
         if (j + 1 < nblk) {
-          if (!(ok = mbar_wait(&bar->k_full[s1], n1 & 1, abort, 11))) break;
-          if (!(ok = mbar_wait(&bar->s_free[i], j & 1, abort, 15))) break;
+          if (!(ok = warp_wait(&bar->k_full[s1], n1 & 1, abort, 11))) break;
+          if (!(ok = warp_wait(&bar->s_free[i], j & 1, abort, 15))) break;
           tc_fence_after();
           issue_s(i, s1);
         }
-        if (!(ok = mbar_wait(&bar->v_full[s], n & 1, abort, 13))) break;
-        if (!(ok = mbar_wait(&bar->p_full[i], j & 1, abort, 14))) break;
+        if (!(ok = warp_wait(&bar->v_full[s], n & 1, abort, 13))) break;
+        if (!(ok = warp_wait(&bar->p_full[i], j & 1, abort, 14))) break;
         tc_fence_after();
         const uint64_t dVs = dV + (uint64_t)((s * C::KV_STAGE) >> 4);
         const uint32_t dO = tm + 256 * i + C::O_COL, aP = tm + 256 * i + C::P_COL;
@@ -396,9 +396,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float scale2 = p.scale2;
     const uint64_t scale2x2 = f2_pack(scale2, scale2);
     float m_run = -INFINITY, l_run = 0.f;
-    bool ok = true;
     for (int j = 0; j < nblk; ++j) {
-      if (!(ok = mbar_wait(&bar->s_full[i], j & 1, abort, 20))) break;
+      mbar_wait(&bar->s_full[i], j & 1, abort, 20);
       tc_fence_after();
       uint32_t sv[C::BK];
 #pragma unroll
@@ -465,12 +464,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         // P of block j overwrites P of block j-1: wait until P V of block
         // j-1 has completed (which also makes O final for the correction).
         if (c == 0 && j > 0) {
-          if (!(ok = mbar_wait(&bar->o_done[i], (j - 1) & 1, abort, 21))) break;
+          mbar_wait(&bar->o_done[i], (j - 1) & 1, abort, 21);
           tc_fence_after();
         }
         tmem_st16(tP + c * 16, pk);
       }
-      if (!ok) break;
       // O *= alpha, only when a row of this warp moved its maximum
       if (j > 0 && warp_grow) {
 #pragma unroll
@@ -494,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       l_run = l_run * alpha + ((a0 + a1) + (a2 + a3));
     }
     // ---- epilogue: O / l -> out[row, h*D + d]
-    if (ok && mbar_wait(&bar->o_done[i], (nblk - 1) & 1, abort, 22)) {
+    if (!__any_sync(0xffffffffu, *abort) && warp_wait(&bar->o_done[i], (nblk - 1) & 1, abort, 22)) {
       tc_fence_after();
       const int64_t qrow = q_row0 + i * kRowsPerTile + row;
       const float inv = 1.0f / l_run;

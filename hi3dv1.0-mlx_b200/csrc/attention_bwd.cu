@@ -371,7 +371,7 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
     int issued = 0, tails = 0;
     for (int j = 0; j < n; ++j, it.next()) {
       const int s = j % NST;
-      if (!mbar_wait(&bar->empty[s], ((j / NST) & 1) ^ 1, abort, 301)) break;
+      if (!warp_wait(&bar->empty[s], ((j / NST) & 1) ^ 1, abort, 301)) break;
       uint8_t* y = sY + s * C::STAGE;
       const int valid = it.valid();
       // Rows past a packed sequence's end are the next sequence's: they are cleared, since a
@@ -388,7 +388,7 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
       }
       if (clear) {
         volatile int no_abort = 0;
-        mbar_wait(&bar->tail, tails & 1, &no_abort, 302);
+        warp_wait(&bar->tail, tails & 1, &no_abort, 302);
         ++tails;
         for (int c = 0; c < 2 * C::NCH; ++c)
           for (int e = valid * 8 + lane; e < BN * 8; e += 32)
@@ -399,12 +399,12 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
       }
       issued = j + 1;
     }
-    if (*abort) {
+    if (__any_sync(0xffffffffu, *abort)) {
       // let every copy already issued land before the CTA exits
       volatile int no_abort = 0;
-      mbar_wait(&bar->x_full, 0, &no_abort, 303);
+      warp_wait(&bar->x_full, 0, &no_abort, 303);
       for (int j = issued > NST ? issued - NST : 0; j < issued; ++j)
-        mbar_wait(&bar->full[j % NST], (j / NST) & 1, &no_abort, 304);
+        warp_wait(&bar->full[j % NST], (j / NST) & 1, &no_abort, 304);
     }
   } else if (warp < 4) {
     // ------------------------------------------------------------ MMA issuers
@@ -422,7 +422,8 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
       const uint64_t dYt = smem_desc(smem_u32(sY), C::Y_CHUNK, 1024, kLayoutSW128);  // rows as the K dimension
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       // d = x y^T over the channels, x in TMEM (x_col) or in shared memory
-      auto product = [&](auto in_tmem, uint32_t d, uint64_t x, uint32_t x_col, uint32_t y_off, uint64_t* done) {
+      auto product = [&](auto in_tmem, uint32_t d, uint64_t x, uint32_t x_col, uint32_t y_off,
+                         uint64_t* done) {
         if (!elect_one()) return;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
@@ -445,21 +446,21 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
           mma_f16_ts(d, a + group * HC + k * 8, dYt + ((y_off + ks * 2048) >> 4), idesc_acc, more || ks > 0 ? 1u : 0u);
         }
       };
-      bool ok = role_id == 2 || mbar_wait(C::X2_TMEM ? &bar->x_tmem : &bar->x_full, 0, abort, 310);
-      if (C::X2_TMEM && !C::X1_TMEM && ok && role_id == 0) ok = mbar_wait(&bar->x_full, 0, abort, 310);
+      bool ok = role_id == 2 || warp_wait(C::X2_TMEM ? &bar->x_tmem : &bar->x_full, 0, abort, 310);
+      if (C::X2_TMEM && !C::X1_TMEM && ok && role_id == 0) ok = warp_wait(&bar->x_full, 0, abort, 310);
       for (int j = 0; ok && j < n; ++j) {
         const uint32_t y = (j % NST) * C::STAGE;
-        if (!(ok = mbar_wait(&bar->full[j % NST], (j / NST) & 1, abort, 311))) break;
+        if (!(ok = warp_wait(&bar->full[j % NST], (j / NST) & 1, abort, 311))) break;
         if (role_id == 0) {  // S(j), once the products that read P(j - 2), dS(j - 2) from this buffer are done
-          if (j > 1 && !(ok = mbar_wait(&bar->acc_done[j & 1], ((j - 2) >> 1) & 1, abort, 314))) break;
+          if (j > 1 && !(ok = warp_wait(&bar->acc_done[j & 1], ((j - 2) >> 1) & 1, abort, 314))) break;
           tc_fence_after();
           product(X1InTmem(), tm + (j & 1) * BN, dX1, x1_col, y, &bar->s_full[j & 1]);
         } else if (role_id == 1) {  // T(j), once T(j - 1) has been read
-          if (j > 0 && !(ok = mbar_wait(&bar->t_free, (j - 1) & 1, abort, 312))) break;
+          if (j > 0 && !(ok = warp_wait(&bar->t_free, (j - 1) & 1, abort, 312))) break;
           tc_fence_after();
           product(X2InTmem(), tm + C::T_COL, dX2, x2_col, y + C::Y_BYTES, &bar->t_full);
         } else {  // the accumulators, once P(j), dS(j) are written
-          if (!(ok = mbar_wait(&bar->pd_full[j & 1], (j >> 1) & 1, abort, 313))) break;
+          if (!(ok = warp_wait(&bar->pd_full[j & 1], (j >> 1) & 1, abort, 313))) break;
           tc_fence_after();
           const uint32_t a = tm + (j & 1) * BN;
           if (elect_one()) {
@@ -499,14 +500,14 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
     const int col0 = KV ? 2 * (lane & 3) : 0;
     auto column = [&](int e) { return col0 + (KV ? 8 * ((e >> 1) & 3) : 2 * e); };
     // One block; MASK: only its first `valid` rows are the sequence's.
-    auto block = [&](int j, int valid, auto mask) -> bool {
+    auto block = [&](int j, int valid, auto mask) {
       constexpr bool MASK = decltype(mask)::value;
       const uint32_t tS = tmem + lane_addr + (j & 1) * BN + group * HC;
       const float4* st = reinterpret_cast<const float4*>(sStat + (j % NST) * BN * 8) + group * (HC / 2) + (lane & 3);
       float4 q[4];
       uint32_t sv[SUB][32], pk[16];
-      if (KV && !mbar_wait(&bar->full[j % NST], (j / NST) & 1, abort, 320)) return false;
-      if (!mbar_wait(&bar->s_full[j & 1], (j >> 1) & 1, abort, 321)) return false;
+      if (KV) mbar_wait(&bar->full[j % NST], (j / NST) & 1, abort, 320);
+      mbar_wait(&bar->s_full[j & 1], (j >> 1) & 1, abort, 321);
       tc_fence_after();
 #pragma unroll
       for (int u = 0; u < SUB; ++u) load_block<KV>(tS + u * 32, sv[u]);
@@ -541,7 +542,7 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
         }
         if constexpr (KV) store_block<KV>(tS + u * 16, pk);
       }
-      if (!mbar_wait(&bar->t_full, j & 1, abort, 322)) return false;
+      mbar_wait(&bar->t_full, j & 1, abort, 322);
       tc_fence_after();
 #pragma unroll
       for (int u = 0; u < SUB; ++u) {
@@ -577,12 +578,10 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar->pd_full[j & 1]);
-      return true;
     };
-    bool ok = true;
     if constexpr (C::X2_TMEM) {
       // this warp's rows of the stationary operands, the column groups one chunk of 64 channels each
-      if ((ok = mbar_wait(&bar->x_full, 0, abort, 324))) {
+      if (warp_wait(&bar->x_full, 0, abort, 324)) {
 #pragma unroll
         for (int x = 0; x < (C::X1_TMEM ? 2 : 1); ++x)
           for (int c = group; c < C::NCH; c += kGroups) {
@@ -605,15 +604,19 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
         if (lane == 0) mbar_arrive(&bar->x_tmem);
       }
     }
-    for (int j = 0; ok && j < n;) {
+    for (int j = 0; j < n;) {
       // the blocks of one sequence and head; its last may be ragged
       const int m = min(n - j, it.nblk - it.blk), whole = (int)(it.len / BN) - it.blk;
-      for (int i = 0; ok && i < m; ++i, ++j)
-        ok = i < whole ? block(j, BN, std::false_type()) : block(j, it.tail(), std::true_type());
+      for (int i = 0; i < m; ++i, ++j) {
+        if (i < whole)
+          block(j, BN, std::false_type());
+        else
+          block(j, it.tail(), std::true_type());
+      }
       it.skip(m);
     }
     // ---- epilogue: the groups alternate, W channels at a time
-    if (ok && mbar_wait(&bar->acc_done[(n - 1) & 1], ((n - 1) >> 1) & 1, abort, 323)) {
+    if (!__any_sync(0xffffffffu, *abort) && warp_wait(&bar->acc_done[(n - 1) & 1], ((n - 1) >> 1) & 1, abort, 323)) {
       tc_fence_after();
       const int64_t r = row0 + row;
       const float mul = p.scale * ldexpf(1.0f, -kexp);

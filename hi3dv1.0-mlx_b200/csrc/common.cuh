@@ -139,6 +139,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 static __device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort, int where,
                                                    uint64_t limit_ns = kWaitNs) {
   uint64_t t0 = 0;
+  if (*abort) return false;
   for (uint32_t i = 0; i < kSpinLimit; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((i & 255u) == 255u) {
@@ -158,6 +159,19 @@ static __device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parit
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int where) {
   if (mbar_try_wait(bar, parity)) return true;
   return mbar_wait_slow(bar, parity, abort, where);
+}
+
+// A wait may be given up by some lanes of a warp just as its phase completes for the others, and lanes
+// that left while the rest went on to a warp-wide instruction (elect, a shuffle, a TMEM access) would
+// leave those waiting for good.  So no lane leaves by its own result.  warp_wait gives the whole warp
+// one, by a vote.  Compute warps, where a vote on every wait costs 3-6 % of an attention kernel, call
+// mbar_wait for the wait alone and run their loop to its end (once a wait ran out, the others return at
+// once); after it the warp looks at `abort`, which every wait that ran out has set.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int where) {
+  bool ok = mbar_try_wait(bar, parity);
+  if (__all_sync(0xffffffffu, ok)) return true;
+  if (!ok) ok = mbar_wait_slow(bar, parity, abort, where);
+  return __all_sync(0xffffffffu, ok);
 }
 
 // ---------------------------------------------------------------------------

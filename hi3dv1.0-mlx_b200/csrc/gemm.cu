@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < 4; ++c) prefetch_residual<OutT>(p, res[c], m0, nh + c * 32, lane);
       }
       __syncwarp();
-      if (!mbar_wait(&bar->acc_full[acc], use & 1, abort, 120)) break;
+      if (!warp_wait(&bar->acc_full[acc], use & 1, abort, 120)) break;
       tc_fence_after();
       const int mr = m0 + lane;  // phase-1 row
       float sa = 1.0f;

@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(CV_THREADS, 1)
     int local = 0;
     for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++local) {
       const int acc = local & 1, use = local >> 1;
-      if (!mbar_wait(&bar->acc_full[acc], use & 1, abort, 220)) break;
+      if (!warp_wait(&bar->acc_full[acc], use & 1, abort, 220)) break;
       tc_fence_after();
       const int mt = tile / p.tiles_n, nt = tile % p.tiles_n;
       const bool any_tap = p.tap_mask[mt] != 0;

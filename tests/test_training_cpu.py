@@ -3,9 +3,11 @@
 from __future__ import annotations
 
 import ctypes
+import re
 
 import pytest
 import torch
+from conftest import REPO
 
 from hi3d_b200 import _lib, attention, optim, vae
 
@@ -109,3 +111,41 @@ def test_no_cpu_path():
         vae.group_norm_act(torch.zeros(4, 8), torch.ones(8), torch.zeros(8), 2)
     with pytest.raises(ValueError):
         optim.adamw_step([torch.zeros(4)], [torch.zeros(4)], torch.zeros(256), torch.zeros(256), step=1, lr=1e-3)
+
+
+def _statements(src: str, word: str):
+    """For each call of `word` in C++ source without comments: its statement, and what opened the blocks
+    around it."""
+    opened, begin = [], 0
+    for i, ch in enumerate(src):
+        if ch in "{};":
+            if ch == "{":
+                opened.append(src[begin:i])
+            elif ch == "}" and opened:
+                opened.pop()
+            begin = i + 1
+        elif src.startswith(word, i) and not (src[i - 1].isalnum() or src[i - 1] == "_"):
+            yield src[begin:src.index(";", i)], list(opened)
+
+
+@pytest.mark.parametrize("name", ["attention.cu", "attention_bwd.cu"])
+def test_a_whole_warp_leaves_a_wait_together(name):
+    """A bounded wait may be given up by some lanes and met by others.  Outside blocks that one lane
+    runs, a lane's own result of a wait is not used, neither to leave a loop nor to issue: a vote gives
+    the warp one result, or the warp looks at the abort flag after its loop."""
+    src = re.sub(r"//[^\n]*", "", (REPO / "hi3dv1.0-mlx_b200" / "csrc" / name).read_text())
+    own = [s for s, around in _statements(src, "mbar_wait(") if not any("lane == 0" in b for b in around)]
+    for s in own:
+        assert re.match(r"\s*(if \(KV\) )?mbar_wait\([^;]*\)$", s), s
+    assert own and "if (!__any_sync(0xffffffffu, *abort) && warp_wait(" in src
+    assert len(list(_statements(src, "warp_wait("))) >= 7
+    head = (REPO / "hi3dv1.0-mlx_b200" / "csrc" / "common.cuh").read_text()
+    body = head[head.index("bool warp_wait("):]
+    assert re.search(r"return __all_sync\(0xffffffffu, ok\);", body[:body.index("\n}")])
+
+
+@pytest.mark.parametrize("name", ["gemm.cu", "sparse.cu"])
+def test_epilogue_warps_leave_a_wait_together(name):
+    src = (REPO / "hi3dv1.0-mlx_b200" / "csrc" / name).read_text()
+    waits = re.findall(r"(mbar_wait|warp_wait)\(&bar->acc_full", src)
+    assert waits and set(waits) == {"warp_wait"}
