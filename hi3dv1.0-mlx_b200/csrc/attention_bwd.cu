@@ -876,7 +876,8 @@ __global__ void __launch_bounds__(256, FEW ? kFewCtas : kStatCtas)
 }
 
 // Sums the fp32 partials of the splits in order and rounds them: out[batch][row][head][D].  8 bytes
-// of partials a split and value of dK, dV: two splits of 2049 x 4 x 128, 5.5 us.
+// of partials a split and value of dK, dV: two splits of 2049 x 4 x 128, 5.5 us.  Rows before the first
+// packed sequence and after the last have no partials and are left alone.
 struct ReduceJob {
   const float* part;
   void* out;
@@ -885,6 +886,8 @@ struct ReduceJob {
   int heads, batches, splits;
   int64_t split_stride;  // floats between two splits
   int64_t items;         // batches * heads * rows * D / 8
+  const int32_t* cu;     // packed rows: [num_seqs + 1] offsets
+  int num_seqs;
 };
 
 template <typename T, int D>
@@ -894,16 +897,17 @@ __global__ void __launch_bounds__(256) reduce_kernel(const ReduceJob j0, const R
   if (i >= j->items) i -= j->items, j = &j1;
   if (j == &j1 && i >= j->items) i -= j->items, j = &j2;
   if (i >= j->items) return;
+  const int d = (int)(i % (D / 8)) * 8;
+  int64_t rest = i / (D / 8);
+  const int64_t row = rest % j->rows;
+  rest /= j->rows;
+  if (j->cu && (row < j->cu[0] || row >= j->cu[j->num_seqs])) return;
   const float* src = j->part + i * 8;
   float a[8] = {};
   for (int s = 0; s < j->splits; ++s, src += j->split_stride) {
     const float4 x = *reinterpret_cast<const float4*>(src), y = *reinterpret_cast<const float4*>(src + 4);
     a[0] += x.x, a[1] += x.y, a[2] += x.z, a[3] += x.w, a[4] += y.x, a[5] += y.y, a[6] += y.z, a[7] += y.w;
   }
-  const int d = (int)(i % (D / 8)) * 8;
-  int64_t rest = i / (D / 8);
-  const int64_t row = rest % j->rows;
-  rest /= j->rows;
   T* dst = static_cast<T*>(j->out) + rest / j->heads * j->s.batch + row * j->s.row + rest % j->heads * j->s.head + d;
   uint4 o;
   o.x = Cvt<T>::pack2(a[0], a[1]);
@@ -1088,9 +1092,10 @@ static int launch(const hi3d_attn_bwd_args* a, const Plan& n, uint8_t* ws, cudaS
   if (n.kv_splits > 1)
     for (int w = 0; w < 2; ++w)
       jobs[w] = {p.part_kv + w * n.kv_part, w == 0 ? a->dk : a->dv, w == 0 ? p.sdk : p.sdv, a->nk, a->kv_heads,
-                 n.kv_batches, n.kv_splits, 2 * n.kv_part, n.kv_part / 8};
+                 n.kv_batches, n.kv_splits, 2 * n.kv_part, n.kv_part / 8, a->cu_seqlens_k, a->num_seqs};
   if (n.q_splits > 1)
-    jobs[2] = {p.part_q, a->dq, p.sdq, a->nq, a->heads, n.q_batches, n.q_splits, n.q_part, n.q_part / 8};
+    jobs[2] = {p.part_q,   a->dq,    p.sdq,           a->nq,          a->heads,   n.q_batches,
+               n.q_splits, n.q_part, n.q_part / 8, a->cu_seqlens_q, a->num_seqs};
   const int64_t items = jobs[0].items + jobs[1].items + jobs[2].items;
   if (items == 0) return HI3D_OK;
   reduce_kernel<T, D><<<(unsigned)((items + 255) / 256), 256, 0, st>>>(jobs[0], jobs[1], jobs[2]);

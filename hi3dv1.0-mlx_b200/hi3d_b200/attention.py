@@ -593,7 +593,7 @@ def flash_attn_varlen_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch
                                grads: tuple | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``(dq, dk, dv)`` of :func:`flash_attn_varlen_lse` in the shapes of ``q, k, v``, as
     :func:`flash_attention_backward`; with ``cu_seqlens_k=None`` ``dk, dv`` sum over all sequences.
-    No longest length is needed.  The offsets must cover all rows."""
+    No longest length is needed.  Gradient rows outside the offsets are not written."""
     p, q, k, v = _planned("packed", q, k, v)
     cu_q, cu_k = _offsets(cu_seqlens_q, cu_seqlens_k, q)
     return _backward(p, grad_out, q, k, v, out, lse, cu_q, cu_k, cu_q.numel() - 1, _scale(scale), grads)

@@ -170,8 +170,8 @@ HI3D_API int hi3d_flash_attn_fwd_lse(const hi3d_attn_args* args, int kv_heads, f
  * cu_seqlens_k == NULL), over all sequences.  P and dS are rounded to the I/O type for the products,
  * which accumulate in fp32; each gradient is rounded once.  No atomics on sums: the same bits on
  * every run.  Layout rules as hi3d_attn_args (strides in elements, multiples of 8; pointers 16-byte
- * aligned); cu_seqlens are read on the device and cut to the rows that exist, no longest length is
- * needed.  Rows outside every sequence are not written.  All sizes >= 1. */
+ * aligned); cu_seqlens (ascending) are read on the device and cut to the rows that exist, no longest
+ * length is needed.  Rows before the first offset and after the last are not written.  All sizes >= 1. */
 typedef struct hi3d_attn_bwd_args {
   const void* q;
   const void* k;

@@ -405,3 +405,35 @@ def test_refusals():
         attention.flash_attn_varlen_lse(t, t, t, cu.float(), cu, 8, 0.1)
     with pytest.raises(ValueError):
         attention.flash_attn_varlen_lse(t, t, t, cu, cu, 0, 0.1)
+
+
+def _poison(nbytes):
+    """Leaves NaN bits in the block of memory that the next workspace of this size is given."""
+    torch.full((nbytes,), 0xFF, dtype=torch.uint8, device=DEV)
+
+
+# 2 heads over many queries and few keys split the key stream, 2 queries' tiles over many keys the query
+# stream; the last is whole.  Rows before the first, after the last offset belong to no sequence.
+UNCOVERED = [([5, 3000, 6000], 6100, [3, 77, 150], 256), ([2, 3, 5], 9, [0, 100, 9000], 9100),
+             ([5, 100, 190], 200, [3, 77, 150], 256)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("cu_q,tq,cu_k,tk", UNCOVERED)
+def test_gradient_rows_of_no_sequence_are_not_written(dtype, cu_q, tq, cu_k, tk):
+    q, do = _rand((tq, 2, 64), dtype, 81), _rand((tq, 2, 64), dtype, 82)
+    k, v = _rand((tk, 2, 64), dtype, 83), _rand((tk, 2, 64), dtype, 84)
+    cq, ck = (torch.tensor(c, dtype=torch.int32, device=DEV) for c in (cu_q, cu_k))
+    out, lse = attention.flash_attn_varlen_lse(q, k, v, cq, ck, max(b - a for a, b in zip(cu_q, cu_q[1:])), 0.125)
+    grads = tuple(torch.full_like(t, 7.0) for t in (q, k, v))
+    p = attention._planned("packed", q, k, v)[0]
+    steps = (128, 64, 0) * 2
+    _poison(attention._backward_plan(p, q.shape, k.shape, steps, True, len(cu_q) - 1, 0.125, 0)[2])
+    dq, dk, dv = attention.flash_attn_varlen_backward(do, q, k, v, out, lse, cq, ck, 0.125, grads=grads)
+    for t, cu in ((dq, cu_q), (dk, cu_k), (dv, cu_k)):
+        assert (t[:cu[0]] == 7).all() and (t[cu[-1]:] == 7).all()
+    rows = lambda t, cu: t[cu[0]:cu[-1]]  # noqa: E731
+    zero = lambda cu: [c - cu[0] for c in cu]  # noqa: E731
+    want = packed_exact(rows(q, cu_q), rows(k, cu_k), rows(v, cu_k), rows(do, cu_q), zero(cu_q), zero(cu_k), 0.125)
+    for name, got, e in (("dq", rows(dq, cu_q), want[2]), ("dk", rows(dk, cu_k), want[3]), ("dv", rows(dv, cu_k), want[4])):
+        check(name, got, e, dtype)
