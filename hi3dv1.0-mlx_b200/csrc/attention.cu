@@ -610,12 +610,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 // out = sum_s 2^(lse_s - max) O_s / sum_s 2^(lse_s - max), rounded once.  Rows
 // whose splits all saw no keys are left untouched, as in the single-pass kernel.
 // LSE: those rows get 0 and -inf instead, and every row its natural log-sum-exp, at
-// lse[batch][head][row] with nq rows per head.
+// lse[batch][head][row] with nq rows per head.  Packed rows before the first sequence and after the
+// last have no partials: they are left untouched in both forms.
 template <typename T, int D, bool LSE = false>
 __global__ void __launch_bounds__(256) merge_kernel(const float* __restrict__ part_o,
                                                     const float* __restrict__ part_lse, T* __restrict__ out,
                                                     int64_t rows, int heads, int splits, int64_t nq, int dense,
                                                     int64_t o_row, int64_t o_head, int64_t o_batch,
+                                                    const int32_t* __restrict__ cu, int num_seqs,
                                                     float* __restrict__ lse = nullptr) {
   constexpr int E = D / 32;  // elements per lane
   const int64_t wid = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
@@ -623,6 +625,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const float* __restrict__ pa
   if (wid >= rows * heads) return;
   const int64_t r = wid / heads;
   const int h = (int)(wid - r * heads);
+  if (cu && (r < cu[0] || r >= cu[num_seqs])) return;
   float mx = -INFINITY;
   for (int s = 0; s < splits; ++s) mx = fmaxf(mx, part_lse[((int64_t)s * rows + r) * heads + h]);
   if (mx == -INFINITY && !LSE) return;
@@ -726,7 +729,7 @@ static int launch_merge(const hi3d_attn_args* a, cudaStream_t st, int num_slots,
   if (warps == 0) return HI3D_OK;
   attn::merge_kernel<T, D, LSE><<<(unsigned)((warps + 7) / 8), 256, 0, st>>>(
       part_o, part_lse, static_cast<T*>(a->out), rows, a->heads, num_slots, a->nq, varlen_q ? 0 : 1, a->o_row,
-      a->o_head, a->o_batch, lse);
+      a->o_head, a->o_batch, a->cu_seqlens_q, a->num_seqs, lse);
   return check_launch("flash_attn_merge");
 }
 

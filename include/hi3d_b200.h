@@ -157,8 +157,8 @@ HI3D_API int hi3d_flash_attn_fwd_split(const hi3d_attn_args* args, int k_splits,
 
 /* hi3d_flash_attn_fwd_split for training: also writes lse = ln sum_k exp(scale q k^T) (fp32,
  * [num_seqs][heads][nq], packed: [heads][nq]).  kv_heads divides heads: query head h reads key head
- * h / (heads / kv_heads).  Rows without keys get out = 0 and lse = -inf.  k_splits == 1 needs no
- * workspace.  nk >= 1.  The reference has no backward pass; its attention is
+ * h / (heads / kv_heads).  Rows without keys get out = 0 and lse = -inf; packed rows before the first
+ * offset and after the last are not written.  k_splits == 1 needs no workspace.  nk >= 1.  The reference has no backward pass; its attention is
  * src/hi3d_mac/mlx_backend/attention.py:238-277. */
 HI3D_API int hi3d_flash_attn_fwd_lse(const hi3d_attn_args* args, int kv_heads, float* lse, int k_splits,
                                      void* workspace, int64_t workspace_bytes, void* stream);

@@ -11,6 +11,7 @@ scores of D products (D 2^-24 relative to sum |q k|), the exponential's 3e-6.
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
@@ -437,3 +438,34 @@ def test_gradient_rows_of_no_sequence_are_not_written(dtype, cu_q, tq, cu_k, tk)
     want = packed_exact(rows(q, cu_q), rows(k, cu_k), rows(v, cu_k), rows(do, cu_q), zero(cu_q), zero(cu_k), 0.125)
     for name, got, e in (("dq", rows(dq, cu_q), want[2]), ("dk", rows(dk, cu_k), want[3]), ("dv", rows(dv, cu_k), want[4])):
         check(name, got, e, dtype)
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("with_lse", [True, False])
+def test_output_rows_of_no_sequence_are_not_written(splits, with_lse):
+    """The C entry on buffers of the caller's: rows outside the offsets keep what they held, with the
+    keys in one pass or split."""
+    tq, tk, heads, cu_q, cu_k = 300, 900, 2, [5, 100, 290], [3, 400, 890]
+    dtype = torch.bfloat16
+    q, k, v = (_rand((n, heads, 64), dtype, 85 + i) for i, n in enumerate((tq, tk, tk)))
+    cq, ck = (torch.tensor(c, dtype=torch.int32, device=DEV) for c in (cu_q, cu_k))
+    out, lse = torch.full_like(q, 7.0), torch.full((heads, tq), 7.0, device=DEV)
+    args = _lib.AttnArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *(128, 64, 0) * 4, cq.data_ptr(),
+                         ck.data_ptr(), tq, tk, 190, 2, heads, 64, _lib.BF16, 0.125)
+    nbytes = ctypes.c_int64()
+    lib = _lib.load()
+    _lib.check(lib.hi3d_flash_attn_split_workspace_size(ctypes.byref(args), splits, ctypes.byref(nbytes)), "size")
+    ws = torch.full((max(1, nbytes.value),), 0x40, dtype=torch.uint8, device=DEV)  # floats of about 3
+    if with_lse:
+        rc = lib.hi3d_flash_attn_fwd_lse(ctypes.byref(args), heads, lse.data_ptr(), splits, ws.data_ptr(), nbytes.value,
+                                         _lib.stream(q))
+    else:
+        rc = lib.hi3d_flash_attn_fwd_split(ctypes.byref(args), splits, ws.data_ptr(), nbytes.value, _lib.stream(q))
+    _lib.check(rc, "forward")
+    gone = torch.ones(tq, dtype=torch.bool, device=DEV)
+    gone[5:290] = False
+    assert (out[gone] == 7).all() and (lse[:, gone] == 7).all()
+    want = packed_exact(q[5:290], k[3:890], v[3:890], q[5:290], [0, 95, 285], [0, 397, 887], 0.125)
+    check("out", out[5:290], want[0], dtype)
+    if with_lse:
+        assert torch.allclose(lse[:, 5:290].double(), want[1], rtol=1e-5, atol=2e-5)
