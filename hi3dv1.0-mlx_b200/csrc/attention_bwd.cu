@@ -71,7 +71,8 @@ struct Params {
   float* part_q;   // [split][query batch][head][query row][D]
   // per pair of query rows {-L log2e, -L log2e, -delta, -delta}, tiles of 128 rows (fp16: + kPShift)
   const float4* stat;
-  const unsigned* amax;  // fp16: largest finite |dO| and |V| (float bits)
+  // fp16: largest finite |dO| of each statistics tile, and |V| of each tile of 128 rows of a key head
+  const float *max_o, *max_v;
   float scale, scale2;
 };
 
@@ -222,11 +223,26 @@ struct Stream {
 
 // Exponent k with 2 D max|dO| max|V| 2^k < 2^15: |dS| 2^k <= |dP| + |delta| scaled stays inside
 // fp16 whatever the gradient's size, and small gradients keep their bits.
-__device__ __forceinline__ int ds_exponent(const unsigned* amax, int D) {
-  const float bound = 2.0f * D * __uint_as_float(amax[0]) * __uint_as_float(amax[1]);
+__device__ __forceinline__ int ds_exponent(float max_o, float max_v, int D) {
+  const float bound = 2.0f * D * max_o * max_v;
   if (!(bound > 0.0f)) return 0;
   const int k = 14 - ilogbf(fminf(bound, 1e30f));
   return min(max(k, -40), 40);
+}
+
+// The largest of runs * inner tile maxima, `outer` from run to run, by a whole warp.
+__device__ __forceinline__ float fold_max(const float* m, int64_t outer, int inner, int runs) {
+  float x = 0.f;
+  for (unsigned e = threadIdx.x & 31; e < (unsigned)(inner * runs); e += 32)
+    x = fmaxf(x, m[(int64_t)(e / (unsigned)inner) * outer + e % (unsigned)inner]);
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, i));
+  return x;
+}
+// [first, first + count) tiles of sequences [b0, b1) in one head's tiles
+__device__ __forceinline__ void tile_range(const int32_t* cu, int b0, int b1, int64_t rows, int& first, int& count) {
+  first = tile_start(cu, b0, rows);
+  count = max(tile_start(cu, b1, rows) - first, 0);
 }
 
 template <int N>
@@ -481,7 +497,26 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
     const uint32_t lane_addr = (uint32_t)(sub * 32) << 16;
     const uint32_t tT = tmem + lane_addr + C::T_COL + group * HC;
     const uint64_t scale2x2 = f2_splat(p.scale2);
-    const int kexp = kHalf ? ds_exponent(p.amax, D) : 0;
+    // The exponent that dS carries, from the rows that enter this CTA's sums alone: another sequence's,
+    // head's or (query CTAs) row tile's sizes do not cost these their bits.
+    int kexp = 0;
+    if constexpr (kHalf) {
+      const int hk = KV ? h : h / p.group, set = p.kv_seqs == 1 ? 0 : seq;
+      int vt = 0, nv = p.kv_tiles, qt = 0, nq = p.q_tiles;
+      if (p.cu_k) tile_range(p.cu_k, seq, seq + 1, p.nk, vt, nv);
+      const float max_v = fold_max(p.max_v + ((int64_t)(p.cu_k ? 0 : set) * p.kv_heads + hk) * p.kv_tiles + vt, 0, nv, 1);
+      float max_o;
+      if constexpr (!KV) {
+        max_o = p.max_o[stat_tile(p, seq, h) + t];
+      } else if (p.cu_q) {
+        tile_range(p.cu_q, b0, b1, p.nq, qt, nq);
+        max_o = fold_max(p.max_o + (int64_t)h * p.group * p.q_tiles + qt, p.q_tiles, nq, p.group);
+      } else {
+        max_o = fold_max(p.max_o + ((int64_t)b0 * p.heads + h * p.group) * p.q_tiles, (int64_t)p.heads * p.q_tiles,
+                         p.group * p.q_tiles, b1 - b0);
+      }
+      kexp = ds_exponent(max_o, max_v, D);
+    }
     // key CTAs keep P 2^kPShift in 16 bits: dS takes the rest of its exponent here
     const uint64_t gain = f2_splat(ldexpf(1.0f, kexp - kPShift));
     // query CTAs: this row's statistics, the exponent of dS inside the probability's
@@ -699,8 +734,8 @@ constexpr int kStatCtas = 8, kFewCtas = 5;
 // the products done again here, 16 FMAs a key and 8 channels (then 0.0024 throughout; 4096 x 16 queries,
 // the whole pass: 4 keys 45 us, 16 keys 62, 36 without).  Blocks
 // [0, stat_blocks): one (tile, head, sequence) each; rows past the sequence's end get
-// probability 0.  fp16: these blocks also take the largest finite |dO|, and the blocks after
-// them the largest finite |V| (integer maxima of the bits: order does not matter).
+// probability 0.  fp16: these blocks also take their tile's largest finite |dO|, and the blocks after
+// them the largest finite |V| of each tile of a key head (tiles as the key CTAs').
 // Reads O and dO once: 4096 x 16 x 64 bf16 7.2 us, 8192 8.4 us (4.0 TB/s; short, so its launch, the
 // first loads' latency and the tail count as much as the bytes).
 struct StatParams {
@@ -708,9 +743,8 @@ struct StatParams {
   Strides so, sdo, sq, sk, sv;
   const float* lse;
   float* stat;
-  unsigned* amax;
-  int64_t v_rows;
-  int v_tiles, v_heads, stat_blocks;
+  float *max_o, *max_v;
+  int stat_blocks;
 };
 
 template <typename T, int D>
@@ -833,7 +867,10 @@ __global__ void __launch_bounds__(256, FEW ? kFewCtas : kStatCtas)
     int64_t start, len;
     seq_range(p.cu_q, b, p.nq, start, len);
     const int batch = p.cu_q ? 0 : b;
-    if (t < 0 || (int64_t)t * kRows >= len) return;
+    if (t < 0 || (int64_t)t * kRows >= len) {
+      if (kHalf && threadIdx.x == 0) q.max_o[tile] = 0.f;
+      return;
+    }
     const T* o = static_cast<const T*>(q.o) + batch * q.so.batch + (int64_t)h * q.so.head + sub * 8;
     const T* d = static_cast<const T*>(q.d_o) + batch * q.sdo.batch + (int64_t)h * q.sdo.head + sub * 8;
     int64_t k_start, keys = p.nk;
@@ -861,17 +898,33 @@ __global__ void __launch_bounds__(256, FEW ? kFewCtas : kStatCtas)
     }
   } else {
     const int blk = blockIdx.x - q.stat_blocks;
-    const int t = blk % q.v_tiles, h = blk / q.v_tiles % q.v_heads, b = blk / q.v_tiles / q.v_heads;
+    int t = blk % p.kv_tiles;
+    const int h = blk / p.kv_tiles % p.kv_heads, b = blk / p.kv_tiles / p.kv_heads;
+    int64_t start = 0, len = p.nk;
+    if (p.cu_k) {
+      const int seq = find_seq(p.cu_k, p.num_seqs, t, p.nk);
+      t -= tile_start(p.cu_k, seq, p.nk);
+      seq_range(p.cu_k, seq, p.nk, start, len);
+    }
     const T* v = static_cast<const T*>(q.v) + (int64_t)b * q.sv.batch + (int64_t)h * q.sv.head + sub * 8;
-    for (int r = threadIdx.x / L; r < kRows; r += 256 / L) {
+    for (int r = threadIdx.x / L; t >= 0 && r < kRows; r += 256 / L) {
       const int64_t row = (int64_t)t * kRows + r;
-      if (row < q.v_rows && on) big = abs_max8<T, D>(*reinterpret_cast<const uint4*>(v + row * q.sv.row), big);
+      if (row < len && on) big = abs_max8<T, D>(*reinterpret_cast<const uint4*>(v + (start + row) * q.sv.row), big);
     }
   }
   if constexpr (kHalf) {
+    __shared__ float most[8];
     for (int m = 16; m > 0; m >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, m));
-    if ((threadIdx.x & 31) == 0 && big > 0.f)
-      atomicMax(q.amax + ((int)blockIdx.x < q.stat_blocks ? 0 : 1), __float_as_uint(big));
+    if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = big;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+      for (int w = 1; w < 8; ++w) big = fmaxf(big, most[w]);
+      if ((int)blockIdx.x < q.stat_blocks)
+        q.max_o[blockIdx.x] = big;
+      else
+        q.max_v[blockIdx.x - q.stat_blocks] = big;
+    }
   }
 }
 
@@ -927,7 +980,9 @@ struct Plan {
   // keys, 16 heads of 64, bf16: 58 us, with the key CTAs first 101.
   bool q_first;
   int kv_splits, q_splits;
-  int64_t stat_bytes, kv_part, q_part;  // floats of one split's partials
+  int64_t max_o, max_v;                 // fp16: tile maxima
+  int64_t max_bytes, stat_bytes;
+  int64_t kv_part, q_part;              // floats of one split's partials
   int64_t bytes;
 };
 
@@ -976,10 +1031,13 @@ static Plan make_plan(const hi3d_attn_bwd_args* a) {
   n.q_ctas = q_tiles * n.q_splits;
   n.q_first = kQueryCost * q_steps / n.q_splits > (double)kv_steps / n.kv_splits;
   const int64_t stat_tiles = (int64_t)n.q_tiles * a->heads * n.q_batches;
+  const bool half = a->dtype == HI3D_F16;
+  n.max_o = half ? stat_tiles : 0, n.max_v = half ? kv_tiles : 0;
+  n.max_bytes = round256((n.max_o + n.max_v) * 4);
   n.stat_bytes = round256(stat_tiles * kRows * 8);
   n.kv_part = (int64_t)n.kv_batches * a->kv_heads * a->nk * a->head_dim;
   n.q_part = (int64_t)n.q_batches * a->heads * a->nq * a->head_dim;
-  n.bytes = 256 + n.stat_bytes + (n.kv_splits > 1 ? round256(n.kv_part * 2 * n.kv_splits * 4) : 0) +
+  n.bytes = n.max_bytes + n.stat_bytes + (n.kv_splits > 1 ? round256(n.kv_part * 2 * n.kv_splits * 4) : 0) +
             (n.q_splits > 1 ? round256(n.q_part * n.q_splits * 4) : 0);
   return n;
 }
@@ -1051,9 +1109,10 @@ static int launch(const hi3d_attn_bwd_args* a, const Plan& n, uint8_t* ws, cudaS
   p.kv_ctas = (int)n.kv_ctas, p.kv_first = n.q_first ? (int)n.q_ctas : 0, p.q_first = n.q_first ? 0 : (int)n.kv_ctas;
   p.kv_splits = n.kv_splits, p.q_splits = n.q_splits;
   p.scale = a->scale, p.scale2 = a->scale * kLog2e;
-  p.amax = reinterpret_cast<const unsigned*>(ws);
-  p.stat = reinterpret_cast<const float4*>(ws + 256);
-  p.part_kv = reinterpret_cast<float*>(ws + 256 + n.stat_bytes);
+  float* const max_o = reinterpret_cast<float*>(ws);
+  p.max_o = max_o, p.max_v = max_o + n.max_o;
+  p.stat = reinterpret_cast<const float4*>(ws + n.max_bytes);
+  p.part_kv = reinterpret_cast<float*>(ws + n.max_bytes + n.stat_bytes);
   p.part_q = p.part_kv + (n.kv_splits > 1 ? round256(n.kv_part * 2 * n.kv_splits * 4) / 4 : 0);
 
   StatParams q;
@@ -1064,18 +1123,10 @@ static int launch(const hi3d_attn_bwd_args* a, const Plan& n, uint8_t* ws, cudaS
   q.sk = {a->k_row, a->k_head, a->k_batch};
   q.sv = {a->v_row, a->v_head, a->v_batch};
   q.lse = a->lse;
-  q.stat = reinterpret_cast<float*>(ws + 256);
-  q.amax = reinterpret_cast<unsigned*>(ws);
-  q.v_rows = a->nk;
-  q.v_tiles = (int)((a->nk + kRows - 1) / kRows);
-  q.v_heads = a->kv_heads;
+  q.stat = reinterpret_cast<float*>(ws + n.max_bytes);
+  q.max_o = max_o, q.max_v = max_o + n.max_o;
   q.stat_blocks = (int)((int64_t)n.q_tiles * a->heads * qb);
-  int64_t blocks = q.stat_blocks;
-  if (std::is_same<T, __half>::value) {
-    blocks += (int64_t)q.v_tiles * a->kv_heads * kb;
-    cudaError_t e = cudaMemsetAsync(ws, 0, 8, st);
-    if (e != cudaSuccess) return set_error(HI3D_ERR_CUDA, "flash_attn_bwd: %s", cudaGetErrorString(e));
-  }
+  const int64_t blocks = q.stat_blocks + n.max_v;
   if (a->cu_seqlens_k || a->nk <= kFewKeys)
     stat_kernel<T, D, true><<<(unsigned)blocks, 256, 0, st>>>(p, q);
   else

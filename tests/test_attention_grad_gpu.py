@@ -469,3 +469,59 @@ def test_output_rows_of_no_sequence_are_not_written(splits, with_lse):
     check("out", out[5:290], want[0], dtype)
     if with_lse:
         assert torch.allclose(lse[:, 5:290].double(), want[1], rtol=1e-5, atol=2e-5)
+
+
+def _each_by_its_own(got, want):
+    """Bounds relative to each gradient's own norm, plus half of fp16's smallest step."""
+    for name, a, b in zip(("dq", "dk", "dv"), got, want):
+        a, b = a.double(), b.double()
+        assert torch.isfinite(a).all(), name
+        err, tol = (a - b).norm(), 1.5 * U[torch.float16] * b.norm() + 2.0 ** -25 * math.sqrt(b.numel())
+        assert err <= tol, f"{name}: {err:.3e} > {tol:.3e} (norm {b.norm():.3e})"
+
+
+@pytest.mark.parametrize("v_mul,do_mul", [(75.0, 0.01), (6000.0, 0.1), (6000.0, 0.01)])
+@pytest.mark.parametrize("kv_heads", [2, 1])
+def test_fp16_gradients_of_a_sequence_do_not_depend_on_its_neighbours_sizes(v_mul, do_mul, kv_heads):
+    """A sequence of 2048 rows beside one with values and output gradients many times its own, and
+    beside rows that no sequence reads: its gradients keep the bits that they have alone."""
+    dtype, cu = torch.float16, [0, 2048, 2400]
+    q, do = _rand((2464, 2, 64), dtype, 91), _rand((2464, 2, 64), dtype, 92)
+    k, v = _rand((2464, kv_heads, 64), dtype, 93), _rand((2464, kv_heads, 64), dtype, 94)
+    v[2048:] *= v_mul
+    v[2400:] = 60000.0
+    do[:2048] *= do_mul
+    do[2400:] = 60000.0
+    got = packed(q, k, v, do, cu, cu, 0.125)
+    own = [t[:2048] for t in (q, k, v, do)]
+    want = packed_exact(*own, [0, 2048], [0, 2048], 0.125)
+    _each_by_its_own([t[:2048] for t in got[2:]], want[2:])
+    alone = packed(*own, [0, 2048], [0, 2048], 0.125)
+    _each_by_its_own([t[:2048] for t in got[2:]], alone[2:])
+
+
+@pytest.mark.parametrize("which", ["head", "batch"])
+def test_fp16_gradients_of_a_head_do_not_depend_on_the_others_sizes(which):
+    dtype = torch.float16
+    q, k, v, do = (_rand((2, 2, 1500, 64), dtype, 95 + i) for i in range(4))
+    big = (slice(None), 1) if which == "head" else (1,)
+    v[big] *= 6000.0
+    do *= 0.01
+    do[big] *= 400.0
+    out, lse, *got = dense(q, k, v, do, 0.125)
+    want = exact(q, k, v, do, 0.125)[2:]
+    small = (slice(None), 0) if which == "head" else (0,)
+    _each_by_its_own([t[small] for t in got], [t[small] for t in want])
+
+
+def test_fp16_query_gradients_do_not_depend_on_other_rows_sizes():
+    """One row tile whose output gradient is thousands of times the others'."""
+    q, k, v, do = (_rand((1, 2, 2000, 64), torch.float16, 99 + i) for i in range(4))
+    do *= 1e-3
+    do[:, :, 256:384] *= 1e6
+    v *= 40.0
+    out, lse, dq, *_ = dense(q, k, v, do, 0.125)
+    want = exact(q, k, v, do, 0.125)[2]
+    rest = torch.ones(2000, dtype=torch.bool, device=DEV)
+    rest[256:384] = False
+    _each_by_its_own([dq[:, :, rest]], [want[:, :, rest]])
