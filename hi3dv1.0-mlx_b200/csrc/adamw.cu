@@ -6,8 +6,10 @@
 // all in fp32.  The moments' products and sums are rounded one by one (no contraction), so the
 // 8-bit codes do not depend on how a compiler fuses; the root and the quotient of the update are
 // the MUFU unit's (2 units in the last place each, on an update that is itself a small part of p):
-// with a correctly rounded quotient the 8-bit step was bound by issue, not by HBM.  What is coded
-// is the correctly rounded root.  16-bit weights are the rounded copy of an fp32 master.
+// with a correctly rounded quotient the 8-bit step was bound by issue, not by HBM.  The MUFU root
+// takes a v below 2^-126 as 0; where eps is so small that this would show, a kernel of its own (SMALL_EPS)
+// takes the rounded root: a branch in the usual one costs it 6 %.  What is coded is the correctly
+// rounded root.  16-bit weights are the rounded copy of an fp32 master.
 //
 // The states of all tensors lie in flat buffers, each tensor beginning at a multiple of kBlock
 // elements.  8 bits: a block of kBlock values of m, and of u = sqrt(v), is stored as e4m3 codes
@@ -133,18 +135,19 @@ __device__ __forceinline__ uint32_t encode4(const float (&v)[4]) {
   return (uint32_t)lo | ((uint32_t)hi << 16);
 }
 
-// sqrt(x) to 2 units in the last place; below 2^-126 0, which adds nothing to eps
+// sqrt(x) to 2 units in the last place; 0 for x below 2^-126
 __device__ __forceinline__ float root_approx(float x) {
   float r;
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 
+template <bool SMALL_EPS>
 __device__ __forceinline__ void update(const Params& a, float gs, float& p, float g, float& m, float& v) {
   g = __fmul_rn(g, gs);
   m = __fadd_rn(__fmul_rn(m, a.b1), __fmul_rn(g, a.b1c));
   v = __fadd_rn(__fmul_rn(v, a.b2), __fmul_rn(__fmul_rn(g, g), a.b2c));
-  const float den = __fadd_rn(__fmul_rn(root_approx(v), a.root), a.eps);
+  const float den = __fadd_rn(__fmul_rn(SMALL_EPS ? __fsqrt_rn(v) : root_approx(v), a.root), a.eps);
   p = __fsub_rn(__fmul_rn(p, a.decay), __fmul_rn(__fdividef(m, den), a.step));
 }
 
@@ -189,7 +192,7 @@ struct Block {
 };
 
 // New moments of four values in m and v (8 bits: v comes in as its root's codes) and weights in w.
-template <bool EIGHT>
+template <bool EIGHT, bool SMALL_EPS>
 __device__ __forceinline__ void update4(const Params& a, float gs, float sm, float su, const float (&g)[4],
                                         float (&w)[4], float (&m)[4], float (&v)[4]) {
 #pragma unroll
@@ -199,7 +202,7 @@ __device__ __forceinline__ void update4(const Params& a, float gs, float sm, flo
       const float u = __fmul_rn(v[k], su);
       v[k] = __fmul_rn(u, u);
     }
-    update(a, gs, w[k], g[k], m[k], v[k]);
+    update<SMALL_EPS>(a, gs, w[k], g[k], m[k], v[k]);
   }
 }
 
@@ -232,7 +235,7 @@ __device__ __forceinline__ void store_codes(const Params& a, int64_t f, float (&
 }
 
 // A whole block of an aligned tensor.
-template <typename P, bool EIGHT>
+template <typename P, bool EIGHT, bool SMALL_EPS>
 __device__ __forceinline__ void whole_block(const Params& a, float gs, P* p, int64_t i, int64_t f,
                                             const Block<P, EIGHT>& b) {
   float m[2][4], v[2][4];
@@ -243,7 +246,7 @@ __device__ __forceinline__ void whole_block(const Params& a, float gs, P* p, int
     b.w[h].get(w);
     b.m[h].get(m[h]);
     b.v[h].get(v[h]);
-    update4<EIGHT>(a, gs, b.sm, b.su, g, w, m[h], v[h]);
+    update4<EIGHT, SMALL_EPS>(a, gs, b.sm, b.su, g, w, m[h], v[h]);
     Four<P>::store(p + i + h * 128, w);
     if constexpr (sizeof(P) == 2) Four<float>::store(a.master + f + h * 128, w);
     if constexpr (!EIGHT) {
@@ -256,7 +259,7 @@ __device__ __forceinline__ void whole_block(const Params& a, float gs, P* p, int
 
 // A tensor's ragged last block, or any of one that vectors cannot address: weights and gradients
 // one by one.  The flat buffers are padded to whole blocks; the padding stays 0.
-template <typename P, bool EIGHT>
+template <typename P, bool EIGHT, bool SMALL_EPS>
 __device__ __noinline__ void odd_block(const Params& a, float gs, P* p, const P* gr, int64_t n, int64_t i, int64_t f) {
   Block<P, EIGHT> b;
   b.load_state(a, f);
@@ -276,7 +279,7 @@ __device__ __noinline__ void odd_block(const Params& a, float gs, P* p, const P*
     }
     b.m[h].get(m[h]);
     b.v[h].get(v[h]);
-    update4<EIGHT>(a, gs, b.sm, b.su, g, w, m[h], v[h]);
+    update4<EIGHT, SMALL_EPS>(a, gs, b.sm, b.su, g, w, m[h], v[h]);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (at + k < n) {
@@ -294,7 +297,7 @@ __device__ __noinline__ void odd_block(const Params& a, float gs, P* p, const P*
   if constexpr (EIGHT) store_codes(a, f, m, v);
 }
 
-template <typename P, bool EIGHT, int MOST>
+template <typename P, bool EIGHT, int MOST, bool SMALL_EPS>
 __global__ void __launch_bounds__(kWarps * 32, EIGHT ? kCtas8 : 1)
     adamw_kernel(const __grid_constant__ Table<MOST> table, const __grid_constant__ Params a) {
   int lo = 0, hi = a.count - 1;
@@ -324,16 +327,16 @@ __global__ void __launch_bounds__(kWarps * 32, EIGHT ? kCtas8 : 1)
     for (; at <= fast; at += kStep) {
       const Block<P, EIGHT> now = b;
       if (at + kStep <= fast) b.load(a, p, g, at + kStep + lane4, flat + at + kStep);
-      whole_block<P, EIGHT>(a, gs, p, at + lane4, flat + at, now);
+      whole_block<P, EIGHT, SMALL_EPS>(a, gs, p, at + lane4, flat + at, now);
     }
   } else {
     for (; at <= fast; at += kStep) {
       Block<P, EIGHT> b;
       b.load(a, p, g, at + lane4, flat + at);
-      whole_block<P, EIGHT>(a, gs, p, at + lane4, flat + at, b);
+      whole_block<P, EIGHT, SMALL_EPS>(a, gs, p, at + lane4, flat + at, b);
     }
   }
-  for (; at < end; at += kStep) odd_block<P, EIGHT>(a, gs, p, g, n, at + lane4, flat + at);
+  for (; at < end; at += kStep) odd_block<P, EIGHT, SMALL_EPS>(a, gs, p, g, n, at + lane4, flat + at);
 }
 
 // Tables of two sizes: the parameters of a launch are copied with it, 2 KB for the usual handful
@@ -341,7 +344,7 @@ __global__ void __launch_bounds__(kWarps * 32, EIGHT ? kCtas8 : 1)
 // the large table 56).
 constexpr int kFew = 64, kMost = 768;
 
-template <typename P, bool EIGHT, int MOST>
+template <typename P, bool EIGHT, int MOST, bool SMALL_EPS>
 static int launch(const hi3d_adamw_args* a, const Params& base, int from, int count, cudaStream_t st) {
   Table<MOST> t;
   Params p = base;
@@ -357,16 +360,20 @@ static int launch(const hi3d_adamw_args* a, const Params& base, int from, int co
     if (chunks > 0x7fffffffu) return set_error(HI3D_ERR_INVALID_ARGUMENT, "adamw_step: too many elements");
   }
   if (p.count == 0) return HI3D_OK;
-  adamw_kernel<P, EIGHT, MOST><<<(unsigned)chunks, kWarps * 32, 0, st>>>(t, p);
+  adamw_kernel<P, EIGHT, MOST, SMALL_EPS><<<(unsigned)chunks, kWarps * 32, 0, st>>>(t, p);
   return check_launch("adamw_step");
 }
 
 template <typename P, bool EIGHT>
 static int run(const hi3d_adamw_args* a, const Params& p, cudaStream_t st) {
+  // whether the root of a v below 2^-126, at most 2^-63, is more than half a unit in the last place of eps
+  // (eps 1e-8: not while 1 - beta2^step is above 1.4e-7)
+  const bool small_eps = !(a->eps * 0x1p-25 >= p.root * 0x1p-63);
   for (int from = 0; from < a->count; from += kMost) {
     const int count = a->count - from < kMost ? a->count - from : kMost;
-    const int rc = count <= kFew ? launch<P, EIGHT, kFew>(a, p, from, count, st)
-                                 : launch<P, EIGHT, kMost>(a, p, from, count, st);
+    const int rc = small_eps       ? launch<P, EIGHT, kMost, true>(a, p, from, count, st)
+                   : count <= kFew ? launch<P, EIGHT, kFew, false>(a, p, from, count, st)
+                                   : launch<P, EIGHT, kMost, false>(a, p, from, count, st);
     if (rc) return rc;
   }
   return HI3D_OK;

@@ -41,7 +41,8 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor], exp_avg: t
     """One AdamW step of ``params`` by ``grads``, in place, on the current stream:
 
     ``p *= 1 - lr * weight_decay; m = b1 m + (1 - b1) g; v = b2 v + (1 - b2) g^2;
-    p -= lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)`` in fp32, each operation rounded.
+    p -= lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)`` in fp32: the moments'
+    operations are rounded one by one, the update's root and quotient good to 2 units in the last place each.
 
     Args:
         params, grads: contiguous tensors of one dtype (float32, float16, bfloat16) on one device.

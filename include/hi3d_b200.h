@@ -527,7 +527,8 @@ HI3D_API int hi3d_group_norm_act_bwd(const hi3d_group_norm_args* args, void* wor
  *   g = grad * grad_scale;  p = p (1 - lr weight_decay);  m = beta1 m + (1 - beta1) g;
  *   v = beta2 v + (1 - beta2) g^2;
  *   p -= lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
- * in fp32, each operation rounded.  params, grads, numels and offsets are host arrays of `count`;
+ * in fp32; the moments' operations are rounded one by one, the update's root and quotient are good to 2
+ * units in the last place each.  params, grads, numels and offsets are host arrays of `count`;
  * params and grads are device pointers of the given type.  16-bit weights are the rounded copy of
  * `master` (fp32, flat), 32-bit ones have none.  Tensor i's state lies at element offsets[i] (a
  * multiple of HI3D_ADAMW_BLOCK) of the flat buffers of `total` elements, padded with zeros:

@@ -312,3 +312,26 @@ def test_refusals():
     with pytest.raises(ValueError):
         a.load_state_dict(optim.AdamW([torch.ones(3, device=DEV)] * 1, state_bits=8).state_dict() | {"param_groups": []})
     assert _lib.device_status()["code"] == 0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-14])
+def test_small_eps_and_tiny_gradients(bits, eps):
+    """A v below fp32's normal numbers still has a root: the first step moves each weight by about lr,
+    as in torch's optimiser.  Expected from the fp32 moments (a subnormal v has few bits), the rest in
+    float64: the root, product, sum, quotient and product of the update, 16 * 2^-24 of it."""
+    f = Flat([(4096,)], torch.float32, bits, seed=41)
+    for t in (f.m, f.v) + (() if f.scales is None else (f.scales,)):
+        t.zero_()
+    g = torch.logspace(-20.5, -15, 4096, device=DEV) * torch.where(torch.arange(4096, device=DEV) % 2 == 0, 1, -1)
+    f.grads[0].copy_(g)
+    w = f.params[0].double()
+    b1, b2, lr = 0.9, 0.999, HYPER["lr"]
+    f.step(1, eps=eps, betas=(b1, b2))
+    f32 = lambda x: torch.tensor(x, dtype=torch.float32)  # noqa: E731
+    c = g.cpu()
+    m, v = c * f32(1 - b1), (c * c) * f32(1 - b2)  # the CPU keeps subnormals
+    up = (m.double() * (lr / (1 - b1)) / (v.double().sqrt() * (1 - b2) ** -0.5 + eps)).to(DEV)
+    want = w * (1 - lr * HYPER["weight_decay"]) - up
+    assert torch.isfinite(f.params[0]).all()
+    assert ((f.params[0].double() - want).abs() <= 4 * E * w.abs() + 16 * E * up.abs() + 1e-12).all()
