@@ -114,6 +114,7 @@ class _Bucket:
         self.scales = None if bits == 32 else torch.zeros((2, total // BLOCK), device=device)
         self.master = None if dtype == torch.float32 else torch.zeros(total, device=device)
         self.at = {p: i for i, p in enumerate(params)}
+        self.held: dict[torch.Tensor, dict] = {}  # the views that the optimiser's state has had
 
     def views(self, p: torch.Tensor) -> dict[str, torch.Tensor]:
         """This tensor's part of each buffer."""
@@ -163,10 +164,14 @@ class AdamW(torch.optim.Optimizer):
 
     def _begin(self, index: int, p: torch.Tensor) -> _Bucket:
         bucket = self._bucket(index, p)
-        if p not in self.state:
+        if not self.state.get(p):
             views = bucket.views(p)
+            if p in bucket.held:  # its state was dropped: nothing of it may remain
+                for name in views:
+                    views[name].zero_()
             if "master" in views:
                 views["master"].copy_(p.detach())
+            bucket.held[p] = views
             self.state[p] = {"step": 0, **views}
         return bucket
 
@@ -221,5 +226,6 @@ class AdamW(torch.optim.Optimizer):
                         raise ValueError(f"{name} is {tuple(saved[name].shape)} {saved[name].dtype}, expected "
                                          f"{tuple(view.shape)} {view.dtype}")
                     view.copy_(saved[name])
+                self._bucket(index, p).held[p] = views
                 self.state[p] = {"step": int(saved["step"]), **views}
             mine.update({k: v for k, v in theirs.items() if k != "params"})
