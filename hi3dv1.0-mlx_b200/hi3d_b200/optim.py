@@ -106,7 +106,7 @@ class _Bucket:
     """The flat states of one parameter group's tensors of one dtype and device."""
 
     def __init__(self, params: list[torch.Tensor], bits: int):
-        dtype, device = params[0].dtype, params[0].device
+        self.dtype, self.device = dtype, device = params[0].dtype, params[0].device
         self.offsets, total = state_layout([p.numel() for p in params])
         kind = torch.float32 if bits == 32 else torch.float8_e4m3fn
         self.exp_avg = torch.zeros(total, dtype=kind, device=device)
@@ -114,6 +114,7 @@ class _Bucket:
         self.scales = None if bits == 32 else torch.zeros((2, total // BLOCK), device=device)
         self.master = None if dtype == torch.float32 else torch.zeros(total, device=device)
         self.at = {p: i for i, p in enumerate(params)}
+        self.shapes = {p: p.shape for p in params}
         self.held: dict[torch.Tensor, dict] = {}  # the views that the optimiser's state has had
 
     def views(self, p: torch.Tensor) -> dict[str, torch.Tensor]:
@@ -132,8 +133,10 @@ class AdamW(torch.optim.Optimizer):
 
     ``state_bits=8`` holds the moments in 8 bits (2 bytes an element and 8 per 256, against 8 bytes).
     16-bit parameters get an fp32 master, taken from them at their first step and rounded back
-    after each: load weights before the first step, or with :meth:`load_state_dict`.
-    ``state[p]`` has ``step`` and views of the flat buffers.
+    after each: load weights before the first step, or with :meth:`load_state_dict`.  Parameters are
+    contiguous.  ``state[p]`` has ``step`` and views of the flat buffers; where a parameter changed its
+    type or device, or the optimiser was copied, its state moves into the buffers of its new kind at the
+    next step.
     """
 
     def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
@@ -143,7 +146,7 @@ class AdamW(torch.optim.Optimizer):
         if lr < 0 or eps < 0 or weight_decay < 0 or not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
             raise ValueError("lr, eps and weight_decay must not be negative, betas lie in [0, 1)")
         self.state_bits = state_bits
-        self._buckets: dict[tuple, _Bucket] = {}
+        self._home: dict[torch.Tensor, _Bucket] = {}
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def add_param_group(self, param_group) -> None:
@@ -152,27 +155,48 @@ class AdamW(torch.optim.Optimizer):
             if p.dtype not in DTYPES:
                 raise ValueError(f"AdamW takes float32, float16 or bfloat16 parameters, got {p.dtype}")
 
+    def __getstate__(self) -> dict:
+        return {**super().__getstate__(), "state_bits": self.state_bits}
+
+    def __setstate__(self, state: dict) -> None:
+        super().__setstate__(state)
+        self._home = {}  # the states move into new buffers
+
+    def _housed(self, p: torch.Tensor) -> _Bucket | None:
+        """The bucket that was made for ``p`` as it is now."""
+        b = self._home.get(p)
+        return b if b is not None and b.dtype == p.dtype and b.device == p.device and b.shapes[p] == p.shape else None
+
     def _bucket(self, index: int, p: torch.Tensor) -> _Bucket:
-        """The bucket of ``p`` in group ``index``, made for all the group's tensors of its kind at first use."""
-        key = (index, p.dtype, p.device)
-        bucket = self._buckets.get(key)
+        """The bucket of ``p`` in group ``index``, made at first use for all the group's tensors of its kind
+        that are in none."""
+        bucket = self._housed(p)
         if bucket is None:
             _lib.require_cuda(p)
-            alike = [q for q in self.param_groups[index]["params"] if q.dtype == p.dtype and q.device == p.device]
-            bucket = self._buckets[key] = _Bucket(alike, self.state_bits)
+            alike = [q for q in self.param_groups[index]["params"]
+                     if q.dtype == p.dtype and q.device == p.device and self._housed(q) is None]
+            bucket = _Bucket(alike, self.state_bits)
+            self._home.update(dict.fromkeys(alike, bucket))
         return bucket
 
     def _begin(self, index: int, p: torch.Tensor) -> _Bucket:
-        bucket = self._bucket(index, p)
-        if not self.state.get(p):
-            views = bucket.views(p)
-            if p in bucket.held:  # its state was dropped: nothing of it may remain
-                for name in views:
-                    views[name].zero_()
-            if "master" in views:
-                views["master"].copy_(p.detach())
-            bucket.held[p] = views
-            self.state[p] = {"step": 0, **views}
+        bucket, state = self._bucket(index, p), self.state.get(p)
+        if state and p in bucket.held and state["exp_avg"] is bucket.held[p]["exp_avg"]:
+            return bucket
+        views = bucket.views(p)
+        if state:  # of another bucket, or a copy: it moves in
+            for name, view in views.items():
+                if name in state and state[name].shape != view.shape:
+                    raise ValueError(f"{name} of shape {tuple(state[name].shape)} for a parameter of shape {tuple(p.shape)}")
+        for name, view in views.items():
+            if state and name in state:
+                view.copy_(state[name])
+            elif name == "master":
+                view.copy_(p.detach())
+            elif p in bucket.held:  # its state was dropped: nothing of it may remain
+                view.zero_()
+        bucket.held[p] = views
+        self.state[p] = {"step": state["step"] if state else 0, **views}
         return bucket
 
     @torch.no_grad()
