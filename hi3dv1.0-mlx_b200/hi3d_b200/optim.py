@@ -232,24 +232,34 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def load_state_dict(self, state_dict) -> None:
         """Takes over groups and states (of the same ``state_bits`` and parameter dtypes), copied into
-        this optimiser's own buffers with their types kept."""
+        this optimiser's own buffers with their types kept.  A state that does not fit changes nothing; a
+        parameter that it does not know starts anew."""
         groups = state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("state_dict has other parameter groups")
+        found = []
         for index, (mine, theirs) in enumerate(zip(self.param_groups, groups)):
             for p, key in zip(mine["params"], theirs["params"]):
                 saved = state_dict["state"].get(key)
-                if saved is None:
-                    self.state.pop(p, None)
+                if not saved:
+                    found.append((p, None, None, None))
                     continue
-                views = self._bucket(index, p).views(p)
+                bucket = self._bucket(index, p)
+                views = bucket.views(p)
                 if set(views) != set(saved) - {"step"}:
                     raise ValueError(f"state has {sorted(saved)}, this optimiser keeps {sorted(views)}")
                 for name, view in views.items():
                     if saved[name].shape != view.shape or saved[name].dtype != view.dtype:
                         raise ValueError(f"{name} is {tuple(saved[name].shape)} {saved[name].dtype}, expected "
                                          f"{tuple(view.shape)} {view.dtype}")
-                    view.copy_(saved[name])
-                self._bucket(index, p).held[p] = views
-                self.state[p] = {"step": int(saved["step"]), **views}
+                found.append((p, bucket, views, saved))
+        for p, bucket, views, saved in found:
+            if saved is None:
+                self.state.pop(p, None)
+                continue
+            for name, view in views.items():
+                view.copy_(saved[name])
+            bucket.held[p] = views
+            self.state[p] = {"step": int(saved["step"]), **views}
+        for mine, theirs in zip(self.param_groups, groups):
             mine.update({k: v for k, v in theirs.items() if k != "params"})

@@ -170,3 +170,19 @@ def test_a_parameter_that_grew_before_its_first_step_leaves_its_neighbours_alone
     ps[1].grad = ps[2].grad = None
     _steps(opt, ps[:1], [1])
     assert torch.equal(opt.state[ps[1]]["exp_avg"], held) and opt.state[ps[0]]["exp_avg"].shape == (700,)
+
+
+def test_a_load_that_is_refused_changes_nothing():
+    ps, qs = _params(), _params()
+    a, b = optim.AdamW(ps, lr=1e-2), optim.AdamW(qs, lr=1e-2)
+    _steps(a, ps, range(2))
+    _steps(b, qs, range(2))
+    bad = optim.AdamW(_params(seed=3), lr=0.5)
+    _steps(bad, bad.param_groups[0]["params"], [1])
+    bad = bad.state_dict()
+    bad["state"][2]["exp_avg"] = torch.zeros(3)
+    with pytest.raises(ValueError):
+        a.load_state_dict(bad)
+    _steps(a, ps, [4])
+    _steps(b, qs, [4])
+    _equal(ps, qs)
