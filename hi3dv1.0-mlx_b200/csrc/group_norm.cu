@@ -7,8 +7,8 @@
 //
 // Each direction is three launches:
 //   1. chunks of rows, one CTA each: per-channel sums of the chunk (forward: mean and squared
-//      deviations about it, from sums shifted by the first value, so a large mean costs no bits;
-//      backward: sum du and sum du xh);
+//      deviations about it, a few rows at a time about the mean of those before them, so neither a
+//      large mean nor an atypical first row costs bits; backward: sum du and sum du xh);
 //   2. per sample and channel, the chunks in order (forward: pooled deviations; backward: sums, and
 //      dw, db, over several samples by one more launch), 32 channels a CTA;
 //   3. the chunks again, last first: a CTA folds the channels of each group (shared memory) and
@@ -169,6 +169,24 @@ __device__ __forceinline__ void each_row(const T* x, int64_t stride, int r, int 
     }
   }
 }
+// body(up to U rows as they lie in memory, their number): the same rows U at a time.
+template <typename T, int V, int U, typename F>
+__device__ __forceinline__ void each_rows(const T* x, int64_t stride, int r, int end, int step, F body) {
+  Raw<T, V> a[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (r + u * step < end) a[u].load(x + (r + u * step) * stride);
+  for (int left = (end - r + step - 1) / step; left > 0; left -= U, r += U * step) {
+    Raw<T, V> now[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      now[u] = a[u];
+      const int next = r + (U + u) * step;
+      if (next < end) a[u].load(x + next * stride);
+    }
+    body(now, min(left, U));
+  }
+}
 template <typename T, int V, int U, typename F>
 __device__ __forceinline__ void each_row(const T* x, const T* y, int64_t stride, int r, int end, int step, F body) {
   Raw<T, V> a[U], b[U];
@@ -236,6 +254,12 @@ __device__ __forceinline__ uint64_t act_grad2(uint64_t u, uint64_t d) {
   return f2_mul(d, f2_mul(s, g));
 }
 
+// 0 for what rounding left below it; a NaN stays one
+template <typename F>
+__device__ __forceinline__ F above0(F v) {
+  return v < 0 ? 0 : v;
+}
+
 // ---------------------------------------------------------------- pass 1
 // Threads: column x (V channels from x V), row lane y; lanes' results join in lane order.
 template <typename T, int V>
@@ -247,29 +271,43 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const T* __restrict__ x
   const int lanes = kThreads / s.cols, cx = threadIdx.x % s.cols, y = threadIdx.x / s.cols;
   const int ch = (blockIdx.y * s.cols + cx) * V;
   const bool on = y < lanes && ch < s.channels;
-  uint64_t k[kPairs<V>], a[kPairs<V>] = {}, b[kPairs<V>] = {};
+  // k: the thread's first value; m: the mean so far less k; q: squared deviations about it
+  uint64_t k[kPairs<V>], m[kPairs<V>] = {}, q[kPairs<V>] = {};
   int n = 0;
-  // sums about the thread's first value
-  auto add = [&](int, const uint64_t (&v)[kPairs<V>]) {
-    if (n++ == 0) {
+  auto add = [&](const Raw<T, V>(&rows)[kInFlight], int have) {
+    uint64_t v[kPairs<V>], a[kPairs<V>] = {}, b[kPairs<V>] = {};
+    if (n == 0) rows[0].get(k);
 #pragma unroll
-      for (int i = 0; i < kPairs<V>; ++i) k[i] = v[i];
+    for (int u = 0; u < kInFlight; ++u) {
+      if (u >= have) break;
+      rows[u].get(v);
+#pragma unroll
+      for (int i = 0; i < kPairs<V>; ++i) {
+        // about k first: a mean of many deviations leaves the difference its bits
+        const uint64_t d = f2_add(f2_fma(k[i], f2_splat(-1.0f), v[i]), f2_mul(m[i], f2_splat(-1.0f)));
+        a[i] = f2_add(a[i], d);
+        b[i] = f2_fma(d, d, b[i]);
+      }
     }
+    // joined by the formula for the deviations of two sets: their own, and n have / (n + have) times the
+    // square of the difference of their means
+    const float inv = 1.0f / have, w = (float)have / (n + have), c = n * w;
+    n += have;
 #pragma unroll
     for (int i = 0; i < kPairs<V>; ++i) {
-      const uint64_t d = f2_fma(k[i], f2_splat(-1.0f), v[i]);
-      a[i] = f2_add(a[i], d);
-      b[i] = f2_fma(d, d, b[i]);
+      const uint64_t e = f2_mul(a[i], f2_splat(inv));
+      const uint64_t own = f2_fma(f2_mul(a[i], f2_splat(-1.0f)), e, b[i]);
+      q[i] = f2_add(q[i], f2_fma(f2_mul(e, e), f2_splat(c), own));
+      m[i] = f2_fma(e, f2_splat(w), m[i]);
     }
   };
   if (on) {
-    each_row<T, V, kInFlight>(x + ch, s.channels, t.r0 + y, t.r1, lanes, add);
+    each_rows<T, V, kInFlight>(x + ch, s.channels, t.r0 + y, t.r1, lanes, add);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float sum = lane_of(a[i / 2], i & 1), m = n ? sum / n : 0.f;  // mean - k
+    for (int i = 0; i < V; ++i)
       sh[(y * s.cols + cx) * V + i] =
-          n ? make_float2(lane_of(k[i / 2], i & 1) + m, fmaxf(0.f, fmaf(-sum, m, lane_of(b[i / 2], i & 1)))) : make_float2(0.f, 0.f);
-    }
+          n ? make_float2(lane_of(k[i / 2], i & 1) + lane_of(m[i / 2], i & 1), above0(lane_of(q[i / 2], i & 1)))
+            : make_float2(0.f, 0.f);
   }
   if (cx == 0 && y < lanes) count[y] = n;
   __syncthreads();
@@ -290,8 +328,7 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const T* __restrict__ x
     }
     const double mean = have ? sum / have : 0, between = fma(-sum, mean, square);
     part[(int64_t)blockIdx.x * s.channels + c] =
-        have ? make_float2((float)(first + mean), (float)(dev + (between < 0 ? 0 : between)))  // a NaN stays one
-             : make_float2(0.f, 0.f);
+        have ? make_float2((float)(first + mean), (float)(dev + above0(between))) : make_float2(0.f, 0.f);
   }
 }
 
@@ -346,26 +383,26 @@ __global__ void __launch_bounds__(kThreads) sums_kernel(const T* __restrict__ x,
 
 // ---------------------------------------------------------------- pass 2
 // 32 channels x 32 chunk lanes a CTA, one sample (forward): {mean, squared deviations} of each
-// channel over the sample's rows, from the chunks' means about the first chunk's (so their
-// squares keep their bits) and deviations.
+// channel over the sample's rows, from the chunks' means and deviations.  In 64 bits about the first
+// chunk's mean, which need not be near the others'.
 __global__ void __launch_bounds__(1024) pool_kernel(const float2* __restrict__ part, const Shape s,
                                                     float2* __restrict__ chan) {
-  __shared__ float red[3][32][33];
+  __shared__ double red[3][32][33];
   const int c = blockIdx.x * 32 + threadIdx.x, smp = blockIdx.y;
   const int lo = offset(s, smp), len = max(offset(s, smp + 1) - lo, 0);
   const int64_t base = lo / s.chunk + smp;
   const int chunks = (len + s.chunk - 1) / s.chunk;
   const bool on = c < s.channels && chunks > 0;
   const float2* p = part + base * s.channels + c;
-  const float first = on ? p->x : 0.f;
-  float a = 0.f, b = 0.f, d = 0.f;
+  const double first = on ? p->x : 0.f;
+  double a = 0, b = 0, d = 0;
   if (on) {
 #pragma unroll 8
     for (int k = threadIdx.y; k < chunks; k += 32) {
       const float2 q = p[(int64_t)k * s.channels];
-      const float e = q.x - first, n = (float)min(s.chunk, len - k * s.chunk);
-      a = fmaf(e, n, a);
-      b = fmaf(e * e, n, b);
+      const double e = q.x - first, n = min(s.chunk, len - k * s.chunk);
+      a = fma(e, n, a);
+      b = fma(e * e, n, b);
       d += q.y;
     }
   }
@@ -374,12 +411,12 @@ __global__ void __launch_bounds__(1024) pool_kernel(const float2* __restrict__ p
   red[2][threadIdx.y][threadIdx.x] = d;
   __syncthreads();
   if (threadIdx.y == 0 && c < s.channels) {
-    a = b = d = 0.f;
+    a = b = d = 0;
 #pragma unroll
     for (int y = 0; y < 32; ++y)
       a += red[0][y][threadIdx.x], b += red[1][y][threadIdx.x], d += red[2][y][threadIdx.x];
-    const float m = chunks > 0 ? a / (float)len : 0.f;
-    chan[(int64_t)smp * s.channels + c] = make_float2(first + m, d + fmaxf(0.f, fmaf(-a, m, b)));
+    const double m = chunks > 0 ? a / len : 0;
+    chan[(int64_t)smp * s.channels + c] = make_float2((float)(first + m), (float)(d + above0(fma(-a, m, b))));
   }
 }
 

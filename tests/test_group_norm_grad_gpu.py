@@ -235,3 +235,25 @@ def test_refusals():
         vae.group_norm_act_backward(y.half(), x, mean, rstd, w, b)
     with pytest.raises(ValueError):
         vae.group_norm_act_backward(y, x, mean.expand(2, 4), rstd.expand(2, 4), w, b)
+
+
+@pytest.mark.parametrize("first", [0.0, 30.0, -3000.0])
+@pytest.mark.parametrize("mean", [0.0, 300.0])
+@pytest.mark.parametrize("samples,rows,channels", [(140, 677, 1024), (1, 40000, 64)])
+def test_an_atypical_first_row_costs_no_bits(first, mean, samples, rows, channels):
+    """A first row far from the others, in samples whose hundreds of rows one thread sums and in one of
+    many chunks: the same bounds."""
+    x = _rand((samples, rows, channels), 50) + mean
+    x[:, 0] = first
+    compare(x, _rand(x.shape, 51), _rand((channels,), 52) * 0.5 + 1, _rand((channels,), 53), 32, "swish",
+            [rows] * samples, packed=False)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_atypical_first_rows_of_many_chunks(dtype):
+    """The first rows, about one chunk of a few hundred, at 1000 where the others are around 0."""
+    x = _rand((60000, 64), 54)
+    x[:200] += 1000.0
+    x = x.to(dtype)
+    compare(x, _rand(x.shape, 55, dtype), _rand((64,), 56) * 0.5 + 1, _rand((64,), 57), 32, "swish", [60000],
+            packed=False)
