@@ -189,8 +189,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           continue;
         }
         float mx = -INFINITY;
-        for (int s = 0; s < p.slot0; ++s) mx = fmaxf(mx, slot_lse(p, s, prow, h));
-        if (mx == -INFINITY) continue;  // no keys at all: the row is left untouched
+        bool none = true;
+        for (int s = 0; s < p.slot0; ++s) {
+          const float ls = slot_lse(p, s, prow, h);
+          mx = fmaxf(mx, ls);
+          none = none && ls == -INFINITY;
+        }
+        if (none) continue;  // no keys at all: the row is left untouched
         float wsum = 0.f;
         for (int s = 0; s < p.slot0; ++s) {
           const float ls = slot_lse(p, s, prow, h);
@@ -418,21 +423,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // Row maximum with four independent chains (a single chain of BK dependent
       // max operations would leave the two softmax warps of each sub-partition
-      // waiting on latency).
+      // waiting on latency).  A NaN score makes it NaN, and with it the row's maximum, sum and output.
       float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int e = 0; e < C::BK; e += 8) {
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          mq[u] = fmax3(mq[u], __uint_as_float(sv[e + 2 * u]), __uint_as_float(sv[e + 2 * u + 1]));
+          mq[u] = fmax3_nan(mq[u], __uint_as_float(sv[e + 2 * u]), __uint_as_float(sv[e + 2 * u + 1]));
       }
-      const float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3]));
+      const float mx = fmax3_nan(fmax3_nan(mq[0], mq[1], mq[2]), mq[3], mq[3]);
       // Running maximum in the scaled log2 domain.  The maximum used for the
       // exponentials (m_run) only moves when a row's maximum grows by more than
       // kRescaleLog2; until then P may reach 2^kRescaleLog2 (exact in the 16-bit
       // P and in fp32 l), and O needs no correction.  O / l is unchanged.
       const float m_blk = mx * scale2;
-      const bool grow = m_blk > m_run + kRescaleLog2;
+      const bool grow = !(m_blk <= m_run + kRescaleLog2);
       const bool warp_grow = __any_sync(0xffffffffu, grow);
       const float m_new = grow ? m_blk : m_run;
       // the correction factor needs the MUFU unit only in the rare blocks where
@@ -627,8 +632,13 @@ __global__ void __launch_bounds__(256) merge_kernel(const float* __restrict__ pa
   const int h = (int)(wid - r * heads);
   if (cu && (r < cu[0] || r >= cu[num_seqs])) return;
   float mx = -INFINITY;
-  for (int s = 0; s < splits; ++s) mx = fmaxf(mx, part_lse[((int64_t)s * rows + r) * heads + h]);
-  if (mx == -INFINITY && !LSE) return;
+  bool none = true;  // no split saw keys (a maximum of -inf could also be that of NaN)
+  for (int s = 0; s < splits; ++s) {
+    const float ls = part_lse[((int64_t)s * rows + r) * heads + h];
+    mx = fmaxf(mx, ls);
+    none = none && ls == -INFINITY;
+  }
+  if (none && !LSE) return;
   float acc[E] = {};
   float wsum = 0.f;
   for (int s = 0; s < splits; ++s) {
@@ -640,14 +650,14 @@ __global__ void __launch_bounds__(256) merge_kernel(const float* __restrict__ pa
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] += wgt * po[e];
   }
-  const float inv = LSE && mx == -INFINITY ? 0.0f : 1.0f / wsum;
+  const float inv = LSE && none ? 0.0f : 1.0f / wsum;
   const int64_t b = dense ? r / nq : 0, qr = dense ? r - b * nq : r;
   T* dst = out + b * o_batch + qr * o_row + (int64_t)h * o_head + lane * E;
 #pragma unroll
   for (int e = 0; e < E; ++e) dst[e] = Cvt<T>::from_f(acc[e] * inv);
   if constexpr (LSE) {
     if (lane == 0)
-      lse[(b * heads + h) * nq + qr] = mx == -INFINITY ? -INFINITY : (mx + log2f(wsum)) * kLn2;
+      lse[(b * heads + h) * nq + qr] = none ? -INFINITY : (mx + log2f(wsum)) * kLn2;
   }
 }
 

@@ -73,6 +73,7 @@ struct Params {
   const float4* stat;
   // fp16: largest finite |dO| of each statistics tile, and |V| of each tile of 128 rows of a key head
   const float *max_o, *max_v;
+  const float* spoiled;  // 1 for each statistics tile that has a NaN log-sum-exp, else 0
   float scale, scale2;
 };
 
@@ -500,23 +501,27 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
     // The exponent that dS carries, from the rows that enter this CTA's sums alone: another sequence's,
     // head's or (query CTAs) row tile's sizes do not cost these their bits.
     int kexp = 0;
+    // the largest of a value of each statistics tile that this CTA's sums run over
+    auto over_tiles = [&](const float* m) {
+      int first = 0, count = p.q_tiles;
+      if constexpr (!KV) return m[stat_tile(p, seq, h) + t];
+      if (p.cu_q) {
+        tile_range(p.cu_q, b0, b1, p.nq, first, count);
+        return fold_max(m + (int64_t)h * p.group * p.q_tiles + first, p.q_tiles, count, p.group);
+      }
+      return fold_max(m + ((int64_t)b0 * p.heads + h * p.group) * p.q_tiles, (int64_t)p.heads * p.q_tiles,
+                      p.group * p.q_tiles, b1 - b0);
+    };
     if constexpr (kHalf) {
       const int hk = KV ? h : h / p.group, set = p.kv_seqs == 1 ? 0 : seq;
-      int vt = 0, nv = p.kv_tiles, qt = 0, nq = p.q_tiles;
+      int vt = 0, nv = p.kv_tiles;
       if (p.cu_k) tile_range(p.cu_k, seq, seq + 1, p.nk, vt, nv);
       const float max_v = fold_max(p.max_v + ((int64_t)(p.cu_k ? 0 : set) * p.kv_heads + hk) * p.kv_tiles + vt, 0, nv, 1);
-      float max_o;
-      if constexpr (!KV) {
-        max_o = p.max_o[stat_tile(p, seq, h) + t];
-      } else if (p.cu_q) {
-        tile_range(p.cu_q, b0, b1, p.nq, qt, nq);
-        max_o = fold_max(p.max_o + (int64_t)h * p.group * p.q_tiles + qt, p.q_tiles, nq, p.group);
-      } else {
-        max_o = fold_max(p.max_o + ((int64_t)b0 * p.heads + h * p.group) * p.q_tiles, (int64_t)p.heads * p.q_tiles,
-                         p.group * p.q_tiles, b1 - b0);
-      }
-      kexp = ds_exponent(max_o, max_v, D);
+      kexp = ds_exponent(over_tiles(p.max_o), max_v, D);
     }
+    // A NaN log-sum-exp must reach dV through every P of its row, also those that the polynomial would
+    // make finite (dK and dQ have it from delta): such CTAs take the exponentials of the masked form.
+    const bool spoiled = KV && over_tiles(p.spoiled) > 0.f;
     // key CTAs keep P 2^kPShift in 16 bits: dS takes the rest of its exponent here
     const uint64_t gain = f2_splat(ldexpf(1.0f, kexp - kPShift));
     // query CTAs: this row's statistics, the exponent of dS inside the probability's
@@ -534,7 +539,7 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
     // broadcast still moves 16 bytes to each lane).
     const int col0 = KV ? 2 * (lane & 3) : 0;
     auto column = [&](int e) { return col0 + (KV ? 8 * ((e >> 1) & 3) : 2 * e); };
-    // One block; MASK: only its first `valid` rows are the sequence's.
+    // One block; MASK: only its first `valid` rows are the sequence's, all exponentials by the MUFU unit.
     auto block = [&](int j, int valid, auto mask) {
       constexpr bool MASK = decltype(mask)::value;
       const uint32_t tS = tmem + lane_addr + (j & 1) * BN + group * HC;
@@ -560,7 +565,7 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
           const uint64_t x =
               f2_fma(f2_pack(__uint_as_float(sv[u][2 * e]), __uint_as_float(sv[u][2 * e + 1])), scale2x2, bias);
           float p0, p1;
-          if (e * kEmuPairs % 16 < kEmuPairs) {  // spread over the 16
+          if (!MASK && e * kEmuPairs % 16 < kEmuPairs) {  // spread over the 16
             f2_unpack(f2_exp2_poly(x), p0, p1);
           } else {
             f2_unpack(x, p0, p1);
@@ -643,10 +648,10 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
       // the blocks of one sequence and head; its last may be ragged
       const int m = min(n - j, it.nblk - it.blk), whole = (int)(it.len / BN) - it.blk;
       for (int i = 0; i < m; ++i, ++j) {
-        if (i < whole)
+        if (i < whole && !spoiled)
           block(j, BN, std::false_type());
         else
-          block(j, it.tail(), std::true_type());
+          block(j, i < whole ? BN : it.tail(), std::true_type());
       }
       it.skip(m);
     }
@@ -743,7 +748,7 @@ struct StatParams {
   Strides so, sdo, sq, sk, sv;
   const float* lse;
   float* stat;
-  float *max_o, *max_v;
+  float *max_o, *max_v, *spoiled;
   int stat_blocks;
 };
 
@@ -784,7 +789,7 @@ __device__ __forceinline__ void put_stat(const StatParams& q, int64_t tile, int 
 // each would take 24), after which a lane has one key.
 template <typename T, int D>
 __device__ __forceinline__ void few_keys(const Params& p, const StatParams& q, int t, int h, int b, int64_t tile,
-                                         float& big) {
+                                         float& big, bool& nan) {
   constexpr bool kHalf = std::is_same<T, __half>::value;
   constexpr int L = D == 64 ? 8 : 16;
   constexpr float shift = kHalf ? (float)kPShift : 0.f;
@@ -808,6 +813,7 @@ __device__ __forceinline__ void few_keys(const Params& p, const StatParams& q, i
       const uint4 a = in ? *reinterpret_cast<const uint4*>(x + (start + row) * q.sq.row) : zero;
       const uint4 g = in ? *reinterpret_cast<const uint4*>(d + (start + row) * q.sdo.row) : zero;
       if (row < len) l = q.lse[((int64_t)batch * p.heads + h) * p.nq + start + row] * kLog2e;
+      nan = nan || l != l;
       if constexpr (kHalf) big = abs_max8<T, D>(g, big);
 #pragma unroll 1
       for (int j = 0; j < (int)keys; j += 4) {
@@ -855,6 +861,7 @@ __global__ void __launch_bounds__(256, FEW ? kFewCtas : kStatCtas)
   const bool on = sub * 8 < D;
   constexpr float shift = kHalf ? (float)kPShift : 0.f;  // the exponent that P carries in 16 bits
   float big = 0.f;
+  bool nan = false;
   if ((int)blockIdx.x < q.stat_blocks) {
     int t = blockIdx.x % p.q_tiles, rest = blockIdx.x / p.q_tiles;
     const int64_t tile = blockIdx.x;
@@ -868,7 +875,10 @@ __global__ void __launch_bounds__(256, FEW ? kFewCtas : kStatCtas)
     seq_range(p.cu_q, b, p.nq, start, len);
     const int batch = p.cu_q ? 0 : b;
     if (t < 0 || (int64_t)t * kRows >= len) {
-      if (kHalf && threadIdx.x == 0) q.max_o[tile] = 0.f;
+      if (threadIdx.x == 0) {
+        q.spoiled[tile] = 0.f;
+        if (kHalf) q.max_o[tile] = 0.f;
+      }
       return;
     }
     const T* o = static_cast<const T*>(q.o) + batch * q.so.batch + (int64_t)h * q.so.head + sub * 8;
@@ -876,7 +886,7 @@ __global__ void __launch_bounds__(256, FEW ? kFewCtas : kStatCtas)
     int64_t k_start, keys = p.nk;
     if (FEW) seq_range(p.cu_k, b, p.nk, k_start, keys);
     if (FEW && keys <= kFewKeys) {
-      few_keys<T, D>(p, q, t, h, b, tile, big);
+      few_keys<T, D>(p, q, t, h, b, tile, big, nan);
     } else {
 #pragma unroll 4
       for (int r = threadIdx.x / L; r < kRows; r += 256 / L) {
@@ -890,12 +900,15 @@ __global__ void __launch_bounds__(256, FEW ? kFewCtas : kStatCtas)
         }
 #pragma unroll
         for (int m = L / 2; m > 0; m >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, m);
-        if (sub == 0)
-          put_stat(q, tile, r,
-                   row < len ? shift - q.lse[((int64_t)batch * p.heads + h) * p.nq + start + row] * kLog2e : -INFINITY,
-                   row < len ? -acc : 0.f);
+        if (sub == 0) {
+          const float l = row < len ? q.lse[((int64_t)batch * p.heads + h) * p.nq + start + row] : INFINITY;
+          nan = nan || l != l;
+          put_stat(q, tile, r, shift - l * kLog2e, row < len ? -acc : 0.f);
+        }
       }
     }
+    const int any = __syncthreads_or(nan);
+    if (threadIdx.x == 0) q.spoiled[tile] = any ? 1.f : 0.f;
   } else {
     const int blk = blockIdx.x - q.stat_blocks;
     int t = blk % p.kv_tiles;
@@ -1033,7 +1046,7 @@ static Plan make_plan(const hi3d_attn_bwd_args* a) {
   const int64_t stat_tiles = (int64_t)n.q_tiles * a->heads * n.q_batches;
   const bool half = a->dtype == HI3D_F16;
   n.max_o = half ? stat_tiles : 0, n.max_v = half ? kv_tiles : 0;
-  n.max_bytes = round256((n.max_o + n.max_v) * 4);
+  n.max_bytes = round256((n.max_o + n.max_v + stat_tiles) * 4);
   n.stat_bytes = round256(stat_tiles * kRows * 8);
   n.kv_part = (int64_t)n.kv_batches * a->kv_heads * a->nk * a->head_dim;
   n.q_part = (int64_t)n.q_batches * a->heads * a->nq * a->head_dim;
@@ -1110,7 +1123,7 @@ static int launch(const hi3d_attn_bwd_args* a, const Plan& n, uint8_t* ws, cudaS
   p.kv_splits = n.kv_splits, p.q_splits = n.q_splits;
   p.scale = a->scale, p.scale2 = a->scale * kLog2e;
   float* const max_o = reinterpret_cast<float*>(ws);
-  p.max_o = max_o, p.max_v = max_o + n.max_o;
+  p.max_o = max_o, p.max_v = max_o + n.max_o, p.spoiled = max_o + n.max_o + n.max_v;
   p.stat = reinterpret_cast<const float4*>(ws + n.max_bytes);
   p.part_kv = reinterpret_cast<float*>(ws + n.max_bytes + n.stat_bytes);
   p.part_q = p.part_kv + (n.kv_splits > 1 ? round256(n.kv_part * 2 * n.kv_splits * 4) / 4 : 0);
@@ -1124,7 +1137,7 @@ static int launch(const hi3d_attn_bwd_args* a, const Plan& n, uint8_t* ws, cudaS
   q.sv = {a->v_row, a->v_head, a->v_batch};
   q.lse = a->lse;
   q.stat = reinterpret_cast<float*>(ws + n.max_bytes);
-  q.max_o = max_o, q.max_v = max_o + n.max_o;
+  q.max_o = max_o, q.max_v = max_o + n.max_o, q.spoiled = max_o + n.max_o + n.max_v;
   q.stat_blocks = (int)((int64_t)n.q_tiles * a->heads * qb);
   const int64_t blocks = q.stat_blocks + n.max_v;
   if (a->cu_seqlens_k || a->nk <= kFewKeys)

@@ -511,9 +511,10 @@ __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
   return d;
 }
 __device__ __forceinline__ uint64_t f2_splat(float v) { return f2_pack(v, v); }
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
+// The largest of three values, or NaN if one is
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
@@ -524,7 +525,9 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
 // relative error over [-0.5, 0.5]; max relative error 2.7e-6 in fp32 Horner);
 // the result's exponent field is then increased by n.  Inputs must be <= 127;
 // they are clamped below at -125 so the exponent arithmetic stays in the
-// normal range (2^-125 rounds to zero in the 16-bit P either way).
+// normal range (2^-125 rounds to zero in the 16-bit P either way).  A NaN comes out
+// as 2^-125: callers see to it that it is not lost (keeping it here, by a product with
+// 2^n, costs the attention backward 4 %).
 __device__ __forceinline__ uint64_t f2_exp2_poly(uint64_t x) {
   float x0, x1;
   f2_unpack(x, x0, x1);

@@ -525,3 +525,36 @@ def test_fp16_query_gradients_do_not_depend_on_other_rows_sizes():
     rest = torch.ones(2000, dtype=torch.bool, device=DEV)
     rest[256:384] = False
     _each_by_its_own([dq[:, :, rest]], [want[:, :, rest]])
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, torch.float16), (64, torch.bfloat16), (128, torch.bfloat16)])
+@pytest.mark.parametrize("nq,nk", [(130, 300), (3, 9000), (70, 7)])
+@pytest.mark.parametrize("at", [0, 1, 2])
+def test_a_nan_reaches_all_that_depends_on_it(dim, dtype, nq, nk, at):
+    """A NaN in a query row makes that row's output and every dk and dv of its head NaN, one in a key
+    every row of the head; the other head stays as it was.  In one pass, split, and over few keys."""
+    q, do = _rand((1, 2, nq, dim), dtype, 111), _rand((1, 2, nq, dim), dtype, 112)
+    k, v = _rand((1, 2, nk, dim), dtype, 113), _rand((1, 2, nk, dim), dtype, 114)
+    clean = dense(q, k, v, do, dim ** -0.5)
+    bad = q.clone()
+    bad[0, 0, at, 5] = math.nan
+    out, lse, dq, dk, dv = dense(bad, k, v, do, dim ** -0.5)
+    assert out[0, 0, at].isnan().all() and lse[0, 0, at].isnan() and dq[0, 0, at].isnan().all()
+    assert dk[0, 0].isnan().all() and dv[0, 0].isnan().all()
+    assert all(t[0, 0].isfinite().any(-1).sum() == nq - 1 for t in (out, dq))
+    for got, want in zip((out, lse, dq, dk, dv), clean):
+        assert torch.allclose(got[0, 1].double(), want[0, 1].double(), rtol=0, atol=2 * U[dtype])
+    bad = k.clone()
+    bad[0, 0, at, 5] = math.nan
+    got = dense(q, bad, v, do, dim ** -0.5)
+    assert all(t[0, 0].isnan().all() for t in got)
+
+
+def test_a_nan_key_spoils_every_row_at_any_place():
+    q, k, v = (_rand((1, 1, 40 + 24 * (i > 0), 64), torch.bfloat16, 115 + i) for i in range(3))
+    for at in range(64):
+        bad = k.clone()
+        bad[0, 0, at] = math.nan
+        out, lse = attention.flash_attention_lse(q, bad, v, 0.125)
+        assert out.isnan().all() and lse.isnan().all(), at
+        assert attention.flash_attention(q, bad, v, 0.125).isnan().all(), at
