@@ -227,31 +227,45 @@ __device__ __forceinline__ void store(T* p, const uint64_t (&v)[kPairs<V>]) {
   }
 }
 
-// sigmoid(u) = 1 / (1 + exp(-u)) of a pair: two exponentials and one reciprocal, of the product
-// (relative error about 2^-21).  Below -40, where it is under 2^-57, it is held there: the product
-// of two denominators then stays finite.
-__device__ __forceinline__ uint64_t sigmoid2(uint64_t u) {
+// u, not below -40 (a NaN stays one).  There sigmoid(u) is under 2^-57, and u sigmoid(u) and its slope are
+// 0 to 1e-15; held, the product of two denominators stays finite and a huge -u is not multiplied
+// by a factor that should have vanished.
+__device__ __forceinline__ float from_40(float u) {
+  return u < -40.0f ? -40.0f : u;
+}
+// {sigmoid(u), 1 - sigmoid(u)} = {1, E} / (1 + E), E = exp(-u), of a pair of u >= -40: two exponentials and
+// one reciprocal, of the product (relative error about 2^-21).
+struct Sigmoid {
+  uint64_t s, rest;
+};
+__device__ __forceinline__ Sigmoid sigmoid2(uint64_t u) {
   float a, b;
+  // a NaN spoils its own value (by the factor u), not its neighbour's through the reciprocal
   f2_unpack(u, a, b);
   f2_unpack(f2_mul(f2_pack(fmaxf(a, -40.0f), fmaxf(b, -40.0f)), f2_splat(-1.4426950408889634f)), a, b);
-  const uint64_t d = f2_add(f2_pack(ex2_approx(a), ex2_approx(b)), f2_splat(1.0f));
-  f2_unpack(d, a, b);
+  const uint64_t e = f2_pack(ex2_approx(a), ex2_approx(b));
+  f2_unpack(f2_add(e, f2_splat(1.0f)), a, b);
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
-  return f2_mul(f2_pack(b, a), f2_splat(r));
+  const uint64_t s = f2_mul(f2_pack(b, a), f2_splat(r));
+  return {s, f2_mul(e, s)};
+}
+__device__ __forceinline__ uint64_t from_40(uint64_t u) {
+  float a, b;
+  f2_unpack(u, a, b);
+  return f2_pack(from_40(a), from_40(b));
 }
 
 template <bool ACT>
 __device__ __forceinline__ uint64_t act2(uint64_t u) {
-  return ACT ? f2_mul(u, sigmoid2(u)) : u;
+  return ACT ? f2_mul(from_40(u), sigmoid2(u).s) : u;
 }
-// d act'(u)
+// d act'(u).  1 - s as E s: its error is relative, so that u (1 - s) vanishes for a large u as it should.
 template <bool ACT>
 __device__ __forceinline__ uint64_t act_grad2(uint64_t u, uint64_t d) {
   if (!ACT) return d;
-  const uint64_t s = sigmoid2(u), one = f2_splat(1.0f);
-  const uint64_t g = f2_fma(u, f2_fma(s, f2_splat(-1.0f), one), one);  // 1 + u (1 - s)
-  return f2_mul(d, f2_mul(s, g));
+  const Sigmoid g = sigmoid2(u);
+  return f2_mul(d, f2_mul(g.s, f2_fma(from_40(u), g.rest, f2_splat(1.0f))));  // s (1 + u (1 - s))
 }
 
 // 0 for what rounding left below it; a NaN stays one

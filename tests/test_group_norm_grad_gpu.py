@@ -257,3 +257,21 @@ def test_atypical_first_rows_of_many_chunks(dtype):
     x = x.to(dtype)
     compare(x, _rand(x.shape, 55, dtype), _rand((64,), 56) * 0.5 + 1, _rand((64,), 57), 32, "swish", [60000],
             packed=False)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("channels", [32, 7])
+def test_swish_far_from_zero(dtype, channels):
+    """u sigmoid(u) of a very negative u is 0 and so is its slope (both below 1e-15 from -40 on); a large u
+    passes with slope 1, whatever its neighbour channel holds."""
+    x, dy = _rand((200, channels), 60, dtype), _rand((200, channels), 61, dtype)
+    w = torch.ones(channels, device=DEV)
+    b = torch.tensor([1e6, 0.3, -1e20, -0.5, -1e4, 1e20, 50.0], device=DEV).repeat(5)[:channels]
+    y, mean, rstd = vae.group_norm_act(x, w, b, 1)
+    dx, dw, db = vae.group_norm_act_backward(dy, x, mean, rstd, w, b)
+    low, high = b < -1000, b > 1000
+    assert (y[:, low].abs() <= 1e-15).all() and (db[low].abs() <= 1e-12).all() and (dw[low].abs() <= 1e-12).all()
+    assert torch.allclose(y[:, high].double(), b[high].double().expand_as(y[:, high]), rtol=2 * U[dtype] + 1e-5)
+    size = dy.double().abs().sum(0)
+    assert ((db.double() - dy.double().sum(0)).abs()[high] <= 1e-6 * size[high]).all()
+    assert torch.isfinite(dx).all()
