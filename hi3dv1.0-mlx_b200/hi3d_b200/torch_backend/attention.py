@@ -4,7 +4,8 @@ Same signatures as the functions the upstream code calls
 (src/sparc3d/nn/sparse/attention/full_attn.py:56-76) and as the reference's CPU shim
 (src/hi3d_mac/torch_backend/attention.py:77-109), including its errors for causal or
 dropout attention.  Inputs are fp16/bf16 CUDA tensors, as for flash-attn itself.  Where a gradient is
-wanted they run the training pair (:mod:`hi3d_b200.training`), so the upstream model can be fine-tuned.
+wanted they run the training pair (:mod:`hi3d_b200.training`): attention and torch's own layers of the
+upstream model train; its sparse convolutions (sparse_conv.py) run forward only and say so in ``backward``.
 """
 
 from __future__ import annotations

@@ -10,6 +10,10 @@ Indices are ``[N, 4]`` int32 ``(batch, x, y, z)``; batches are separated by offs
 voxel neighbours another batch's.  The neighbour table is built on the GPU and cached per
 ``indice_key`` like spconv's indice dict.  Features run in the weight dtype (fp16/bf16 on the
 tensor cores); fp32 weights raise ``NotImplementedError``.
+
+The convolution has no backward pass.  Features that want a gradient give an output through which
+``backward`` raises ``NotImplementedError``, instead of a gradient without the convolution's part; weights
+that want one on features that do not are warned about.
 """
 
 from __future__ import annotations
@@ -17,6 +21,7 @@ from __future__ import annotations
 import enum
 import itertools
 import math
+import warnings
 from typing import Any, Sequence
 
 import torch
@@ -112,6 +117,19 @@ def _indice_data(indices: torch.Tensor, spatial_shape: Sequence[int], kernel_siz
                       ConvAlgo.Native, table=table, tap_mask=_sparse.conv_tap_mask(table, n))
 
 
+class _ForwardOnly(torch.autograd.Function):
+    """The convolution's output, marked as depending on its features."""
+
+    @staticmethod
+    def forward(ctx, out, features):
+        return out.view_as(out)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise NotImplementedError("SubMConv3d has no gradient here: freeze it (requires_grad_(False), under "
+                                  "torch.no_grad() or on detached features) to train what lies around it")
+
+
 class SubMConv3d(nn.Module):
     """Submanifold 3D convolution with spconv's parameter names and ``(out, k, k, k, in)`` layout."""
 
@@ -153,7 +171,13 @@ class SubMConv3d(nn.Module):
             raise NotImplementedError("the B200 sparse convolution runs in float16 or bfloat16")
         data = self._pairs(input)
         x = input.features.to(self.weight.dtype)
-        out = _sparse.conv(x, data.table, self.weight, self.bias, n_in=x.shape[0], tap_mask=data.tap_mask)
+        with torch.no_grad():
+            out = _sparse.conv(x, data.table, self.weight, self.bias, n_in=x.shape[0], tap_mask=data.tap_mask)
+        if torch.is_grad_enabled():
+            if x.requires_grad:
+                out = _ForwardOnly.apply(out, x)
+            elif any(p.requires_grad for p in self.parameters()):
+                warnings.warn("SubMConv3d has no gradient here: its weights will not be trained", stacklevel=2)
         return input.replace_feature(out)
 
 

@@ -140,3 +140,25 @@ def test_example_trains(bits):
     finally:
         ex.training, ex.optim = saved
     assert losses[-1] < 1.2 * plain[-1]
+
+
+def test_a_gradient_through_the_convolution_raises():
+    """The convolution has no backward pass: a training loop learns of it instead of losing the
+    convolution's part of every gradient in silence."""
+    from hi3d_b200.torch_backend import sparse_conv
+
+    idx = torch.tensor([[0, x, y, z] for x in range(3) for y in range(3) for z in range(2)], dtype=torch.int32, device=DEV)
+    conv = sparse_conv.SubMConv3d(16, 16, 3, indice_key="a").to(DEV, torch.float16)
+    x = _rand((idx.shape[0], 16), 30).requires_grad_()
+    run = lambda f: conv(sparse_conv.SparseConvTensor(f, idx, [8, 8, 8], 1)).features  # noqa: E731
+    out = run(x)
+    with torch.no_grad():
+        assert torch.equal(run(x), out) and not run(x).requires_grad
+    with pytest.raises(NotImplementedError, match="gradient"):
+        (x + out).sum().backward()  # a residual block
+    with pytest.warns(UserWarning, match="will not be trained"):
+        assert not run(x.detach()).requires_grad  # as it was
+    conv.requires_grad_(False)
+    assert not run(x.detach()).requires_grad
+    with pytest.raises(NotImplementedError, match="gradient"):
+        run(x).sum().backward()
