@@ -239,6 +239,12 @@ def on_device(t: torch.Tensor):
     return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
+def changed(*ts: torch.Tensor | None) -> None:
+    """Tells autograd that the library wrote into these tensors, as torch's in-place operations do: a backward
+    pass that saved one of them before then raises instead of using the new values."""
+    torch.autograd.graph.increment_version([t for t in ts if t is not None])
+
+
 def require_cuda(*ts: torch.Tensor | None) -> None:
     for t in ts:
         if t is not None and not t.is_cuda:

@@ -100,6 +100,7 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor], exp_avg: t
         dtype=_lib.dtype_code(first), state_bits=8 if eight else 32)
     with _lib.on_device(first):
         _lib.check(_lib.load().hi3d_adamw_step(ctypes.byref(args), _lib.stream(first)), "adamw_step")
+    _lib.changed(*params, exp_avg, exp_avg_sq, master, scales)
 
 
 class _Bucket:

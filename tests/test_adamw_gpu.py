@@ -335,3 +335,19 @@ def test_small_eps_and_tiny_gradients(bits, eps):
     want = w * (1 - lr * HYPER["weight_decay"]) - up
     assert torch.isfinite(f.params[0]).all()
     assert ((f.params[0].double() - want).abs() <= 4 * E * w.abs() + 16 * E * up.abs() + 1e-12).all()
+
+
+def test_a_backward_pass_over_weights_that_a_step_changed_raises():
+    p = torch.nn.Parameter(_rand((16, 16), 51))
+    x = _rand((4, 16), 52).requires_grad_()
+    opt = optim.AdamW([p])
+    y = x @ p
+    y.sum().backward(retain_graph=True)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    f = Flat([(300,)], torch.bfloat16, 8)
+    held = [f.params[0], f.m, f.v, f.master, f.scales]
+    before = [t._version for t in held]
+    f.step(1)
+    assert all(t._version > b for t, b in zip(held, before)) and f.grads[0]._version == 0
