@@ -552,6 +552,7 @@ def _backward(p: _Plan, grad_out, q, k, v, out, lse, cu_q, cu_k, num_seqs: int, 
             given = None
         else:
             (dq, dk, dv), given = _given(grads, (q, k, v), p)
+            _lib.changed(*grads)
         if p.nq == 0 or p.nk == 0 or p.batch == 0 or num_seqs == 0:
             for t in (dq, dk, dv):
                 t.zero_()

@@ -558,3 +558,13 @@ def test_a_nan_key_spoils_every_row_at_any_place():
         out, lse = attention.flash_attention_lse(q, bad, v, 0.125)
         assert out.isnan().all() and lse.isnan().all(), at
         assert attention.flash_attention(q, bad, v, 0.125).isnan().all(), at
+
+
+def test_given_gradient_tensors_count_as_changed():
+    """Autograd's check for tensors changed in place sees the gradients that are written into the caller's."""
+    q, k, v, do = (_rand((1, 2, 20, 64), torch.float16, 121 + i) for i in range(4))
+    out, lse = attention.flash_attention_lse(q, k, v, 0.125)
+    fused = torch.zeros((1, 2, 3, 20, 64), dtype=torch.float16, device=DEV)
+    before = fused._version
+    attention.flash_attention_backward(do.transpose(1, 2).flatten(2), q, k, v, out, lse, 0.125, grads=fused.unbind(2))
+    assert fused._version > before
