@@ -27,6 +27,9 @@ def flash_attn_varlen_qkvpacked_func(qkv: torch.Tensor, cu_seqlens: torch.Tensor
     if causal or dropout_p:
         raise NotImplementedError("causal or dropout attention is not used by Hi3D")
     scale = qkv.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale
+    if scale < 0:
+        return flash_attn_varlen_kvpacked_func(qkv[:, 0], qkv[:, 1:], cu_seqlens.to(qkv.device),
+                                               cu_seqlens.to(qkv.device), max_seqlen, max_seqlen, softmax_scale=scale)
     if _wants_grad(qkv):
         return _train.flash_attn_varlen_qkvpacked(qkv, cu_seqlens.to(qkv.device), int(max_seqlen), scale)
     q, k, v = qkv.unbind(1)
@@ -41,6 +44,8 @@ def flash_attn_varlen_kvpacked_func(q: torch.Tensor, kv: torch.Tensor, cu_seqlen
     if causal or dropout_p:
         raise NotImplementedError("causal or dropout attention is not used by Hi3D")
     scale = q.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale
+    if scale < 0:  # the kernels' masked scores are -inf and have to stay it
+        q, scale = -q, -scale
     if _wants_grad(q, kv):
         return _train.flash_attn_varlen_kvpacked(q, kv, cu_seqlens_q.to(q.device), cu_seqlens_k.to(q.device),
                                                  int(max_seqlen_q), scale)

@@ -162,3 +162,33 @@ def test_a_gradient_through_the_convolution_raises():
     assert not run(x.detach()).requires_grad
     with pytest.raises(NotImplementedError, match="gradient"):
         run(x).sum().backward()
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_flash_attn_module_takes_a_negative_scale(grad):
+    """Scores of the other sign, with and without a gradient, on lengths that end inside a block."""
+    cu, cu_k = (torch.tensor(c, dtype=torch.int32, device=DEV) for c in ([0, 40, 130], [0, 17, 60]))
+    q, kv = _rand((130, 4, 64), 31), _rand((60, 2, 4, 64), 32)
+    qkv, do = _rand((130, 3, 4, 64), 33), _rand((130, 4, 64), 34)
+
+    def plain(q, k, v, cut, cut_k):
+        rows = []
+        for a, b, c, d in zip(cut, cut[1:], cut_k, cut_k[1:]):
+            s, e, f = (t.transpose(0, 1) for t in (q[a:b], k[c:d], v[c:d]))
+            rows.append((torch.softmax(s @ e.mT * -0.2, -1) @ f).transpose(0, 1))
+        return torch.cat(rows)
+
+    for call, leaves, ref in (
+            (lambda q, kv: shim.flash_attn_varlen_kvpacked_func(q, kv, cu, cu_k, 90, 43, softmax_scale=-0.2), (q, kv),
+             lambda q, kv: plain(q, *kv.unbind(1), [0, 40, 130], [0, 17, 60])),
+            (lambda x: shim.flash_attn_varlen_qkvpacked_func(x, cu, 90, softmax_scale=-0.2), (qkv,),
+             lambda x: plain(*x.unbind(1), [0, 40, 130], [0, 40, 130]))):
+        mine = [t.clone().requires_grad_(grad) for t in leaves]
+        theirs = [t.double().requires_grad_() for t in leaves]
+        out, want = call(*mine), ref(*theirs)
+        # one rounding each of the output and of P, 2^-11 at most, checked as 1.5 of them in the 2-norm
+        assert (out.double() - want).norm() <= 1.5 * 2.0 ** -11 * want.norm()
+        assert out.requires_grad == grad
+        if grad:
+            for g, e in zip(torch.autograd.grad(out, mine, do), torch.autograd.grad(want, theirs, do.double())):
+                assert (g.double() - e).norm() <= 1.5 * 2.0 ** -11 * e.norm()
