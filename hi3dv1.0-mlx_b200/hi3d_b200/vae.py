@@ -105,8 +105,9 @@ def _norm_plan(shape, dtype, weight_shape, bias_shape, groups: int, act, eps: fl
     nb = ctypes.c_int64()
     if samples:
         args = _lib.GroupNormArgs(*[16] * 3, 16 if packed else None, *[16] * 7, *sizes)
-        _lib.check(_lib.load().hi3d_group_norm_act_workspace_size(ctypes.byref(args), ctypes.byref(nb)),
-                   "group_norm_act", launched=False)
+        with torch.cuda.device(devices[0]):  # the size follows the device's SM count
+            _lib.check(_lib.load().hi3d_group_norm_act_workspace_size(ctypes.byref(args), ctypes.byref(nb)),
+                       "group_norm_act", launched=False)
     return samples, sizes, nb.value
 
 

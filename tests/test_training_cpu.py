@@ -149,3 +149,29 @@ def test_epilogue_warps_leave_a_wait_together(name):
     src = (REPO / "hi3dv1.0-mlx_b200" / "csrc" / name).read_text()
     waits = re.findall(r"(mbar_wait|warp_wait)\(&bar->acc_full", src)
     assert waits and set(waits) == {"warp_wait"}
+
+
+def test_group_norm_workspace_is_sized_on_the_device_of_x(monkeypatch):
+    """The size follows the SM count of the current device, so the device of x has to be the current one."""
+    current, asked = [0], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            current.append(self.index)
+
+        def __exit__(self, *exc):
+            current.pop()
+
+    class Library:
+        @staticmethod
+        def hi3d_group_norm_act_workspace_size(args, nbytes):
+            asked.append(current[-1])
+            return _lib.OK
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(_lib, "load", Library)
+    vae._norm_plan.__wrapped__((90, 64), torch.float32, (64,), (64,), 8, "swish", 1e-6, None, (3, 3, 3, 3))
+    assert asked == [3] and current == [0]
