@@ -29,7 +29,9 @@
 // addresses travel in the kernel's parameters, so no table is copied to the device and the
 // launch can be captured.  A CTA finds its tensor by a binary search over the first chunks.
 #include <math.h>
+#include <stdlib.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "abi.h"
@@ -379,6 +381,23 @@ static int run(const hi3d_adamw_args* a, const Params& p, cudaStream_t st) {
   return HI3D_OK;
 }
 
+// Whether two tensors' states share a block: two CTAs would write it.
+static bool overlap(const hi3d_adamw_args* a) {
+  int* by_offset = static_cast<int*>(malloc(sizeof(int) * a->count));
+  if (!by_offset) return true;
+  int n = 0;
+  for (int i = 0; i < a->count; ++i)
+    if (a->numels[i] > 0) by_offset[n++] = i;
+  std::sort(by_offset, by_offset + n, [a](int x, int y) { return a->offsets[x] < a->offsets[y]; });
+  bool shared = false;
+  for (int i = 1; i < n && !shared; ++i) {
+    const int64_t blocks = (a->numels[by_offset[i - 1]] + kBlock - 1) / kBlock;
+    shared = a->offsets[by_offset[i]] < a->offsets[by_offset[i - 1]] + blocks * kBlock;
+  }
+  free(by_offset);
+  return shared;
+}
+
 }  // namespace adamw
 }  // namespace hi3d
 
@@ -408,6 +427,8 @@ extern "C" int hi3d_adamw_step(const hi3d_adamw_args* a, void* stream) {
     return set_error(HI3D_ERR_INVALID_ARGUMENT, "adamw_step: %lld state elements, not a multiple of %d",
                      (long long)a->total, kBlock);
   const int size = a->dtype == HI3D_F32 ? 4 : 2;
+  int64_t end = 0;  // of the states so far, while they come in order
+  bool ordered = true;
   for (int i = 0; i < a->count; ++i) {
     const int64_t n = a->numels[i], at = a->offsets[i];
     if (n < 0 || at < 0 || at % kBlock || at > a->total || n > a->total - at)
@@ -416,7 +437,12 @@ extern "C" int hi3d_adamw_step(const hi3d_adamw_args* a, void* stream) {
     const uintptr_t p = reinterpret_cast<uintptr_t>(a->params[i]), g = reinterpret_cast<uintptr_t>(a->grads[i]);
     if (n > 0 && (!p || !g || (p | g) % size))
       return set_error(HI3D_ERR_INVALID_ARGUMENT, "adamw_step: tensor %d: null or misaligned pointer", i);
+    if (n == 0) continue;
+    ordered = ordered && at >= end;
+    end = at + (n + kBlock - 1) / kBlock * kBlock;
   }
+  if (!ordered && overlap(a))
+    return set_error(HI3D_ERR_INVALID_ARGUMENT, "adamw_step: two tensors share state");
   Params p;
   p.count = 0;
   p.master = a->master, p.m = a->exp_avg, p.v = a->exp_avg_sq;

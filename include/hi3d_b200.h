@@ -531,7 +531,8 @@ HI3D_API int hi3d_group_norm_act_bwd(const hi3d_group_norm_args* args, void* wor
  * units in the last place each.  params, grads, numels and offsets are host arrays of `count`;
  * params and grads are device pointers of the given type.  16-bit weights are the rounded copy of
  * `master` (fp32, flat), 32-bit ones have none.  Tensor i's state lies at element offsets[i] (a
- * multiple of HI3D_ADAMW_BLOCK) of the flat buffers of `total` elements, padded with zeros:
+ * multiple of HI3D_ADAMW_BLOCK) of the flat buffers of `total` elements, padded with zeros; no two tensors
+ * share a block:
  *   state_bits 32: exp_avg = m, exp_avg_sq = v, fp32;
  *   state_bits  8: e4m3 codes of m / s and sqrt(v) / s, s = max|.| / 448 of each block of
  *     HI3D_ADAMW_BLOCK values; scales [2][total / HI3D_ADAMW_BLOCK] = s of m, s of sqrt(v).

@@ -351,3 +351,14 @@ def test_a_backward_pass_over_weights_that_a_step_changed_raises():
     before = [t._version for t in held]
     f.step(1)
     assert all(t._version > b for t, b in zip(held, before)) and f.grads[0]._version == 0
+
+
+def test_states_in_another_order():
+    """Offsets that fall, with an empty tensor inside another's state: the same step as in order."""
+    a, b = Flat([(300,), (0,), (256,), (5,)], torch.float32, 32, seed=61), Flat([(300,), (0,), (256,), (5,)],
+                                                                                  torch.float32, 32, seed=61)
+    b.m, b.v = (torch.cat([t[768:], t[512:768], t[:512]]) for t in (b.m, b.v))
+    a.step(3)
+    b.step(3, offsets=[512, 512, 256, 0])
+    assert all(torch.equal(p, q) for p, q in zip(a.params, b.params))
+    assert torch.equal(torch.cat([b.m[512:], b.m[256:512], b.m[:256]]), a.m)

@@ -175,3 +175,10 @@ def test_group_norm_workspace_is_sized_on_the_device_of_x(monkeypatch):
     monkeypatch.setattr(_lib, "load", Library)
     vae._norm_plan.__wrapped__((90, 64), torch.float32, (64,), (64,), 8, "swish", 1e-6, None, (3, 3, 3, 3))
     assert asked == [3] and current == [0]
+
+
+def test_adamw_tensors_that_share_state_are_refused():
+    for numels, offsets in (((300, 5), (0, 256)), ((5, 300), (256, 0)), ((256, 256), (256, 256)), ((1, 256), (0, 0)),
+                            ((5, 0, 300), (512, 0, 256))):
+        ptrs = tuple(16 * (i + 1) for i in range(len(numels)))
+        assert _adamw(numels=numels, offsets=offsets, ptrs=ptrs) == _lib.ERR_INVALID_ARGUMENT, (numels, offsets)
