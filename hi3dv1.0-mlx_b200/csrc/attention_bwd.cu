@@ -246,14 +246,6 @@ __device__ __forceinline__ void tile_range(const int32_t* cu, int b0, int b1, in
   count = max(tile_start(cu, b1, rows) - first, 0);
 }
 
-template <int N>
-__device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&r)[N]) {
-  if constexpr (N == 8)
-    tmem_ld8(taddr, r);
-  else
-    tmem_ld16(taddr, r);
-}
-
 // 32 lanes x 32 fp32 columns, and 32 lanes x 16 columns of packed 16-bit pairs.  BY_COLUMN: a
 // thread holds four rows of eight columns (two halves of 16 lanes), else one row.
 template <bool BY_COLUMN>
@@ -671,11 +663,12 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
         part += (((set * (cu ? 1 : sets) + x_batch) * xheads + h) * rows + x_start + r) * D;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
-          constexpr int W = 32 / kGroups;  // 8 or 16
+          constexpr int W = 32 / kGroups;
+          static_assert(W == 16, "one 16-column load a group");
           const int d0 = c * 32 + group * W;
           uint32_t v[W];
           __syncwarp();
-          load_columns<W>(tmem + lane_addr + C::ACC_COL + w * D + d0, v);
+          tmem_ld16(tmem + lane_addr + C::ACC_COL + w * D + d0, v);
           tmem_wait_ld();
           if (r < x_len) {
             if (partial) {

@@ -340,12 +340,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr));
 }
 
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(taddr));
-}
-
 // 16 TMEM lanes x 4 repetitions of 256 bits (32 columns) -> 16 registers.
 // Thread t holds rows L + t/4 and L + 8 + t/4 (L = the address lane), columns
 // 8k + 2(t%4) and +1 of repetition k: r[4k], r[4k+1] (first row), r[4k+2], r[4k+3].
