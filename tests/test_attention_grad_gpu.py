@@ -568,3 +568,13 @@ def test_given_gradient_tensors_count_as_changed():
     before = fused._version
     attention.flash_attention_backward(do.transpose(1, 2).flatten(2), q, k, v, out, lse, 0.125, grads=fused.unbind(2))
     assert fused._version > before
+
+
+@pytest.mark.parametrize("nq,nk,heads,kv_heads,dim,dtype", [(130, 40000, 2, 1, 64, torch.bfloat16),
+                                                            (40000, 130, 2, 2, 128, torch.float16),
+                                                            (20011, 20011, 1, 1, 64, torch.float16)])
+def test_long_sequences_match_float64(nq, nk, heads, kv_heads, dim, dtype):
+    """Streams of hundreds of blocks, split and whole."""
+    q, do = _rand((1, heads, nq, dim), dtype, 131), _rand((1, heads, nq, dim), dtype, 132)
+    k, v = _rand((1, kv_heads, nk, dim), dtype, 133), _rand((1, kv_heads, nk, dim), dtype, 134)
+    compare(q, k, v, do, dim ** -0.5)
