@@ -119,6 +119,7 @@ struct Barriers {
   uint64_t s_free[2];  // the tile's softmax has read its scores into registers
   uint64_t p_full[2];
   uint64_t o_done[2];
+  uint64_t drained[2];  // after a time-out: the tile's products are done
   uint64_t v_tail;  // LSE: values of a ragged last block, before its rows past the end are cleared
   uint32_t tmem_base;
   int abort;
@@ -254,6 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bar->s_free[i], 4);  // one arrival per softmax warp of the tile
       mbar_init(&bar->p_full[i], kRowsPerTile);
       mbar_init(&bar->o_done[i], 1);
+      mbar_init(&bar->drained[i], 1);
     }
     if constexpr (LSE) mbar_init(&bar->v_tail, 1);
     bar->abort = 0;
@@ -356,24 +358,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_commit(&bar->s_full[i]);
       };
       const int i = warp == 1 ? 0 : 1;
-      bool ok = warp_wait(&bar->q_full, 0, abort, 10) && warp_wait(&bar->k_full[0], 0, abort, 11);
-      if (ok) {
-        tc_fence_after();
-        issue_s(i, 0);
-      }
+      mbar_wait(&bar->q_full, 0, abort, 10);
+      mbar_wait(&bar->k_full[0], 0, abort, 11);
+      tc_fence_after();
+      issue_s(i, 0);
       // Per block j: S_i(j+1) as soon as softmax i has read S_i(j) (s_free), then
       // P_i(j) V once it has published P_i(j).
-      for (int j = 0; ok && j < nblk; ++j) {
+      for (int j = 0; j < nblk; ++j) {
         const int s = j % C::NST, n = j / C::NST;
         const int s1 = (j + 1) % C::NST, n1 = (j + 1) / C::NST;
         if (j + 1 < nblk) {
-          if (!(ok = warp_wait(&bar->k_full[s1], n1 & 1, abort, 11))) break;
-          if (!(ok = warp_wait(&bar->s_free[i], j & 1, abort, 15))) break;
+          mbar_wait(&bar->k_full[s1], n1 & 1, abort, 11);
+          mbar_wait(&bar->s_free[i], j & 1, abort, 15);
           tc_fence_after();
           issue_s(i, s1);
         }
-        if (!(ok = warp_wait(&bar->v_full[s], n & 1, abort, 13))) break;
-        if (!(ok = warp_wait(&bar->p_full[i], j & 1, abort, 14))) break;
+        mbar_wait(&bar->v_full[s], n & 1, abort, 13);
+        mbar_wait(&bar->p_full[i], j & 1, abort, 14);
         tc_fence_after();
         const uint64_t dVs = dV + (uint64_t)((s * C::KV_STAGE) >> 4);
         const uint32_t dO = tm + 256 * i + C::O_COL, aP = tm + 256 * i + C::P_COL;
@@ -387,6 +388,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (j + C::NST < nblk) tc_commit(&bar->kv_empty[s]);
         }
         __syncwarp();
+      }
+      if (__any_sync(0xffffffffu, *abort)) {
+        // products were issued on whatever their buffers held: they end before the CTA's memory goes
+        volatile int no_abort = 0;
+        if (elect_one()) tc_commit(&bar->drained[i]);
+        warp_wait(&bar->drained[i], 0, &no_abort, 16);
       }
     }
   } else {

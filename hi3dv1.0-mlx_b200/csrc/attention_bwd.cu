@@ -116,6 +116,7 @@ struct Barriers {
   uint64_t t_free;    // T is in the compute warps' registers
   uint64_t pd_full[2];
   uint64_t acc_done[2];
+  uint64_t drained[3];  // after a time-out: an issuing warp's products are done
   uint32_t tmem_base;
   int abort;
 };
@@ -347,6 +348,7 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
       mbar_init(&bar->empty[s], 1);
     }
     mbar_init(&bar->tail, 1);
+    for (int i = 0; i < 3; ++i) mbar_init(&bar->drained[i], 1);
     mbar_init(&bar->t_full, 1);
     mbar_init(&bar->t_free, 4 * kGroups);  // one arrival per compute warp
     for (int i = 0; i < 2; ++i) {
@@ -455,21 +457,21 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
           mma_f16_ts(d, a + group * HC + k * 8, dYt + ((y_off + ks * 2048) >> 4), idesc_acc, more || ks > 0 ? 1u : 0u);
         }
       };
-      bool ok = role_id == 2 || warp_wait(C::X2_TMEM ? &bar->x_tmem : &bar->x_full, 0, abort, 310);
-      if (C::X2_TMEM && !C::X1_TMEM && ok && role_id == 0) ok = warp_wait(&bar->x_full, 0, abort, 310);
-      for (int j = 0; ok && j < n; ++j) {
+      if (role_id != 2) mbar_wait(C::X2_TMEM ? &bar->x_tmem : &bar->x_full, 0, abort, 310);
+      if (C::X2_TMEM && !C::X1_TMEM && role_id == 0) mbar_wait(&bar->x_full, 0, abort, 310);
+      for (int j = 0; j < n; ++j) {
         const uint32_t y = (j % NST) * C::STAGE;
-        if (!(ok = warp_wait(&bar->full[j % NST], (j / NST) & 1, abort, 311))) break;
+        mbar_wait(&bar->full[j % NST], (j / NST) & 1, abort, 311);
         if (role_id == 0) {  // S(j), once the products that read P(j - 2), dS(j - 2) from this buffer are done
-          if (j > 1 && !(ok = warp_wait(&bar->acc_done[j & 1], ((j - 2) >> 1) & 1, abort, 314))) break;
+          if (j > 1) mbar_wait(&bar->acc_done[j & 1], ((j - 2) >> 1) & 1, abort, 314);
           tc_fence_after();
           product(X1InTmem(), tm + (j & 1) * BN, dX1, x1_col, y, &bar->s_full[j & 1]);
         } else if (role_id == 1) {  // T(j), once T(j - 1) has been read
-          if (j > 0 && !(ok = warp_wait(&bar->t_free, (j - 1) & 1, abort, 312))) break;
+          if (j > 0) mbar_wait(&bar->t_free, (j - 1) & 1, abort, 312);
           tc_fence_after();
           product(X2InTmem(), tm + C::T_COL, dX2, x2_col, y + C::Y_BYTES, &bar->t_full);
         } else {  // the accumulators, once P(j), dS(j) are written
-          if (!(ok = warp_wait(&bar->pd_full[j & 1], (j >> 1) & 1, abort, 313))) break;
+          mbar_wait(&bar->pd_full[j & 1], (j >> 1) & 1, abort, 313);
           tc_fence_after();
           const uint32_t a = tm + (j & 1) * BN;
           if (elect_one()) {
@@ -480,6 +482,12 @@ __device__ __forceinline__ void role(const CUtensorMap* tmX1, const CUtensorMap*
           }
         }
         __syncwarp();
+      }
+      if (__any_sync(0xffffffffu, *abort)) {
+        // products were issued on whatever their buffers held: they end before the CTA's memory goes
+        volatile int no_abort = 0;
+        if (elect_one()) tc_commit(&bar->drained[role_id]);
+        warp_wait(&bar->drained[role_id], 0, &no_abort, 315);
       }
     }
   } else {

@@ -164,9 +164,10 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
 // A wait may be given up by some lanes of a warp just as its phase completes for the others, and lanes
 // that left while the rest went on to a warp-wide instruction (elect, a shuffle, a TMEM access) would
 // leave those waiting for good.  So no lane leaves by its own result.  warp_wait gives the whole warp
-// one, by a vote.  Compute warps, where a vote on every wait costs 3-6 % of an attention kernel, call
-// mbar_wait for the wait alone and run their loop to its end (once a wait ran out, the others return at
-// once); after it the warp looks at `abort`, which every wait that ran out has set.
+// one, by a vote.  Inner loops, where a vote on every wait costs 3-7 % of an attention kernel, call
+// mbar_wait for the wait alone and run to their end (once a wait ran out, the others return at once);
+// after the loop the warp looks at `abort`, which every wait that ran out has set: what was computed
+// meanwhile is not stored, and an issuing warp waits for the products that it issued.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int where) {
   bool ok = mbar_try_wait(bar, parity);
   if (__all_sync(0xffffffffu, ok)) return true;
