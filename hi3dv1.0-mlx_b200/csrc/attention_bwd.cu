@@ -25,8 +25,8 @@
 // S(j+2) runs when the accumulator products of j are done with its buffer, T(j+1) as soon as T(j)
 // has been read, so a compute warp finds the next block ready.
 //
-// What bounds it.  8192 x 16 x 64 bf16: 878 us, 783 TFLOP/s of the five products that a backward
-// pass cannot do without, 1096 of the seven done (67 % of the measured burst rate, and near the
+// What bounds it.  8192 x 16 x 64 bf16: 895 us, 768 TFLOP/s of the five products that a backward
+// pass cannot do without, 1075 of the seven done (66 % of the measured burst rate, and near the
 // power limit: a sustained loop runs at 1.55-1.7 GHz).  Counters at 4096: tensor pipe 47 %, FMA pipe
 // 49 %, MUFU 34 %, issue 51 %, DRAM 2 %: a scheduler's two compute warps take the exponentials, then
 // the products' elementwise part, in step, so no pipe is busy throughout.  Measured and not kept
@@ -731,7 +731,7 @@ constexpr int kFewKeys = 16;
 // CTAs an SM: the kernel is short and waits for its loads.  8192 x 16 x 64 bf16: eight 8.4 us (32
 // registers, a little spilled), six 11.4, unbounded 15.3.  The form for few keys needs registers:
 // 16384 x 16 queries on 16 keys, the whole pass, four 200 us, five 202, six 211; packed 5873 x 22 x 96
-// fp16, this kernel, 23.2, 21.8, 21.0.
+// fp16, this kernel, 23.2, 21.8, 21.0 (23.6 with five since it also takes its tiles' maxima).
 constexpr int kStatCtas = 8, kFewCtas = 5;
 
 // Row statistics {-L log2e, -delta} in tiles of 128 rows, delta = rowsum(dO O) in fp32.  Over few

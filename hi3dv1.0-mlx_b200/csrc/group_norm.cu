@@ -16,11 +16,12 @@
 // Fixed orders everywhere: no atomics.  A chunk belongs to one sample; sample s begins at chunk
 // offsets[s] / R + s, which covers every sample's rows without a host copy of the offsets.
 //
-// Bound by HBM for fp32 (200k x 256: 282 us for 1.64 GB of passes, 5.8 TB/s, 89 % of the measured
+// Bound by HBM for fp32 (200k x 256: 284 us for 1.64 GB of passes, 5.8 TB/s, 88 % of the measured
 // copy rate): x is read twice forward, x and dy twice backward, y and dx written once with a
-// streaming hint.  In 16 bits (100k x 512 bf16: 171 us for 0.82 GB, 4.8 TB/s) instruction issue
-// (54-60 %) and the MUFU unit come close beside it.  A floor of one reading each (62 and 125 us)
-// would need the chunks to stay on chip between the passes; they are 3 to 7 times what L2 keeps.
+// streaming hint.  In 16 bits (100k x 512 bf16: 174 us for 0.82 GB, 4.7 TB/s) instruction issue
+// (57-61 %) and the MUFU unit come close beside it.  A floor of one reading each (62 and 125 us)
+// would need x, and backward dy beside it, to stay on chip between the passes: 102 and 205 MB each,
+// where L2 has 126 MB for all that passes through it.
 #include <type_traits>
 
 #include "abi.h"
